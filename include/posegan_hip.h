@@ -309,6 +309,22 @@ int pg_warp_mask_max_bwd(const float* gout, const uint8_t* argmax, const float* 
                          int32_t N, int32_t T, int32_t C, int32_t h, int32_t w, int32_t H0, int32_t W0,
                          int32_t align_corners, float* dfeat, void* stream);
 
+/* ---- root-mean-square norm along the channels of rows (NHWC pixels), with the residual's addition and an 8-bit output
+ *   h = rnd(x + res),  s = 1 / sqrt(mean_c h^2 + eps),  y = h s gamma          io_flags 0: x, res, h, y fp32; 3: bf16 (gamma, rstd fp32)
+ * x [rows][C] with row stride ldx, res (NULL: none) ldr, y (NULL: not written) ldy; h (NULL: not written), q packed [rows][C].
+ * q (NULL: none): e4m3 bytes of y / scale, scale = max|y| / 448 of a group of `group` channels (32, 64, 128, 256; 0: of the row; the last
+ * group may be short), 1 where the group is all zero; scales [rows][ceil(C / group)].  rstd (NULL: none) [rows] = s, for the backward
+ * pass.  h may be x or res, y may be x, res or h (row strides equal) for C <= 2048; a NaN stays in its row.                       */
+int pg_rms_norm_fwd(const void* x, const void* res, const float* gamma, int64_t rows, int32_t C, int64_t ldx, int64_t ldr, float eps,
+                    int32_t io_flags, void* h, void* y, int64_t ldy, void* q, float* scales, int32_t group, float* rstd, void* stream);
+/* backward: dx (= the residual's gradient) = s (w - h s mean_c(w h s)) + dh with w = dy gamma; dgamma[c] (+)= sum_rows dy h s.  dy has row
+ * stride lddy; dh (the gradient that reaches h past the norm; NULL: none), h, dx packed.  dx may be dy (lddy == C), dh or h for C <= 2048.
+ * No atomics.  workspace: pg_rms_norm_bwd_workspace bytes.                                                                      */
+int64_t pg_rms_norm_bwd_workspace(int64_t rows, int32_t C, int32_t io_flags);
+int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, const void* h, const float* rstd, const float* gamma, int64_t rows,
+                    int32_t C, int32_t io_flags, void* dx, float* dgamma, int32_t accumulate, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
 /* ---- losses (models/pose_gan.py)
  * GAN log loss on D logits [rows][K] (sigmoid fused; pose_gan.py:90-98,140-160):
  *   mode 0: -log(sigmoid(x)+1e-7) (real / generator), mode 1: -log(1-sigmoid(x)+1e-7) (fake);
@@ -343,6 +359,54 @@ int pg_adam(float* p, const float* g, float* m, float* v, int64_t n, float b1, f
  * K-contiguous weight operand of the bf16 data path (the arena's packed [tap][Cout][Cin] layout).  n % 4 == 0.          */
 int pg_adam_ex(float* p, const float* g, const void* g_bf16, float* m, float* v, int64_t n, float b1, float b2, float eps,
                float step_size, float bc2_sqrt, float grad_scale, void* p_bf16, void* stream);
+
+/* ---- matrix optimiser
+ * Orthogonalisation by Newton-Schulz products: out = X_steps, X_0 = x / (|x|_F + eps), X_{k+1} = (aI + bA + cA^2) X_k, A = X_k X_k^T
+ * on the short side, (a, b, c) = (3.4445, -4.7750, 2.0315): the singular values of x go to within 0.68 .. 1.21.  `batch` matrices of
+ * rows x cols, row strides ldx / ldo, matrix strides x_batch / out_batch (elements); x and out fp32 or bf16 each (x may be read
+ * by several matrices, out must not overlap itself or x).  Products have fp32 accuracy whatever the types.  A matrix with an
+ * infinity or NaN gives NaN, without effect on the others; a zero matrix gives zeros.  steps 1..32, eps > 0, at most 2^31 - 1 elements a matrix.
+ * The workspace (pg_orthogonalise_workspace bytes, 256-byte aligned; -1: sizes out of range) is the call's until its work is done.  */
+int64_t pg_orthogonalise_workspace(int64_t batch, int64_t rows, int64_t cols);
+int pg_orthogonalise(const void* x, int32_t x_is_bf16, int64_t batch, int64_t rows, int64_t cols, int64_t x_batch, int64_t ldx,
+                     void* out, int32_t out_is_bf16, int64_t out_batch, int64_t ldo, int32_t steps, float eps,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+/* One parameter tensor of a flat arena.  kind 0: a matrix [rows, taps * cols] stored [taps][rows][cols] (a packed convolution weight: rows =
+ * Cout, cols = Cin) that the Muon step updates; kind 1: anything else, updated by Adam (taps * rows * cols elements).       */
+typedef struct {
+  int64_t off;                 /* first element in the arena */
+  int32_t taps, rows, cols;
+  int32_t kind;
+  float scale;                 /* kind 0: factor of the orthogonal update, e.g. 0.2 sqrt(max(rows, taps * cols)) for an rms of 0.2 */
+  int32_t _pad;
+} pg_muon_entry_t;
+/* The optimiser step of every tensor of an arena (entries in ascending, disjoint order, a HOST array read during the call):
+ *   kind 0: m = momentum m + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum m : m;
+ *           p = p (1 - lr weight_decay) - lr scale orthogonalise(u)
+ *   kind 1: Adam with (beta1, beta2, adam_eps), the step number `step` (+ *ctr if ctr is given: replay-safe, as pg_adam_ctr)
+ * g: fp32 gradients, or g_bf16 (read instead if given), times grad_scale; p_bf16 (optional): bf16 copy of the updated parameters.       */
+typedef struct {
+  float* p;
+  const float* g;
+  const void* g_bf16;
+  float* m;
+  float* v;                    /* Adam's second moment; NULL only without kind 1 entries */
+  void* p_bf16;
+  const pg_muon_entry_t* entries;
+  int64_t total;               /* elements of the arena */
+  int32_t n;
+  int32_t nesterov, steps;
+  float lr, momentum, weight_decay, grad_scale, eps;   /* eps: the orthogonalisation's */
+  double beta1, beta2;
+  float adam_eps;
+  int32_t _pad;
+  int64_t step;
+  const uint64_t* ctr;
+  void* workspace;             /* pg_muon_workspace bytes, 256-byte aligned */
+  int64_t workspace_bytes;
+} pg_muon_t;
+int64_t pg_muon_workspace(const pg_muon_entry_t* entries, int32_t n);
+int pg_muon_step(const pg_muon_t* d, void* stream);
 
 /* ---- replay-safe scalars (HIP-graph capture of the iteration, runtime/graph.py): a captured graph freezes kernel
  * arguments, so the two per-iteration scalars of the step — the dropout key and Adam's step number — come from a device

@@ -1,0 +1,566 @@
+// Root-mean-square norm along the channels of NHWC pixels (rows), with the residual's addition in front of it and an optional
+// 8-bit output behind it, gfx950.  The per-sample norm of the reference's blocks (norm.hip) has one scalar gain and statistics over
+// (C,H,W); here every row (pixel) has its own scale and every channel its own gain:
+//   h = rnd_T(x + r),  s = 1 / sqrt(mean_c h^2 + eps),  y = h s gamma
+//   backward:  xh = h s,  w = dy gamma:  dx = dr = s (w - xh mean_c(w xh)) + dh,   dgamma = sum_rows dy xh
+// where dh is the gradient that reaches h past the norm (the residual stream).  Statistics and sums are fp32 (dgamma's last sum fp64);
+// the only roundings to fewer bits are the stores: T (fp32 or bf16) and e4m3.
+// Both passes are HBM-bound (6 / 12 flops per element).  A row lives in the registers of a group of LPR lanes (the smallest
+// power of two that covers it in one 16-byte chunk per lane, then several chunks per lane of a whole wave): ONE read of every input,
+// statistics by lane exchanges, no LDS and no barrier.  16-byte accesses at any element alignment (gfx950 global memory takes
+// them); the last chunk of a row whose length is no multiple of 8 (bf16) / 4 (fp32) goes element by element.  Rows longer than the
+// registers hold take a workgroup each and read their inputs twice.
+#include "common.h"
+
+namespace pg {
+
+typedef unsigned short bf16_t;
+
+__device__ __forceinline__ unsigned rms_pack_bf16(float lo, float hi) {
+  unsigned r;
+  asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
+  return r;
+}
+__device__ __forceinline__ float rms_ld1(const float* p) { return *p; }
+__device__ __forceinline__ float rms_ld1(const bf16_t* p) { return __uint_as_float((unsigned)*p << 16); }
+__device__ __forceinline__ void rms_st1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void rms_st1(bf16_t* p, float v) { *p = (bf16_t)(rms_pack_bf16(v, 0.f) & 0xffffu); }
+__device__ __forceinline__ float rms_round(float v, const float*) { return v; }
+__device__ __forceinline__ float rms_round(float v, const bf16_t*) { return __uint_as_float(rms_pack_bf16(v, 0.f) << 16); }
+
+struct __attribute__((packed, aligned(2))) RmsU4 { unsigned x, y, z, w; };     // 16 bytes at the alignment of one element
+struct __attribute__((packed, aligned(4))) RmsF4 { float x, y, z, w; };
+struct __attribute__((packed, aligned(1))) RmsB8 { unsigned x, y; };
+struct __attribute__((packed, aligned(1))) RmsB4 { unsigned x; };
+
+template <typename T> struct RmsV { static constexpr int N = 16 / (int)sizeof(T); };
+
+// the chunk of RmsV<T>::N elements that starts at column c of a row of C elements; zero behind the row's end
+template <typename T>
+__device__ __forceinline__ void rms_load(const T* row, int c, int C, float (&v)[RmsV<T>::N]) {
+  constexpr int V = RmsV<T>::N;
+  if (c + V <= C) {
+    const RmsU4 u = *reinterpret_cast<const RmsU4*>(row + c);
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (V == 4) v[e] = __uint_as_float(w[e]);
+      else { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (c + e < C) ? rms_ld1(row + c + e) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void rms_store(T* row, int c, int C, const float (&v)[RmsV<T>::N]) {
+  constexpr int V = RmsV<T>::N;
+  if (c + V <= C) {
+    RmsU4 u;
+    if constexpr (V == 4) {
+      u.x = __float_as_uint(v[0]); u.y = __float_as_uint(v[1]); u.z = __float_as_uint(v[2]); u.w = __float_as_uint(v[3]);
+    } else {
+      u.x = rms_pack_bf16(v[0], v[1]); u.y = rms_pack_bf16(v[2], v[3]); u.z = rms_pack_bf16(v[4], v[5]); u.w = rms_pack_bf16(v[6], v[7]);
+    }
+    *reinterpret_cast<RmsU4*>(row + c) = u;
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (c + e < C) rms_st1(row + c + e, v[e]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void rms_gain(const float* g, int c, int C, float (&v)[V]) {
+  if (c + V <= C) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      const RmsF4 f = *reinterpret_cast<const RmsF4*>(g + c + 4 * q);
+      v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (c + e < C) ? g[c + e] : 0.f;
+  }
+}
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v, int lpr = LPR) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// 8 bits: q = e4m3(448 z / max|z|), z = h gamma of a group, in fp64 and rounded to fp32 once: the row's s cancels, and a
+// value next to a border of e4m3's steps goes to the side that the definition gives (in fp32, with y and the scale rounded first,
+// one value in 500 000 changed sides).  scale = s max|z| / 448.  s joins in so that a row whose statistic is NaN is NaN.
+struct Q8 {
+  double r;
+  float scale;
+  __device__ __forceinline__ Q8(double am, float s) {
+    r = am > 0.0 ? 448.0 / am : 0.0;
+    scale = am > 0.0 ? (float)((double)s * am / 448.0) : 1.f;
+    if (s != s) { r = (double)s; scale = s; }
+  }
+};
+// round to nearest even; |t| <= 448 up to the rounding of the quotient, which the comparison takes off; NaN stays NaN
+__device__ __forceinline__ float q8_clip(float t) { return t > 448.f ? 448.f : (t < -448.f ? -448.f : t); }
+template <int V>
+__device__ __forceinline__ void q8_store(uint8_t* row, int c, int C, const float (&h)[V], const float (&g)[V], const Q8& k) {
+  unsigned w[V / 4];
+  float t[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) t[e] = q8_clip((float)((double)h[e] * (double)g[e] * k.r));
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) {
+    int p = 0;
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * q], t[4 * q + 1], p, false);
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * q + 2], t[4 * q + 3], p, true);
+    w[q] = (unsigned)p;
+  }
+  if (c + V <= C) {
+    if constexpr (V == 8) { RmsB8 b; b.x = w[0]; b.y = w[1]; *reinterpret_cast<RmsB8*>(row + c) = b; }
+    else { RmsB4 b; b.x = w[0]; *reinterpret_cast<RmsB4*>(row + c) = b; }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (c + e < C) row[c + e] = (uint8_t)(w[e / 4] >> (8 * (e & 3)));
+  }
+}
+template <int V>
+__device__ __forceinline__ double abs_max(const float (&h)[V], const float (&g)[V]) {
+  double m = 0.0;
+#pragma unroll
+  for (int e = 0; e < V; ++e) m = fmax(m, fabs((double)h[e] * (double)g[e]));
+  return m;
+}
+
+struct RmsFwdK {
+  const void* x; const void* res; const float* gamma;
+  long rows; int C; long ldx, ldr, ldy; float eps;
+  void* h; void* y; uint8_t* q; float* scales; int group, ngroups; float* rstd;
+};
+
+// Q: 0 = no 8-bit output, 1 = one scale per row, 2 = one scale per `group` channels (group / V a power of two <= LPR: host)
+template <typename T, int LPR, int NCH, int Q>
+__global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdK p) {
+  constexpr int V = RmsV<T>::N;
+  const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (row >= p.rows) return;
+  const int ln = threadIdx.x % LPR;
+  const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
+  float h[NCH][V];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) rms_load(x, (i * LPR + ln) * V, p.C, h[i]);
+  if (p.res) {
+    const T* r = reinterpret_cast<const T*>(p.res) + row * p.ldr;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      float t[V];
+      rms_load(r, (i * LPR + ln) * V, p.C, t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) h[i][e] = rms_round(h[i][e] + t[e], x);
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+  ss = group_sum<LPR>(ss);
+  const float s = 1.f / sqrtf(ss / (float)p.C + p.eps);
+  if (p.h) {
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) rms_store(reinterpret_cast<T*>(p.h) + row * p.C, (i * LPR + ln) * V, p.C, h[i]);
+  }
+  if (p.rstd && ln == 0) p.rstd[row] = s;
+  float g[NCH][V];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    rms_gain<V>(p.gamma, (i * LPR + ln) * V, p.C, g[i]);
+    if (p.y) {
+      float y[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] = h[i][e] * s * g[i][e];
+      rms_store(reinterpret_cast<T*>(p.y) + row * p.ldy, (i * LPR + ln) * V, p.C, y);
+    }
+  }
+  if constexpr (Q != 0) {
+    double am[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) am[i] = abs_max<V>(h[i], g[i]);
+    if constexpr (Q == 1) {
+#pragma unroll
+      for (int i = 1; i < NCH; ++i) am[0] = fmax(am[0], am[i]);
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) am[0] = fmax(am[0], __shfl_xor(am[0], o, 64));
+      const Q8 k(am[0], s);
+      if (ln == 0) p.scales[row] = k.scale;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) q8_store<V>(p.q + row * p.C, (i * LPR + ln) * V, p.C, h[i], g[i], k);
+    } else {
+      const int gl = p.group / V;                       // lanes of a group
+      for (int o = gl >> 1; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) am[i] = fmax(am[i], __shfl_xor(am[i], o, 64));
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const int c = (i * LPR + ln) * V;
+        const Q8 k(am[i], s);
+        if ((ln & (gl - 1)) == 0 && c < p.C) p.scales[row * p.ngroups + c / p.group] = k.scale;
+        q8_store<V>(p.q + row * p.C, c, p.C, h[i], g[i], k);
+      }
+    }
+  }
+}
+
+// rows that do not fit a wave's registers: a workgroup per row, inputs read twice
+__device__ __forceinline__ double block_sum_d(double v, double* red) {
+  v = wave_sum_d(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return red[0] + red[1] + red[2] + red[3];
+}
+__device__ __forceinline__ double block_max_d(double v, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmax(fmax(red[0], red[1]), fmax(red[2], red[3]));
+}
+template <typename T>
+__device__ __forceinline__ void rms_sum_chunk(const T* x, const T* r, int c, int C, float (&h)[RmsV<T>::N]) {
+  rms_load(x, c, C, h);
+  if (r) {
+    float t[RmsV<T>::N];
+    rms_load(r, c, C, t);
+#pragma unroll
+    for (int e = 0; e < RmsV<T>::N; ++e) h[e] = rms_round(h[e] + t[e], x);
+  }
+}
+template <typename T, int Q>
+__global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwdK p) {
+  constexpr int V = RmsV<T>::N;
+  __shared__ double red[4];
+  const long row = blockIdx.x;
+  const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
+  const T* r = p.res ? reinterpret_cast<const T*>(p.res) + row * p.ldr : nullptr;
+  double ss = 0.0;
+  for (long c = (long)threadIdx.x * V; c < p.C; c += 256 * V) {
+    float h[V];
+    rms_sum_chunk(x, r, (int)c, p.C, h);
+    float a = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) a = fmaf(h[e], h[e], a);
+    ss += (double)a;
+  }
+  const float s = (float)(1.0 / sqrt(block_sum_d(ss, red) / (double)p.C + (double)p.eps));
+  if (p.rstd && threadIdx.x == 0) p.rstd[row] = s;
+  double am = 0.0;
+  for (long c = (long)threadIdx.x * V; c < p.C; c += 256 * V) {
+    float h[V], g[V];
+    rms_sum_chunk(x, r, (int)c, p.C, h);
+    if (p.h) rms_store(reinterpret_cast<T*>(p.h) + row * p.C, (int)c, p.C, h);
+    rms_gain<V>(p.gamma, (int)c, p.C, g);
+    if constexpr (Q == 1) am = fmax(am, abs_max<V>(h, g));
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[e] = h[e] * s * g[e];
+    if (p.y) rms_store(reinterpret_cast<T*>(p.y) + row * p.ldy, (int)c, p.C, h);
+  }
+  if constexpr (Q != 0) {
+    if constexpr (Q == 1) {
+      am = block_max_d(am, red);
+      if (threadIdx.x == 0) p.scales[row] = Q8(am, s).scale;
+    }
+    // groups: the chunks of a group belong to consecutive lanes of one wave; every lane of a wave makes every trip
+    const long trips = ((long)p.C + 256 * V - 1) / (256 * V);
+    for (long t = 0; t < trips; ++t) {
+      const long cl = (t * 256 + threadIdx.x) * V;
+      const int c = cl < p.C ? (int)cl : p.C;
+      float h[V], g[V];
+      rms_sum_chunk(x, r, c, p.C, h);
+      rms_gain<V>(p.gamma, c, p.C, g);
+      if constexpr (Q == 2) {
+        am = abs_max<V>(h, g);
+        const int gl = p.group / V;
+        for (int o = gl >> 1; o > 0; o >>= 1) am = fmax(am, __shfl_xor(am, o, 64));
+        if ((threadIdx.x & (gl - 1)) == 0 && c < p.C) p.scales[row * p.ngroups + c / p.group] = Q8(am, s).scale;
+      }
+      if (c < p.C) q8_store<V>(p.q + row * p.C, c, p.C, h, g, Q8(am, s));
+    }
+  }
+}
+
+struct RmsBwdK {
+  const void* dy; const void* dh; const void* h; const float* rstd; const float* gamma;
+  long rows; int C; long lddy;
+  void* dx; float* part; float* dgamma; int accumulate;
+};
+
+// A group of LPR lanes walks rows; every lane keeps the dgamma sums of its own columns in registers, the workgroup's groups are
+// joined in LDS, the workgroups by rms_dgamma_kernel (one workgroup: written here).  No atomics: the order is fixed.
+template <typename T, int LPR, int NCH>
+__global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdK p) {
+  constexpr int V = RmsV<T>::N, G = 256 / LPR;
+  __shared__ float red[256 * NCH * V];
+  const int ln = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+  float acc[NCH][V], gain[NCH][V];
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    rms_gain<V>(p.gamma, (i * LPR + ln) * V, p.C, gain[i]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[i][e] = 0.f;
+  }
+  for (long row = (long)blockIdx.x * G + grp; row < p.rows; row += (long)gridDim.x * G) {
+    const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.lddy;
+    const T* h = reinterpret_cast<const T*>(p.h) + row * p.C;
+    float a[NCH][V], b[NCH][V], d[NCH][V];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) { rms_load(dy, (i * LPR + ln) * V, p.C, a[i]); rms_load(h, (i * LPR + ln) * V, p.C, b[i]); }
+    if (p.dh) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) rms_load(reinterpret_cast<const T*>(p.dh) + row * p.C, (i * LPR + ln) * V, p.C, d[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[i][e] = 0.f;
+    }
+    const float s = p.rstd[row];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        b[i][e] *= s;                                        // xh
+        acc[i][e] = fmaf(a[i][e], b[i][e], acc[i][e]);
+        a[i][e] *= gain[i][e];                               // w
+        dot = fmaf(a[i][e], b[i][e], dot);
+      }
+    dot = group_sum<LPR>(dot) / (float)p.C;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) a[i][e] = (a[i][e] - b[i][e] * dot) * s + d[i][e];
+      rms_store(reinterpret_cast<T*>(p.dx) + row * p.C, (i * LPR + ln) * V, p.C, a[i]);
+    }
+  }
+  // red[group][column]
+#pragma unroll
+  for (int i = 0; i < NCH; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) red[(grp * NCH + i) * LPR * V + ln * V + e] = acc[i][e];
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.C; c += 256) {
+    float t = 0.f;
+    for (int k = 0; k < G; ++k) t += red[k * NCH * LPR * V + c];
+    if (gridDim.x == 1) p.dgamma[c] = p.accumulate ? p.dgamma[c] + t : t;
+    else p.part[(long)blockIdx.x * p.C + c] = t;
+  }
+}
+
+// dgamma[c] = sum of nblk partial rows: 32 columns x 32 slices per workgroup, fp64
+__global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* part, int nblk, int C, float* dgamma, int accumulate) {
+  __shared__ double red[32][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), sl = threadIdx.x >> 5;
+  double t = 0.0;
+  if (c < C) {
+#pragma unroll 8
+    for (int k = sl; k < nblk; k += 32) t += (double)part[(long)k * C + c];
+  }
+  red[sl][threadIdx.x & 31] = t;
+  __syncthreads();
+  if (threadIdx.x < 32 && c < C) {
+    double a = 0.0;
+    for (int k = 0; k < 32; ++k) a += red[k][threadIdx.x];
+    dgamma[c] = (float)(accumulate ? (double)dgamma[c] + a : a);
+  }
+}
+
+// long rows: dx by a workgroup per row ...
+template <typename T>
+__global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwdK p) {
+  constexpr int V = RmsV<T>::N;
+  __shared__ double red[4];
+  const long row = blockIdx.x;
+  const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.lddy;
+  const T* h = reinterpret_cast<const T*>(p.h) + row * p.C;
+  const T* dh = p.dh ? reinterpret_cast<const T*>(p.dh) + row * p.C : nullptr;
+  const float s = p.rstd[row];
+  double dot = 0.0;
+  for (long c = (long)threadIdx.x * V; c < p.C; c += 256 * V) {
+    float a[V], b[V], g[V], t = 0.f;
+    rms_load(dy, (int)c, p.C, a); rms_load(h, (int)c, p.C, b);
+    rms_gain<V>(p.gamma, (int)c, p.C, g);
+#pragma unroll
+    for (int e = 0; e < V; ++e) t = fmaf(a[e] * g[e], b[e] * s, t);
+    dot += (double)t;
+  }
+  const float m = (float)(block_sum_d(dot, red) / (double)p.C);
+  for (long c = (long)threadIdx.x * V; c < p.C; c += 256 * V) {
+    float a[V], b[V], g[V], d[V];
+    rms_load(dy, (int)c, p.C, a); rms_load(h, (int)c, p.C, b);
+    rms_gain<V>(p.gamma, (int)c, p.C, g);
+    if (dh) rms_load(dh, (int)c, p.C, d);
+    else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) a[e] = (a[e] * g[e] - b[e] * s * m) * s + d[e];
+    rms_store(reinterpret_cast<T*>(p.dx) + row * p.C, (int)c, p.C, a);
+  }
+}
+// ... and dgamma's partial sums by column strips (256 columns) x row ranges
+template <typename T>
+__global__ __launch_bounds__(256) void rms_dgamma_long_kernel(const RmsBwdK p) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= p.C) return;
+  const T* dy = reinterpret_cast<const T*>(p.dy) + c;
+  const T* h = reinterpret_cast<const T*>(p.h) + c;
+  double t = 0.0;
+  for (long row = blockIdx.y; row < p.rows; row += gridDim.y)
+    t += (double)(rms_ld1(dy + row * p.lddy) * (rms_ld1(h + row * p.C) * p.rstd[row]));
+  p.part[(long)blockIdx.y * p.C + c] = (float)t;
+}
+
+// lanes and chunks per lane that hold a row of C elements (V per chunk); nch = 0: it takes the long-row form
+static void rms_shape(int C, int V, int group, int& lpr, int& nch) {
+  lpr = 8;
+  while (lpr < 64 && (lpr * V < C || lpr * V < group)) lpr *= 2;
+  nch = 1;
+  while (nch * lpr * V < C) nch *= 2;
+  if (nch * V > 32) nch = 0;
+}
+static long rms_bwd_blocks(long rows, int lpr) {
+  const long g = 256 / lpr;
+  long b = (rows + g - 1) / g;
+  // few rows: one workgroup that writes dgamma itself; otherwise at least two rows per group, at most 4 workgroups per CU
+  if (b <= 16) return 1;
+  b = (b + 1) / 2;
+  return b > 1024 ? 1024 : b;
+}
+static int rms_long_slices(long rows) { return rows < 64 ? (int)rows : 64; }
+
+}  // namespace pg
+
+using namespace pg;
+
+extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamma, int64_t rows, int32_t C, int64_t ldx, int64_t ldr,
+                               float eps, int32_t io_flags, void* h, void* y, int64_t ldy, void* q, float* scales, int32_t group,
+                               float* rstd, void* stream) {
+  PG_REQUIRE(x && gamma && rows >= 0 && C > 0 && ldx >= C && eps >= 0.f, "pg_rms_norm_fwd: x, gamma, rows >= 0, C > 0 and ldx >= C required");
+  PG_REQUIRE(io_flags == 0 || io_flags == 3, "pg_rms_norm_fwd: io_flags 0 (fp32) or 3 (bf16)");
+  PG_REQUIRE(y || q || h, "pg_rms_norm_fwd: nothing to write (y, q and h are all NULL)");
+  PG_REQUIRE(!res || ldr >= C, "pg_rms_norm_fwd: ldr >= C required");
+  PG_REQUIRE(!y || ldy >= C, "pg_rms_norm_fwd: ldy >= C required");
+  PG_REQUIRE(!q || scales, "pg_rms_norm_fwd: an 8-bit output needs `scales`");
+  PG_REQUIRE(!q || group == 0 || group == 32 || group == 64 || group == 128 || group == 256,
+             "pg_rms_norm_fwd: group 0 (a scale per row), 32, 64, 128 or 256 channels");
+  const size_t em = io_flags ? 1 : 3;
+  PG_REQUIRE((((size_t)x | (size_t)res | (size_t)h | (size_t)y) & em) == 0 && (((size_t)gamma | (size_t)scales | (size_t)rstd) & 3) == 0,
+             "pg_rms_norm_fwd: a pointer is not aligned to its element");
+  if (rows == 0) return 0;
+  const int V = io_flags ? 8 : 4;
+  const int grp = q ? group : 0;
+  const int Q = !q ? 0 : (group == 0 ? 1 : 2);
+  int lpr, nch;
+  rms_shape(C, V, grp, lpr, nch);
+  const long blocks = nch ? (rows + 256 / lpr - 1) / (256 / lpr) : rows;
+  PG_REQUIRE(blocks < (1L << 31), "pg_rms_norm_fwd: too many rows");
+  PG_REQUIRE(nch || ((h == nullptr || (h != x && h != res)) && (y == nullptr || (y != x && y != res && y != h))),
+             "pg_rms_norm_fwd: rows of more than 2048 channels are read twice: outputs must not be inputs");
+  PG_REQUIRE((h == nullptr || ((h != x || ldx == C) && (h != res || ldr == C))) &&
+             (y == nullptr || ((y != x || ldy == ldx) && (y != res || ldy == ldr) && (y != h || ldy == C))),
+             "pg_rms_norm_fwd: an output in place of an input needs the same row stride");
+  RmsFwdK k = {x, res, gamma, (long)rows, C, (long)ldx, (long)ldr, (long)ldy, eps, h, y, (uint8_t*)q, scales, group,
+               group ? (C + group - 1) / group : 1, rstd};
+  hipStream_t st = (hipStream_t)stream;
+#define PG_RF1(T, L, N)                                                                                            \
+  do {                                                                                                             \
+    if (Q == 0) PG_KLAUNCH((rms_fwd_kernel<T, L, N, 0>), dim3((unsigned)blocks), dim3(256), 0, st, k);             \
+    else if (Q == 1) PG_KLAUNCH((rms_fwd_kernel<T, L, N, 1>), dim3((unsigned)blocks), dim3(256), 0, st, k);        \
+    else PG_KLAUNCH((rms_fwd_kernel<T, L, N, 2>), dim3((unsigned)blocks), dim3(256), 0, st, k);                    \
+  } while (0)
+#define PG_RFL(T)                                                                                                  \
+  do {                                                                                                             \
+    if (Q == 0) PG_KLAUNCH((rms_fwd_long_kernel<T, 0>), dim3((unsigned)blocks), dim3(256), 0, st, k);              \
+    else if (Q == 1) PG_KLAUNCH((rms_fwd_long_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, st, k);         \
+    else PG_KLAUNCH((rms_fwd_long_kernel<T, 2>), dim3((unsigned)blocks), dim3(256), 0, st, k);                     \
+  } while (0)
+#define PG_RF(T)                                                                                                   \
+  do {                                                                                                             \
+    if (nch == 0) PG_RFL(T);                                                                                       \
+    else if (lpr == 8) PG_RF1(T, 8, 1);                                                                            \
+    else if (lpr == 16) PG_RF1(T, 16, 1);                                                                          \
+    else if (lpr == 32) PG_RF1(T, 32, 1);                                                                          \
+    else if (nch == 1) PG_RF1(T, 64, 1);                                                                           \
+    else if (nch == 2) PG_RF1(T, 64, 2);                                                                           \
+    else if (nch == 4) PG_RF1(T, 64, 4);                                                                           \
+    else PG_RF1(T, 64, 32 / RmsV<T>::N);                                                                           \
+  } while (0)
+  if (io_flags == 0) PG_RF(float);
+  else PG_RF(bf16_t);
+#undef PG_RF
+#undef PG_RFL
+#undef PG_RF1
+  PG_LAUNCH_OK("pg_rms_norm_fwd");
+  return 0;
+}
+
+extern "C" int64_t pg_rms_norm_bwd_workspace(int64_t rows, int32_t C, int32_t io_flags) {
+  if (rows <= 0 || C <= 0) return 0;
+  int lpr, nch;
+  rms_shape(C, io_flags ? 8 : 4, 0, lpr, nch);
+  const long nb = nch ? rms_bwd_blocks(rows, lpr) : rms_long_slices(rows);
+  return nch && nb == 1 ? 0 : (int64_t)nb * C * 4;
+}
+
+extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, const void* h, const float* rstd, const float* gamma,
+                               int64_t rows, int32_t C, int32_t io_flags, void* dx, float* dgamma, int32_t accumulate,
+                               void* workspace, int64_t workspace_bytes, void* stream) {
+  PG_REQUIRE(dy && h && rstd && gamma && dx && dgamma && rows >= 0 && C > 0 && lddy >= C,
+             "pg_rms_norm_bwd: dy, h, rstd, gamma, dx, dgamma, rows >= 0, C > 0 and lddy >= C required");
+  PG_REQUIRE(io_flags == 0 || io_flags == 3, "pg_rms_norm_bwd: io_flags 0 (fp32) or 3 (bf16)");
+  const size_t em = io_flags ? 1 : 3;
+  PG_REQUIRE((((size_t)dy | (size_t)dh | (size_t)h | (size_t)dx) & em) == 0 &&
+             (((size_t)gamma | (size_t)rstd | (size_t)dgamma | (size_t)workspace) & 3) == 0,
+             "pg_rms_norm_bwd: a pointer is not aligned to its element");
+  const int64_t need = pg_rms_norm_bwd_workspace(rows, C, io_flags);
+  PG_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "pg_rms_norm_bwd: workspace of %lld bytes required", (long long)need);
+  hipStream_t st = (hipStream_t)stream;
+  if (rows == 0) {                 // an empty sum
+    if (!accumulate) PG_KLAUNCH(rms_dgamma_kernel, dim3((C + 31) / 32), dim3(1024), 0, st, (const float*)nullptr, 0, C, dgamma, 0);
+    PG_LAUNCH_OK("pg_rms_norm_bwd");
+    return 0;
+  }
+  int lpr, nch;
+  rms_shape(C, io_flags ? 8 : 4, 0, lpr, nch);
+  const long nb = nch ? rms_bwd_blocks(rows, lpr) : rms_long_slices(rows);
+  PG_REQUIRE(nch || rows < (1L << 31), "pg_rms_norm_bwd: too many rows");
+  PG_REQUIRE(nch || (dx != dy && dx != dh && dx != h), "pg_rms_norm_bwd: rows of more than 2048 channels are read twice: dx must not be an input");
+  PG_REQUIRE(dx != dy || lddy == C, "pg_rms_norm_bwd: dx in place of dy needs lddy == C");
+  RmsBwdK k = {dy, dh, h, rstd, gamma, (long)rows, C, (long)lddy, dx, (float*)workspace, dgamma, accumulate};
+#define PG_RB1(T, L, N) PG_KLAUNCH((rms_bwd_kernel<T, L, N>), dim3((unsigned)nb), dim3(256), 0, st, k)
+#define PG_RB(T)                                                                                                   \
+  do {                                                                                                             \
+    if (nch == 0) {                                                                                                \
+      PG_KLAUNCH((rms_bwd_long_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, k);                             \
+      PG_KLAUNCH((rms_dgamma_long_kernel<T>), dim3((C + 255) / 256, (unsigned)nb), dim3(256), 0, st, k);           \
+    }                                                                                                              \
+    else if (lpr == 8) PG_RB1(T, 8, 1);                                                                            \
+    else if (lpr == 16) PG_RB1(T, 16, 1);                                                                          \
+    else if (lpr == 32) PG_RB1(T, 32, 1);                                                                          \
+    else if (nch == 1) PG_RB1(T, 64, 1);                                                                           \
+    else if (nch == 2) PG_RB1(T, 64, 2);                                                                           \
+    else if (nch == 4) PG_RB1(T, 64, 4);                                                                           \
+    else PG_RB1(T, 64, 32 / RmsV<T>::N);                                                                           \
+  } while (0)
+  if (io_flags == 0) PG_RB(float);
+  else PG_RB(bf16_t);
+#undef PG_RB
+#undef PG_RB1
+  if (!(nch && nb == 1))
+    PG_KLAUNCH(rms_dgamma_kernel, dim3((C + 31) / 32), dim3(1024), 0, st, (const float*)workspace, (int)nb, C, dgamma, accumulate);
+  PG_LAUNCH_OK("pg_rms_norm_bwd");
+  return 0;
+}

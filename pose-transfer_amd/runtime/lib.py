@@ -59,6 +59,15 @@ class WgradDesc(C.Structure):
                 ("ksplit", C.c_int32), ("cout_store", C.c_int32)]
 
 
+class MuonDesc(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("g_bf16", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+                ("p_bf16", C.c_void_p), ("entries", C.c_void_p), ("total", C.c_int64), ("n", C.c_int32),
+                ("nesterov", C.c_int32), ("steps", C.c_int32),
+                ("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("grad_scale", C.c_float),
+                ("eps", C.c_float), ("beta1", C.c_double), ("beta2", C.c_double), ("adam_eps", C.c_float), ("_pad", C.c_int32),
+                ("step", C.c_int64), ("ctr", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 _i32, _i64, _u64, _f32, _vp = C.c_int32, C.c_int64, C.c_uint64, C.c_float, C.c_void_p
 _PROTOS = {
     "pg_conv": [C.POINTER(ConvDesc), _vp],
@@ -156,6 +165,13 @@ _PROTOS = {
     "pg_out_conv_wgrad_bf16": [_vp, _i32, _i32, _i32, _i32, C.POINTER(Dst), _i32, _vp, _vp, _i64, _vp],
     "pg_out_conv_bwd_direct": [_vp, _i32, _vp, _i32, _i32, _i32, C.POINTER(Dst), _i32, _vp, _vp, _i64, _vp, _vp],
     "pg_out_conv_dgrad_wgrad": [_vp, _vp, _i32, _i32, _i32, C.POINTER(Dst), _i32, _vp, _vp, _i64, _vp],
+    "pg_rms_norm_fwd": [_vp, _vp, _vp, _i64, _i32, _i64, _i64, _f32, _i32, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _vp],
+    "pg_rms_norm_bwd_workspace": [_i64, _i32, _i32],
+    "pg_rms_norm_bwd": [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _i32, _vp, _i64, _vp],
+    "pg_orthogonalise_workspace": [_i64, _i64, _i64],
+    "pg_orthogonalise": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _i64, _i64, _i32, _f32, _vp, _i64, _vp],
+    "pg_muon_workspace": [_vp, _i32],
+    "pg_muon_step": [C.POINTER(MuonDesc), _vp],
     "pg_version": [],
     "pg_set_deterministic": [_i32],
     "pg_get_deterministic": [],
@@ -184,7 +200,8 @@ def load():
         fn = getattr(lib, name)
         fn.argtypes = args
         fn.restype = C.c_int
-    lib.pg_stem_pack_elems.restype = C.c_int64
+    for name in ("pg_stem_pack_elems", "pg_rms_norm_bwd_workspace", "pg_orthogonalise_workspace", "pg_muon_workspace"):
+        getattr(lib, name).restype = C.c_int64
     lib.pg_last_error.argtypes = []
     lib.pg_last_error.restype = C.c_char_p
     _lib = lib
