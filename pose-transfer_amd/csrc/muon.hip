@@ -35,7 +35,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int SG = 12, SP = 10;                 // log2 of the scales of G, Q, Q G and of P
 constexpr int K0_ELEMS = 16384;                 // elements per workgroup of the momentum / square-sum pass
-constexpr int GT = 128, CT = 64, AI = 128, AJ = 128;      // tiles: Gram, chain, apply (rows, columns)
+constexpr int GT = 128, CT = 64, AI = 128, AJ = 256;      // tiles: Gram, chain, apply (rows, columns)
 
 struct NsMat {
   long src, ld, st;             // the caller's storage: element offset, row stride, tap stride
@@ -326,21 +326,72 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
   }
 }
 
-// ---------------------------------------------------------------------------------------------- product core, both operands K-contiguous
-// C[BM][BN] = sum_k A[i][k] B[j][k], operands as PL fp16 planes; 4 waves (2 x 2), K in steps of 32 through two LDS stages.
-// An LDS row is 32 halves = four 16-byte slots, chunk c of row r at slot c ^ ((r >> 2) & 3): the 16 lanes that a
-// ds_read_b128 serves at a time (16 consecutive rows, one chunk) then cover the 256 bytes of a bank row once.
-template <int BM, int BN, int PL>
+// ---------------------------------------------------------------------------------------------- product cores
+// Workgroups are dealt round-robin to the 8 XCDs, each with an L2 of its own: `grp` consecutive tiles, which share operand rows, go
+// to one of them.  The grid is padded to a multiple of 8; < 0: no tile.
+__device__ __forceinline__ int xcd_tile(int b, int total, int grp) {
+  const int chunk = 8 * grp, full = total / chunk * chunk;
+  if (b < full) {
+    const int q = b / chunk, r = b - q * chunk;
+    return q * chunk + (r & 7) * grp + (r >> 3);
+  }
+  const int r = b - full, g2 = (total - full + 7) >> 3;
+  const int t = full + (r & 7) * g2 + (r >> 3);
+  return (r >> 3) < g2 && t < total ? t : -1;
+}
+
+// LDS image of an operand with K contiguous: rows of BK halves = CH 16-byte chunks; chunk c of row r at slot c ^ ((r CH / 16) % CH): the 16
+// lanes that a ds_read_b128 serves at a time (16 consecutive rows, one chunk) then cover the 256 bytes of a bank row once.
+// Tiles go global -> LDS without registers (one instruction = 64 lanes x 16 bytes = 1 KB in LDS order), ST stages deep; the operand
+// reads of a K step and their wait are ONE asm block: the compiler, which would wait for every transfer in flight before any LDS
+// read, does not see them, and nothing can come between a read and its wait.  The other waves of the SIMD cover that wait.
+__device__ __forceinline__ void dma16(const _Float16* src, char* dst) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<const float*>(src), reinterpret_cast<float*>(dst), 16, 0, 0);
+}
+template <int N>
+__device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void wg_barrier() {
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+template <int CH>
+__device__ __forceinline__ int swz(int row) { return (row * CH / 16) % CH; }
+
+// one K step (16) of TM + TN fragments: rows 32 apart (RB bytes each), planes PS bytes apart
+#define NS_RD "ds_read_b128 "
+template <int RB, int PSA, int PSB>
+__device__ __forceinline__ void fetch_1x1(unsigned pa, unsigned pb, half8 (&a)[2][1], half8 (&b)[2][1]) {
+  asm volatile(NS_RD "%0, %4\n\t" NS_RD "%1, %4 offset:%6\n\t" NS_RD "%2, %5\n\t" NS_RD "%3, %5 offset:%7\n\t" "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0][0]), "=&v"(a[1][0]), "=&v"(b[0][0]), "=&v"(b[1][0]) : "v"(pa), "v"(pb), "n"(PSA), "n"(PSB) : "memory");
+}
+template <int RB, int PSA, int PSB>
+__device__ __forceinline__ void fetch_2x2(unsigned pa, unsigned pb, half8 (&a)[2][2], half8 (&b)[2][2]) {
+  asm volatile(NS_RD "%0, %8\n\t" NS_RD "%4, %9\n\t" NS_RD "%1, %8 offset:%10\n\t" NS_RD "%5, %9 offset:%10\n\t"
+               NS_RD "%2, %8 offset:%11\n\t" NS_RD "%3, %8 offset:%12\n\t" NS_RD "%6, %9 offset:%13\n\t" NS_RD "%7, %9 offset:%14\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(b[0][0]), "=&v"(b[0][1]), "=&v"(b[1][0]), "=&v"(b[1][1])
+               : "v"(pa), "v"(pb), "n"(32 * RB), "n"(PSA), "n"(PSA + 32 * RB), "n"(PSB), "n"(PSB + 32 * RB) : "memory");
+}
+template <int RB>
+__device__ __forceinline__ void fetch_2x2(unsigned pa, unsigned pb, half8 (&a)[1][2], half8 (&b)[1][2]) {
+  asm volatile(NS_RD "%0, %4\n\t" NS_RD "%2, %5\n\t" NS_RD "%1, %4 offset:%6\n\t" NS_RD "%3, %5 offset:%6\n\t" "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(b[0][0]), "=&v"(b[0][1]) : "v"(pa), "v"(pb), "n"(32 * RB) : "memory");
+}
+
+// C[BM][BN] = sum_k A[i][k] B[j][k], operands as PL fp16 planes; 4 waves (2 x 2), K in steps of BK, ST LDS stages.
+// Rows behind a_rows / b_rows read the last one instead: their products belong to rows and columns that nobody stores.
+template <int BM, int BN, int PL, int BK, int ST>
 struct NtCore {
-  static constexpr int TM = BM / 64, TN = BN / 64;
-  static constexpr int ROWS = (BM + BN) * PL;                       // LDS rows of a stage
-  static constexpr int PASS = ROWS * 4 / 256;                       // 16-byte chunks per thread
-  static constexpr int LDS_BYTES = 2 * ROWS * 64;
+  static constexpr int TM = BM / 64, TN = BN / 64, CH = BK / 8, RB = BK * 2, RPI = 1024 / RB;
+  static constexpr int A_BYTES = BM * PL * RB, STAGE = (BM + BN) * PL * RB;
+  static constexpr int NI = STAGE / 1024 / 4;                       // transfers per wave and stage
+  static constexpr int LDS_BYTES = ST * STAGE;
+  static_assert(TM == TN && (TM == 1 || TM == 2) && (BM % RPI) == 0 && (BN % RPI) == 0 && LDS_BYTES <= 80 * 1024, "tile");
   f32x16 acc[TM][TN];
 
   __device__ __forceinline__ void run(char* smem, const _Float16* A, long a_plane, long lda, int a_rows, const _Float16* B, long b_plane,
                                       long ldb, int b_rows, int k0, int k1) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -348,48 +399,42 @@ struct NtCore {
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    const _Float16* src[PASS];
-    int dst[PASS];
+    const _Float16* src[NI];
 #pragma unroll
-    for (int q = 0; q < PASS; ++q) {
-      const int c = q * 256 + tid, row = c >> 2, slot = c & 3;
+    for (int q = 0; q < NI; ++q) {
+      const int row = (q * 4 + wave) * RPI + lane / CH, slot = lane % CH;
       const bool isA = row < BM * PL;
       const int rr = isA ? row : row - BM * PL;
       const int pl = rr / (isA ? BM : BN), lr = rr - pl * (isA ? BM : BN);
-      const bool ok = lr < (isA ? a_rows : b_rows);
-      src[q] = !ok ? nullptr : (isA ? A + pl * a_plane + (long)lr * lda : B + pl * b_plane + (long)lr * ldb) + slot * 8;
-      dst[q] = row * 64 + ((slot ^ ((row >> 2) & 3)) << 4);
+      const int c = slot ^ swz<CH>(row);
+      src[q] = (isA ? A + pl * a_plane + (long)min(lr, a_rows - 1) * lda : B + pl * b_plane + (long)min(lr, b_rows - 1) * ldb) + c * 8 + k0;
     }
-    uint4 v[PASS];
-    auto load = [&](int k) {
+    auto issue = [&](int st) {
 #pragma unroll
-      for (int q = 0; q < PASS; ++q) v[q] = src[q] ? *reinterpret_cast<const uint4*>(src[q] + k) : make_uint4(0u, 0u, 0u, 0u);
+      for (int q = 0; q < NI; ++q) { dma16(src[q], smem + st * STAGE + (q * 4 + wave) * 1024); src[q] += BK; }
     };
-    auto put = [&](int st) {
+    const int n = (k1 - k0) / BK;
+    const unsigned lds0 = (unsigned)(size_t)smem;
+    const int r = lane & 31;
+    const unsigned off0 = (unsigned)(((lane >> 5) ^ swz<CH>(r)) << 4);
+    const unsigned pa = lds0 + (wm + r) * RB + off0, pb = lds0 + A_BYTES + (wn + r) * RB + off0;
 #pragma unroll
-      for (int q = 0; q < PASS; ++q) *reinterpret_cast<uint4*>(smem + st * (ROWS * 64) + dst[q]) = v[q];
-    };
-    auto frag = [&](int st, int row, int ks) {
-      const int c = ks * 2 + (lane >> 5);
-      return *reinterpret_cast<const half8*>(smem + st * (ROWS * 64) + row * 64 + ((c ^ ((row >> 2) & 3)) << 4));
-    };
-    load(k0);
-    put(0);
-    __syncthreads();
-    int st = 0;
-    for (int k = k0; k < k1; k += 32) {
-      const bool more = k + 32 < k1;
-      if (more) load(k + 32);
+    for (int q = 0; q < ST - 1; ++q)
+      if (q < n) issue(q);
+    int cur = 0, nxt = ST - 1;
+    for (int it = 0; it < n; ++it) {
+      if (it + ST - 2 < n) wait_dma<NI * (ST - 2)>();
+      else wait_dma<0>();
+      wg_barrier();
+      if (it + ST - 1 < n) issue(nxt);
+      const unsigned so = (unsigned)(cur * STAGE);
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
+      for (int ks = 0; ks < BK / 16; ++ks) {
         half8 a[PL][TM], b[PL][TN];
-#pragma unroll
-        for (int pl = 0; pl < PL; ++pl) {
-#pragma unroll
-          for (int i = 0; i < TM; ++i) a[pl][i] = frag(st, pl * BM + wm + i * 32 + (lane & 31), ks);
-#pragma unroll
-          for (int j = 0; j < TN; ++j) b[pl][j] = frag(st, BM * PL + pl * BN + wn + j * 32 + (lane & 31), ks);
-        }
+        const unsigned qa = ((pa ^ (unsigned)(ks << 5)) + so), qb = ((pb ^ (unsigned)(ks << 5)) + so);
+        if constexpr (TM == 1) fetch_1x1<RB, BM * RB, BN * RB>(qa, qb, a, b);
+        else if constexpr (PL == 2) fetch_2x2<RB, BM * RB, BN * RB>(qa, qb, a, b);
+        else fetch_2x2<RB>(qa, qb, a, b);
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -401,9 +446,8 @@ struct NtCore {
             }
           }
       }
-      if (more) put(st ^ 1);
-      __syncthreads();
-      st ^= 1;
+      cur = cur + 1 == ST ? 0 : cur + 1;
+      nxt = nxt + 1 == ST ? 0 : nxt + 1;
     }
   }
   // f(row, column, value) of the tile, for every accumulator element: rows 8 (e >> 2) + 4 (lane >> 5) + (e & 3), column lane & 31
@@ -423,6 +467,26 @@ struct NtCore {
   }
 };
 
+// four rows of one column of a symmetric matrix in the lower triangle, to both triangles
+__device__ __forceinline__ void put_sym(_Float16* C, long pl, long ld, int gi, int gj, bool diag, const float (&v)[4]) {
+  half4 hh, ll;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    _Float16 h, l;
+    split16(v[e], h, l);
+    hh[e] = h; ll[e] = l;
+    if (!diag || gi + e >= gj) { C[(long)(gi + e) * ld + gj] = h; C[pl + (long)(gi + e) * ld + gj] = l; }
+  }
+  if (!diag) {
+    *reinterpret_cast<half4*>(C + (long)gj * ld + gi) = hh;
+    *reinterpret_cast<half4*>(C + pl + (long)gj * ld + gi) = ll;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (gi + e > gj) { C[(long)gj * ld + gi + e] = hh[e]; C[pl + (long)gj * ld + gi + e] = ll[e]; }
+  }
+}
+
 // tile number of the lower triangle (bi >= bj), row by row
 __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
   int i = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
@@ -432,12 +496,14 @@ __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
   bj = t - i * (i + 1) / 2;
 }
 
-// G = X X^T over one slice of the long side: fp32 partial tiles
+// G = X X^T over one slice of the long side: fp32 partial tiles, in the order of the accumulators (one float4 = four rows of a column)
 template <int PL>
-__global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, const _Float16* ws, float* part) {
-  typedef NtCore<GT, GT, PL> Core;
-  __shared__ __attribute__((aligned(16))) char smem[Core::LDS_BYTES];
-  const NsRef r = ns_find<&NsMat::bg, &NsGroup::ng>(gr, blockIdx.x);
+__global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int total, const _Float16* ws, float* part) {
+  typedef NtCore<GT, GT, PL, 32, 2> Core;
+  __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
+  const int b = xcd_tile(blockIdx.x, total, 10);
+  if (b < 0) return;
+  const NsRef r = ns_find<&NsMat::bg, &NsGroup::ng>(gr, b);
   const NsMat& m = r.m;
   const int nt = (m.Mp + GT - 1) / GT, ntri = nt * (nt + 1) / 2;
   const int split = r.tile / ntri, t = r.tile - split * ntri;
@@ -448,58 +514,52 @@ __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, const
   Core c;
   c.run(smem, X + (long)bi * GT * m.Np, plane, m.Np, m.Mp - bi * GT, X + (long)bj * GT * m.Np, plane, m.Np, m.Mp - bj * GT,
         split * m.kc, min(m.Np, (split + 1) * m.kc));
-  float* out = part + m.part + (long)r.tile * (GT * GT);
-  c.each4([&](int i, int j, const float (&v)[4]) {
+  float4* out = reinterpret_cast<float4*>(part + m.part + (long)r.tile * (GT * GT));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[(i + e) * GT + j] = v[e];
-  });
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        out[((wave * 4 + i * 2 + j) * 4 + q) * 64 + lane] =
+            make_float4(c.acc[i][j][4 * q], c.acc[i][j][4 * q + 1], c.acc[i][j][4 * q + 2], c.acc[i][j][4 * q + 3]);
 }
 
-// join of the slices, in order; both triangles of G from the lower one; one workgroup = 64 x 64 elements
+// join of the slices, in order; both triangles of G from the lower one.  One workgroup = one 32 x 32 block, a float4 per thread
 __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, const float* part, const float* cfac, float cconst, _Float16* ws) {
-  __shared__ float tile[64][65];
   const NsRef r = ns_find<&NsMat::br, &NsGroup::nr>(gr, blockIdx.x);
   const NsMat& m = r.m;
   int bi, bj;
-  tri(r.tile, bi, bj);                               // in units of 64
-  const int gi = bi / 2, gj = bj / 2;                // the 128-tile that holds it
+  tri(r.tile, bi, bj);                               // in units of 32
+  const int gi = bi / 4, gj = bj / 4, fi = bi & 3, fj = bj & 3;      // its 128-tile, and where in it
   const int nt = (m.Mp + GT - 1) / GT, ntri = nt * (nt + 1) / 2;
-  const long t0 = gi * (gi + 1) / 2 + gj;
+  const int wave = (fi >> 1) * 2 + (fj >> 1), frag = wave * 4 + (fi & 1) * 2 + (fj & 1);
+  const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const float4* src = reinterpret_cast<const float4*>(part + m.part + (long)(gi * (gi + 1) / 2 + gj) * (GT * GT)) + (frag * 4 + q) * 64 + lane;
   const float c1 = cfac ? cfac[r.id] : cconst;
   const float c2 = c1 * c1 * (float)(1 << SG);
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  for (int q = ty; q < 64; q += 4) {
-    const float* src = part + m.part + t0 * (GT * GT) + (long)((bi & 1) * 64 + q) * GT + (bj & 1) * 64 + tx;
-    float a = 0.f;
-    for (int s = 0; s < m.ks; ++s) a += src[(long)s * ntri * (GT * GT)];
-    tile[q][tx] = a * c2;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < m.ks; ++s) {
+    const float4 f = src[(long)s * ntri * (GT * GT / 4)];
+    v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
   }
-  __syncthreads();
-  _Float16* G = ws + m.g;
-  const long pl = (long)m.Mp * m.Mp;
-  for (int q = ty; q < 64; q += 4) {
-    _Float16 h, l;
-    const float v = (bi == bj && tx > q) ? tile[tx][q] : tile[q][tx];
-    split16(v, h, l);
-    const long at = (long)(bi * 64 + q) * m.Mp + bj * 64 + tx;
-    G[at] = h; G[pl + at] = l;
-    if (bi != bj) {
-      split16(tile[tx][q], h, l);
-      const long bt = (long)(bj * 64 + q) * m.Mp + bi * 64 + tx;
-      G[bt] = h; G[pl + bt] = l;
-    }
-  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] *= c2;
+  put_sym(ws + m.g, (long)m.Mp * m.Mp, m.Mp, bi * 32 + 8 * q + 4 * (lane >> 5), bj * 32 + (lane & 31), bi == bj, v);
 }
 
 // chain planes of a matrix: 0 G, 1 Q, 2 Q G, 3 P, 4 the other P  (hi and lo each)
 // C = A B of commuting symmetric matrices: the lower triangle of 64 x 64 tiles, mirrored.  `quad`: C = a I + b A + c A A
 struct ChainJob { int a, b, c; float mul; int quad; };
-__global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int njobs, _Float16* ws) {
-  typedef NtCore<CT, CT, 2> Core;
-  __shared__ __attribute__((aligned(16))) char smem[Core::LDS_BYTES];
-  const int job = njobs == 2 ? (int)(blockIdx.x & 1) : 0;
-  const NsRef r = ns_find<&NsMat::bc, &NsGroup::nc>(gr, njobs == 2 ? (int)(blockIdx.x >> 1) : (int)blockIdx.x);
-  const ChainJob jb = job ? j1 : j0;
+__global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
+  typedef NtCore<CT, CT, 2, 32, 4> Core;
+  __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
+  const int t = xcd_tile(blockIdx.x, total, 36);
+  if (t < 0) return;
+  const ChainJob jb = t >= tiles ? j1 : j0;          // two jobs: the second one's tiles come behind the first one's
+  const NsRef r = ns_find<&NsMat::bc, &NsGroup::nc>(gr, t >= tiles ? t - tiles : t);
   const NsMat& m = r.m;
   int bi, bj;
   tri(r.tile, bi, bj);
@@ -511,29 +571,17 @@ __global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, Chai
   c.run(smem, A + (long)bi * CT * m.Mp, pl, m.Mp, CT, B + (long)bj * CT * m.Mp, pl, m.Mp, CT, 0, m.Mp);
   c.each4([&](int i, int j, const float (&v)[4]) {
     const int gi = bi * CT + i, gj = bj * CT + j;
-    half4 hh, ll;
+    float u[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      float t = v[e] * jb.mul;
-      const long at = (long)(gi + e) * m.Mp + gj;
+      u[e] = v[e] * jb.mul;
       if (jb.quad) {
-        t += NS_B * ((float)A[at] + (float)A[pl + at]);
-        if (gi + e == gj) t += NS_A * (float)(1 << SG);
+        const long at = (long)(gi + e) * m.Mp + gj;
+        u[e] += NS_B * ((float)A[at] + (float)A[pl + at]);
+        if (gi + e == gj) u[e] += NS_A * (float)(1 << SG);
       }
-      _Float16 h, l;
-      split16(t, h, l);
-      hh[e] = h; ll[e] = l;
-      if (bi != bj || gi + e >= gj) { C[at] = h; C[pl + at] = l; }
     }
-    if (bi != bj) {
-      const long bt = (long)gj * m.Mp + gi;
-      *reinterpret_cast<half4*>(C + bt) = hh;
-      *reinterpret_cast<half4*>(C + pl + bt) = ll;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (gi + e > gj) { C[(long)gj * m.Mp + gi + e] = hh[e]; C[pl + (long)gj * m.Mp + gi + e] = ll[e]; }
-    }
+    put_sym(C, pl, m.Mp, gi, gj, bi == bj, u);
   });
 }
 
@@ -547,98 +595,112 @@ struct ApplyK {
   void* out; long ldo;
   NsStep s;
 };
+// one K step of the apply product: P rows 32 bytes each (one K step per stage), 4 fragments of 32 rows; X rows (K) of 256 columns through
+// the transposing read: in a group of 16 lanes lane 4 r + c gives the address of four columns of row r and gets one column of four
+// rows; two of them make a fragment
+#define NS_TR "ds_read_b64_tr_b16 "
+__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][4], half4 (&b)[2][2][2]) {
+  asm volatile(NS_RD "%0, %16\n\t" NS_TR "%8, %17\n\t" NS_TR "%9, %17 offset:2048\n\t" NS_RD "%1, %16 offset:1024\n\t"
+               NS_TR "%10, %18\n\t" NS_TR "%11, %18 offset:2048\n\t" NS_RD "%2, %16 offset:2048\n\t" NS_RD "%3, %16 offset:3072\n\t"
+               NS_RD "%4, %16 offset:4096\n\t" NS_RD "%5, %16 offset:5120\n\t" NS_RD "%6, %16 offset:6144\n\t" NS_RD "%7, %16 offset:7168\n\t"
+               NS_TR "%12, %17 offset:8192\n\t" NS_TR "%13, %17 offset:10240\n\t" NS_TR "%14, %18 offset:8192\n\t" NS_TR "%15, %18 offset:10240\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[0][2]), "=&v"(a[0][3]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(a[1][2]), "=&v"(a[1][3]),
+                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1]),
+                 "=&v"(b[1][0][0]), "=&v"(b[1][0][1]), "=&v"(b[1][1][0]), "=&v"(b[1][1][1])
+               : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
+}
+__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][4], half4 (&b)[1][2][2]) {
+  asm volatile(NS_RD "%0, %12\n\t" NS_TR "%8, %13\n\t" NS_TR "%9, %13 offset:2048\n\t" NS_RD "%1, %12 offset:1024\n\t"
+               NS_TR "%10, %14\n\t" NS_TR "%11, %14 offset:2048\n\t" NS_RD "%2, %12 offset:2048\n\t" NS_RD "%3, %12 offset:3072\n\t"
+               NS_RD "%4, %12 offset:4096\n\t" NS_RD "%5, %12 offset:5120\n\t" NS_RD "%6, %12 offset:6144\n\t" NS_RD "%7, %12 offset:7168\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[0][2]), "=&v"(a[0][3]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(a[1][2]), "=&v"(a[1][3]),
+                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1])
+               : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
+}
+
+// A tile is 128 rows x 256 columns: 4 waves side by side, 128 x 64 each (per K step 12 KB of LDS reads for 24 MFMAs; 64 x 64 would need
+// two thirds more), K steps of 16 through three stages: 72 KB, two workgroups per CU, whose epilogues run under each other's products.
 template <int PX, int OUT>
-__global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, const ApplyK k) {
-  constexpr int A_BYTES = AI * 2 * 64, B_BYTES = 32 * AJ * 2 * PX, STAGE = A_BYTES + B_BYTES;
-  constexpr int PA = AI * 2 * 4 / 256, PB = 32 * (AJ / 8) * PX / 256;
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
-  const NsRef r = ns_find<&NsMat::ba, &NsGroup::na>(gr, blockIdx.x);
+__global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int total, const ApplyK k) {
+  constexpr int A_BYTES = AI * 2 * 32, B_BYTES = 16 * AJ * 2 * PX, STAGE = A_BYTES + B_BYTES, ST = 3;
+  constexpr int PA = A_BYTES / 4096, PB = B_BYTES / 4096, NI = PA + PB;
+  __shared__ __attribute__((aligned(1024))) char smem[ST * STAGE];
+  const int bt = xcd_tile(blockIdx.x, total, 4);
+  if (bt < 0) return;
+  const NsRef r = ns_find<&NsMat::ba, &NsGroup::na>(gr, bt);
   const NsMat& m = r.m;
   const int ti = (m.Mp + AI - 1) / AI;
   const int i0 = (r.tile % ti) * AI, j0 = (r.tile / ti) * AJ;
   const long pl = (long)m.Mp * m.Mp, xpl = (long)m.Mp * m.Np;
   const _Float16* P = k.wsg + m.g + k.pbuf * 2 * pl;
   const _Float16* X = k.wsx + m.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  f32x16 acc[2][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave * 64;
+  f32x16 acc[4][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  const _Float16* as[PA]; int ad[PA];
+  // P: 32 rows of two chunks per transfer; X: two rows of 32 chunks, chunk c of row k at slot c ^ ((k & 3) << 2) for the transposing reads.
+  // Rows and columns behind the matrix read its last ones: products that nobody stores.
+  const _Float16* as[PA];
 #pragma unroll
   for (int q = 0; q < PA; ++q) {
-    const int c = q * 256 + tid, row = c >> 2, slot = c & 3, plane = row / AI, lr = row - plane * AI;
-    as[q] = i0 + lr < m.Mp ? P + plane * pl + (long)(i0 + lr) * m.Mp + slot * 8 : nullptr;
-    ad[q] = row * 64 + ((slot ^ ((row >> 2) & 3)) << 4);
+    const int row = (q * 4 + wave) * 32 + (lane >> 1), plane = row / AI, lr = min(i0 + row - plane * AI, m.Mp - 1);
+    as[q] = P + plane * pl + (long)lr * m.Mp + ((lane & 1) ^ swz<2>(row)) * 8;
   }
-  // X rows = K: [32][128] halves per plane, chunk c of row k at slot c ^ ((k & 3) << 2) for the transposing reads
-  const _Float16* bs[PB]; int bd[PB];
+  const _Float16* bs[PB];
 #pragma unroll
   for (int q = 0; q < PB; ++q) {
-    const int c = q * 256 + tid, row = c >> 4, slot = c & 15, plane = row >> 5, kr = row & 31;
-    bs[q] = j0 + slot * 8 < m.Np ? X + plane * xpl + (long)kr * m.Np + j0 + slot * 8 : nullptr;
-    bd[q] = A_BYTES + row * (AJ * 2) + ((slot ^ ((kr & 3) << 2)) << 4);
+    const int row = (q * 4 + wave) * 2 + (lane >> 5), plane = row >> 4, kr = row & 15;
+    const int col = min(j0 + (((lane & 31) ^ ((kr & 3) << 2)) * 8), m.Np - 8);
+    bs[q] = X + plane * xpl + (long)kr * m.Np + col;
   }
-  uint4 va[PA], vb[PB];
-  auto load = [&](int kk) {
+  const long bstep = 16L * m.Np;
+  auto issue = [&](int st) {
 #pragma unroll
-    for (int q = 0; q < PA; ++q) va[q] = as[q] ? *reinterpret_cast<const uint4*>(as[q] + kk) : make_uint4(0u, 0u, 0u, 0u);
+    for (int q = 0; q < PA; ++q) { dma16(as[q], smem + st * STAGE + (q * 4 + wave) * 1024); as[q] += 16; }
 #pragma unroll
-    for (int q = 0; q < PB; ++q) vb[q] = bs[q] ? *reinterpret_cast<const uint4*>(bs[q] + (long)kk * m.Np) : make_uint4(0u, 0u, 0u, 0u);
+    for (int q = 0; q < PB; ++q) { dma16(bs[q], smem + st * STAGE + A_BYTES + (q * 4 + wave) * 1024); bs[q] += bstep; }
   };
-  auto put = [&](int st) {
-#pragma unroll
-    for (int q = 0; q < PA; ++q) *reinterpret_cast<uint4*>(smem + st * STAGE + ad[q]) = va[q];
-#pragma unroll
-    for (int q = 0; q < PB; ++q) *reinterpret_cast<uint4*>(smem + st * STAGE + bd[q]) = vb[q];
-  };
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const unsigned lds0 = (unsigned)(size_t)smem;
   const int r4 = (lane >> 2) & 3, cq = lane & 3, mb = (lane >> 4) & 1, kh = lane >> 5;
-  load(0);
-  put(0);
-  __syncthreads();
-  int st = 0;
-  for (int kk = 0; kk < m.Mp; kk += 32) {
-    const bool more = kk + 32 < m.Mp;
-    if (more) load(kk + 32);
+  const unsigned pa = lds0 + (lane & 31) * 32 + ((kh ^ swz<2>(lane & 31)) << 4);
+  const int chunk = (wn >> 3) + 2 * mb + (cq >> 1);
+  const unsigned pb0 = lds0 + A_BYTES + (8 * kh + r4) * (AJ * 2) + ((chunk ^ (r4 << 2)) << 4) + ((cq & 1) << 3);
+  const unsigned pb1 = lds0 + A_BYTES + (8 * kh + r4) * (AJ * 2) + (((chunk + 4) ^ (r4 << 2)) << 4) + ((cq & 1) << 3);
+  const int n = m.Mp / 16;
+  issue(0);
+  issue(1);
+  int cur = 0, nxt = 2;
+  for (int it = 0; it < n; ++it) {
+    if (it + 1 < n) wait_dma<NI>();
+    else wait_dma<0>();
+    wg_barrier();
+    if (it + 2 < n) issue(nxt);
+    const unsigned so = (unsigned)(cur * STAGE);
+    half8 a[2][4];
+    half4 bq[PX][2][2];
+    fetch_apply(pa + so, pb0 + so, pb1 + so, a, bq);
+    half8 b[PX][2];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      half8 a[2][2], b[PX][2];
+    for (int p = 0; p < PX; ++p)
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+      for (int j = 0; j < 2; ++j) b[p][j] = __builtin_shufflevector(bq[p][j][0], bq[p][j][1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = p * AI + wm + i * 32 + (lane & 31), c = ks * 2 + kh;
-          a[p][i] = *reinterpret_cast<const half8*>(smem + st * STAGE + row * 64 + ((c ^ ((row >> 2) & 3)) << 4));
-        }
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int p = 0; p < PX; ++p)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int chunk = ((wn + j * 32) >> 3) + 2 * mb + (cq >> 1);
-          char* q = smem + st * STAGE + A_BYTES + (p * 32 + ks * 16 + 8 * kh + r4) * (AJ * 2) + ((chunk ^ (r4 << 2)) << 4) + ((cq & 1) << 3);
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 4 * AJ * 2));
-          typedef short s16x8 __attribute__((ext_vector_type(8)));
-          const s16x8 w = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          b[p][j] = __builtin_bit_cast(half8, w);
-        }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][i], b[0][j], acc[i][j], 0, 0, 0);
-          if constexpr (PX == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[1][j], acc[i][j], 0, 0, 0);
-        }
-    }
-    if (more) put(st ^ 1);
-    __syncthreads();
-    st ^= 1;
+      for (int j = 0; j < 2; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][j], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][i], b[0][j], acc[i][j], 0, 0, 0);
+        if constexpr (PX == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[1][j], acc[i][j], 0, 0, 0);
+      }
+    cur = cur == ST - 1 ? 0 : cur + 1;
+    nxt = nxt == ST - 1 ? 0 : nxt + 1;
   }
   const float f = (k.cfac ? k.cfac[r.id] : k.cconst) * k.mul;
   const float keep = 1.f - k.s.lr * k.s.wd, step = k.s.lr * m.scale;
@@ -653,10 +715,10 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, cons
     // wide: the column is the lane's for all rows; tall: it is the stored row
     const long cbase = OUT == 0 ? (long)gj : m.tall ? 0L : ns_at(m, 0, gj);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int ii = i0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        const int ii = i0 + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
         const float v = acc[i][j][e] * f;
         if constexpr (OUT == 0) {
           if (ii < m.Mp) {
@@ -722,8 +784,9 @@ static NsCounts ns_counts(NsMat& m, long others, bool flat) {
   m.kc = (int)up(cdiv(m.Np, ks), 32);
   m.ks = (int)cdiv(m.Np, m.kc);
   c.ng = ntri * m.ks;
-  const long n64 = m.Mp / 64;
-  c.nr = c.nc = n64 * (n64 + 1) / 2;
+  const long n64 = m.Mp / 64, n32 = m.Mp / 32;
+  c.nc = n64 * (n64 + 1) / 2;
+  c.nr = n32 * (n32 + 1) / 2;
   c.na = (long)cdiv(m.Mp, AI) * cdiv(m.Np, AJ);
   c.x = 2L * m.Mp * m.Np;
   c.g = 10L * m.Mp * m.Mp;
@@ -816,22 +879,24 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     const bool last = steps == 0;
     const float* cf = first ? cfac : nullptr;
     const bool one = first && in.kind == 1;
-    if (one) PG_KLAUNCH((ns_gram_kernel<1>), dim3((unsigned)pl.ng), blk, 0, st, gr, (const _Float16*)xin, part);
-    else PG_KLAUNCH((ns_gram_kernel<2>), dim3((unsigned)pl.ng), blk, 0, st, gr, (const _Float16*)xin, part);
+    if (one) PG_KLAUNCH((ns_gram_kernel<1>), dim3((unsigned)up(pl.ng, 8)), blk, 0, st, gr, (int)pl.ng, (const _Float16*)xin, part);
+    else PG_KLAUNCH((ns_gram_kernel<2>), dim3((unsigned)up(pl.ng, 8)), blk, 0, st, gr, (int)pl.ng, (const _Float16*)xin, part);
     PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.nr), blk, 0, st, gr, (const float*)part, cf, 1.f / sx, g);
     // buffers: 0 G, 1 Q, 2 Q G, 3 and 4 P in turn; the first step's Q is the first P (and keeps Q's scale)
     const float q1 = 1.f / (float)(1 << SG);
     int p = 3, psc = SG;
+    const int nc = (int)pl.nc;
+    const dim3 gc((unsigned)up(pl.nc, 8));
     for (int k = 0; k < ns; ++k) {
       const int q = k == 0 ? 3 : 1;
       const ChainJob quad = {0, 0, q, NS_C * q1, 1};
-      PG_KLAUNCH(ns_chain_kernel, dim3((unsigned)pl.nc), blk, 0, st, gr, quad, quad, 1, g);
+      PG_KLAUNCH(ns_chain_kernel, gc, blk, 0, st, gr, quad, quad, nc, nc, g);
       const ChainJob qg = {q, 0, 2, q1, 0}, qp = {q, p, 7 - p, (float)ldexp(1.0, SP - SG - psc), 0}, qqg = {q, 2, 0, q1, 0};
       const bool more = k + 1 < ns;
-      if (more && k > 0) PG_KLAUNCH(ns_chain_kernel, dim3((unsigned)pl.nc * 2), blk, 0, st, gr, qg, qp, 2, g);
-      else if (more) PG_KLAUNCH(ns_chain_kernel, dim3((unsigned)pl.nc), blk, 0, st, gr, qg, qg, 1, g);
-      else if (k > 0) PG_KLAUNCH(ns_chain_kernel, dim3((unsigned)pl.nc), blk, 0, st, gr, qp, qp, 1, g);
-      if (more) PG_KLAUNCH(ns_chain_kernel, dim3((unsigned)pl.nc), blk, 0, st, gr, qqg, qqg, 1, g);
+      if (more && k > 0) PG_KLAUNCH(ns_chain_kernel, dim3((unsigned)up(2 * pl.nc, 8)), blk, 0, st, gr, qg, qp, 2 * nc, nc, g);
+      else if (more) PG_KLAUNCH(ns_chain_kernel, gc, blk, 0, st, gr, qg, qg, nc, nc, g);
+      else if (k > 0) PG_KLAUNCH(ns_chain_kernel, gc, blk, 0, st, gr, qp, qp, nc, nc, g);
+      if (more) PG_KLAUNCH(ns_chain_kernel, gc, blk, 0, st, gr, qqg, qqg, nc, nc, g);
       if (k > 0) { p = 7 - p; psc = SP; }
     }
     ApplyK a;
@@ -841,16 +906,17 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     a.mul = (float)ldexp(1.0, -psc) * (last ? 1.f : sx);
     a.out = out; a.ldo = ldo; a.s = step;
     const int o = last ? out_kind : 0;
-    const dim3 gd((unsigned)pl.na);
+    const dim3 gd((unsigned)up(pl.na, 8));
+    const int na = (int)pl.na;
     if (one) {
-      if (o == 0) PG_KLAUNCH((ns_apply_kernel<1, 0>), gd, blk, 0, st, gr, a);
-      else if (o == 1) PG_KLAUNCH((ns_apply_kernel<1, 1>), gd, blk, 0, st, gr, a);
-      else PG_KLAUNCH((ns_apply_kernel<1, 2>), gd, blk, 0, st, gr, a);
+      if (o == 0) PG_KLAUNCH((ns_apply_kernel<1, 0>), gd, blk, 0, st, gr, na, a);
+      else if (o == 1) PG_KLAUNCH((ns_apply_kernel<1, 1>), gd, blk, 0, st, gr, na, a);
+      else PG_KLAUNCH((ns_apply_kernel<1, 2>), gd, blk, 0, st, gr, na, a);
     } else {
-      if (o == 0) PG_KLAUNCH((ns_apply_kernel<2, 0>), gd, blk, 0, st, gr, a);
-      else if (o == 1) PG_KLAUNCH((ns_apply_kernel<2, 1>), gd, blk, 0, st, gr, a);
-      else if (o == 2) PG_KLAUNCH((ns_apply_kernel<2, 2>), gd, blk, 0, st, gr, a);
-      else PG_KLAUNCH((ns_apply_kernel<2, 3>), gd, blk, 0, st, gr, a);
+      if (o == 0) PG_KLAUNCH((ns_apply_kernel<2, 0>), gd, blk, 0, st, gr, na, a);
+      else if (o == 1) PG_KLAUNCH((ns_apply_kernel<2, 1>), gd, blk, 0, st, gr, na, a);
+      else if (o == 2) PG_KLAUNCH((ns_apply_kernel<2, 2>), gd, blk, 0, st, gr, na, a);
+      else PG_KLAUNCH((ns_apply_kernel<2, 3>), gd, blk, 0, st, gr, na, a);
     }
     _Float16* t = xin; xin = xout; xout = t;
     first = false;
