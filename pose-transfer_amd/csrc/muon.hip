@@ -34,7 +34,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int SG = 12, SP = 10;                 // log2 of the scales of G, Q, Q G and of P
-constexpr int K0_ELEMS = 16384;                 // elements per workgroup of the momentum / square-sum pass
+// elements per workgroup of the momentum / square-sum pass: small tensors give few workgroups, large ones many partial sums
+__host__ __device__ constexpr int k0_elems(long n) { return n < (1L << 21) ? 4096 : 16384; }
 constexpr int GT = 128, CT = 64, AI = 128, AJ = 256;      // tiles: Gram, chain, apply (rows, columns)
 
 struct NsMat {
@@ -122,17 +123,22 @@ struct NsStep {
 __device__ __forceinline__ float ns_grad(const NsStep& s, long i) { return (s.gb ? bf2f(s.gb[i]) : s.g[i]) * s.gscale; }
 __device__ __forceinline__ float ns_update(const NsStep& s, float g, float m1) { return s.nesterov ? (1.f - s.mu) * g + s.mu * m1 : m1; }
 
-// one workgroup = K0_ELEMS consecutive elements of a tensor; 28 bytes / element for Adam's, 12 for a matrix's
+// one workgroup = k0_elems consecutive elements of a tensor; 28 bytes / element for Adam's, 12 for a matrix's
 __global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, const NsStep s, double* sq) {
   __shared__ double red[4];
   const NsRef r = ns_find<&NsMat::b0, &NsGroup::n0>(gr, blockIdx.x);
   const long n = (long)r.m.taps * r.m.rows * r.m.cols;
-  const long e0 = (long)r.tile * K0_ELEMS, e1 = min(n, e0 + K0_ELEMS);
+  const long e0 = (long)r.tile * k0_elems(n), e1 = min(n, e0 + k0_elems(n));
   const long base = r.m.src;
   if (r.m.kind == 1) {
-    const double t = (double)(s.step0 + (s.ctr ? (long)s.ctr[0] : 0L));
-    const float step_size = (float)((double)s.lr / (1.0 - pow(s.b1d, t)));
-    const float bc2 = (float)sqrt(1.0 - pow(s.b2d, t));
+    if (threadIdx.x < 2) {                             // 1 - beta^t, in fp64, by one lane each
+      const double t = (double)(s.step0 + (s.ctr ? (long)s.ctr[0] : 0L));
+      red[threadIdx.x] = 1.0 - pow(threadIdx.x ? s.b2d : s.b1d, t);
+    }
+    __syncthreads();
+    const float step_size = (float)((double)s.lr / red[0]);
+    const float bc2 = (float)sqrt(red[1]);
+#pragma unroll 4
     for (long i = e0 + threadIdx.x; i < e1; i += 256) {
       const float g = ns_grad(s, base + i);
       const float m = s.m[base + i] * s.b1 + (1.f - s.b1) * g;
@@ -193,6 +199,7 @@ __device__ __forceinline__ long ns_at(const NsMat& m, int row, int fc) {
   const int tap = m.taps == 1 ? 0 : fc / m.cols;
   return m.src + (long)tap * m.st + (long)row * m.ld + (fc - tap * m.cols);
 }
+struct __attribute__((packed, aligned(2))) NsU2 { unsigned x, y; };
 struct __attribute__((packed, aligned(2))) NsU4 { unsigned x, y, z, w; };      // 16 bytes at the alignment of one element
 __device__ __forceinline__ void ns_ld8(const float* q, float (&v)[8]) {
   const NsU4 a = reinterpret_cast<const NsU4*>(q)[0], b = reinterpret_cast<const NsU4*>(q)[1];
@@ -235,14 +242,15 @@ __device__ __forceinline__ void ns_load8(const NsMat& m, const void* x, const Ns
   }
 }
 
-// one workgroup = K0_ELEMS / 8 runs of eight stored neighbours
+// one workgroup = 512 runs of eight stored neighbours
+constexpr int SQ_RUNS = 512;
 template <int SRC>
 __global__ __launch_bounds__(256) void ns_sumsq_kernel(const NsGroup gr, const void* x, double* sq) {
   __shared__ double red[4];
   const NsRef r = ns_find<&NsMat::b0, &NsGroup::n0>(gr, blockIdx.x);
   const unsigned rpr = (unsigned)(r.m.cols + 7) / 8u;
   const unsigned n = (unsigned)r.m.rows * rpr;
-  const unsigned e0 = (unsigned)r.tile * (K0_ELEMS / 8), e1 = min(n, e0 + K0_ELEMS / 8);
+  const unsigned e0 = (unsigned)r.tile * SQ_RUNS, e1 = min(n, e0 + SQ_RUNS);
   double acc = 0.0;
   const NsStep s{};
   for (unsigned i = e0 + threadIdx.x; i < e1; i += 256) {
@@ -359,10 +367,10 @@ __device__ __forceinline__ int swz(int row) { return (row * CH / 16) % CH; }
 
 // one K step (16) of TM + TN fragments: rows 32 apart (RB bytes each), planes PS bytes apart
 #define NS_RD "ds_read_b128 "
-template <int RB, int PSA, int PSB>
-__device__ __forceinline__ void fetch_1x1(unsigned pa, unsigned pb, half8 (&a)[2][1], half8 (&b)[2][1]) {
-  asm volatile(NS_RD "%0, %4\n\t" NS_RD "%1, %4 offset:%6\n\t" NS_RD "%2, %5\n\t" NS_RD "%3, %5 offset:%7\n\t" "s_waitcnt lgkmcnt(0)"
-               : "=&v"(a[0][0]), "=&v"(a[1][0]), "=&v"(b[0][0]), "=&v"(b[1][0]) : "v"(pa), "v"(pb), "n"(PSA), "n"(PSB) : "memory");
+template <int PS>
+__device__ __forceinline__ void fetch_1x1(unsigned pa, unsigned pb, half8 (&a)[2], half8 (&b)[2]) {
+  asm volatile(NS_RD "%0, %4\n\t" NS_RD "%2, %5\n\t" NS_RD "%1, %4 offset:%6\n\t" NS_RD "%3, %5 offset:%6\n\t" "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0]), "=&v"(a[1]), "=&v"(b[0]), "=&v"(b[1]) : "v"(pa), "v"(pb), "n"(PS) : "memory");
 }
 template <int RB, int PSA, int PSB>
 __device__ __forceinline__ void fetch_2x2(unsigned pa, unsigned pb, half8 (&a)[2][2], half8 (&b)[2][2]) {
@@ -386,7 +394,7 @@ struct NtCore {
   static constexpr int A_BYTES = BM * PL * RB, STAGE = (BM + BN) * PL * RB;
   static constexpr int NI = STAGE / 1024 / 4;                       // transfers per wave and stage
   static constexpr int LDS_BYTES = ST * STAGE;
-  static_assert(TM == TN && (TM == 1 || TM == 2) && (BM % RPI) == 0 && (BN % RPI) == 0 && LDS_BYTES <= 80 * 1024, "tile");
+  static_assert(TM == 2 && TN == 2 && (BM % RPI) == 0 && (BN % RPI) == 0 && LDS_BYTES <= 80 * 1024, "tile");
   f32x16 acc[TM][TN];
 
   __device__ __forceinline__ void run(char* smem, const _Float16* A, long a_plane, long lda, int a_rows, const _Float16* B, long b_plane,
@@ -432,8 +440,7 @@ struct NtCore {
       for (int ks = 0; ks < BK / 16; ++ks) {
         half8 a[PL][TM], b[PL][TN];
         const unsigned qa = ((pa ^ (unsigned)(ks << 5)) + so), qb = ((pb ^ (unsigned)(ks << 5)) + so);
-        if constexpr (TM == 1) fetch_1x1<RB, BM * RB, BN * RB>(qa, qb, a, b);
-        else if constexpr (PL == 2) fetch_2x2<RB, BM * RB, BN * RB>(qa, qb, a, b);
+        if constexpr (PL == 2) fetch_2x2<RB, BM * RB, BN * RB>(qa, qb, a, b);
         else fetch_2x2<RB>(qa, qb, a, b);
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -450,42 +457,11 @@ struct NtCore {
       nxt = nxt + 1 == ST ? 0 : nxt + 1;
     }
   }
-  // f(row, column, value) of the tile, for every accumulator element: rows 8 (e >> 2) + 4 (lane >> 5) + (e & 3), column lane & 31
-  template <typename F>
-  __device__ __forceinline__ void each4(F&& f) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          f(wm + i * 32 + 8 * q + 4 * (lane >> 5), wn + j * 32 + (lane & 31), v);
-        }
-  }
 };
 
-// four rows of one column of a symmetric matrix in the lower triangle, to both triangles
-__device__ __forceinline__ void put_sym(_Float16* C, long pl, long ld, int gi, int gj, bool diag, const float (&v)[4]) {
-  half4 hh, ll;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    _Float16 h, l;
-    split16(v[e], h, l);
-    hh[e] = h; ll[e] = l;
-    if (!diag || gi + e >= gj) { C[(long)(gi + e) * ld + gj] = h; C[pl + (long)(gi + e) * ld + gj] = l; }
-  }
-  if (!diag) {
-    *reinterpret_cast<half4*>(C + (long)gj * ld + gi) = hh;
-    *reinterpret_cast<half4*>(C + pl + (long)gj * ld + gi) = ll;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (gi + e > gj) { C[(long)gj * ld + gi + e] = hh[e]; C[pl + (long)gj * ld + gi + e] = ll[e]; }
-  }
-}
+// Chain matrices are stored in blocks of 16 columns, [column / 16][row][16]: a K step of any run of rows is contiguous, so that the
+// transfers to LDS move whole kilobytes (row by row they took 32 or 64 bytes of a line at a time: chain launches of 10 us, apply 337 us)
+__device__ __forceinline__ long cat(long Mp, int i, int j) { return ((long)(j >> 4) * Mp + i) * 16 + (j & 15); }
 
 // tile number of the lower triangle (bi >= bj), row by row
 __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
@@ -545,17 +521,35 @@ __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, con
     const float4 f = src[(long)s * ntri * (GT * GT / 4)];
     v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
   }
+  const int i0 = bi * 32 + 8 * q + 4 * (lane >> 5), j0 = bj * 32 + (lane & 31);
+  const long pl = (long)m.Mp * m.Mp;
+  _Float16* G = ws + m.g;
+  half4 hh, ll;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] *= c2;
-  put_sym(ws + m.g, (long)m.Mp * m.Mp, m.Mp, bi * 32 + 8 * q + 4 * (lane >> 5), bj * 32 + (lane & 31), bi == bj, v);
+  for (int e = 0; e < 4; ++e) {
+    _Float16 h, l;
+    split16(v[e] * c2, h, l);
+    hh[e] = h; ll[e] = l;
+    if (i0 + e >= j0) { G[cat(m.Mp, i0 + e, j0)] = h; G[pl + cat(m.Mp, i0 + e, j0)] = l; }
+  }
+  if (bi != bj) {
+    *reinterpret_cast<half4*>(G + cat(m.Mp, j0, i0)) = hh;
+    *reinterpret_cast<half4*>(G + pl + cat(m.Mp, j0, i0)) = ll;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i0 + e > j0) { G[cat(m.Mp, j0, i0 + e)] = hh[e]; G[pl + cat(m.Mp, j0, i0 + e)] = ll[e]; }
+  }
 }
 
 // chain planes of a matrix: 0 G, 1 Q, 2 Q G, 3 P, 4 the other P  (hi and lo each)
 // C = A B of commuting symmetric matrices: the lower triangle of 64 x 64 tiles, mirrored.  `quad`: C = a I + b A + c A A
+// 4 waves of 32 x 32; K in steps of 32 (two blocks) through four LDS stages of 16 KB, two workgroups per CU: such a product is a
+// few microseconds of latency, the depth covers it.  The tile leaves through LDS in both orientations, 2 KB runs.
 struct ChainJob { int a, b, c; float mul; int quad; };
 __global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
-  typedef NtCore<CT, CT, 2, 32, 4> Core;
-  __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
+  constexpr int ST = 4, STAGE = 16384;               // [operand][plane][block][64 rows][16]
+  __shared__ __attribute__((aligned(1024))) char smem[ST * STAGE];
   const int t = xcd_tile(blockIdx.x, total, 36);
   if (t < 0) return;
   const ChainJob jb = t >= tiles ? j1 : j0;          // two jobs: the second one's tiles come behind the first one's
@@ -563,26 +557,100 @@ __global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, Chai
   const NsMat& m = r.m;
   int bi, bj;
   tri(r.tile, bi, bj);
-  const long pl = (long)m.Mp * m.Mp;
+  const long Mp = m.Mp, pl = Mp * Mp;
   const _Float16* A = ws + m.g + jb.a * 2 * pl;
   const _Float16* B = ws + m.g + jb.b * 2 * pl;
   _Float16* C = ws + m.g + jb.c * 2 * pl;
-  Core c;
-  c.run(smem, A + (long)bi * CT * m.Mp, pl, m.Mp, CT, B + (long)bj * CT * m.Mp, pl, m.Mp, CT, 0, m.Mp);
-  c.each4([&](int i, int j, const float (&v)[4]) {
-    const int gi = bi * CT + i, gj = bj * CT + j;
-    float u[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
+  const _Float16* src[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      u[e] = v[e] * jb.mul;
-      if (jb.quad) {
-        const long at = (long)(gi + e) * m.Mp + gj;
-        u[e] += NS_B * ((float)A[at] + (float)A[pl + at]);
-        if (gi + e == gj) u[e] += NS_A * (float)(1 << SG);
+  for (int q = 0; q < 4; ++q) {                      // transfer x of a stage: operand x >> 3, plane, block, half of the rows
+    const int x = q * 4 + wave, row = (x & 1) * 32 + (lane >> 1);
+    src[q] = ((x >> 3) ? B : A) + ((x >> 2) & 1) * pl + (((x >> 1) & 1) * Mp + ((x >> 3) ? bj : bi) * CT + row) * 16 +
+             ((lane & 1) ^ swz<2>(row)) * 8;
+  }
+  const long step = 32 * Mp;
+  auto issue = [&](int st) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { dma16(src[q], smem + st * STAGE + (q * 4 + wave) * 1024); src[q] += step; }
+  };
+  f32x16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  const int n = m.Mp / 32;
+  const unsigned lds0 = (unsigned)(size_t)smem;
+  const int l31 = lane & 31;
+  const unsigned off = (unsigned)(l31 * 32 + (((lane >> 5) ^ swz<2>(l31)) << 4));
+  const unsigned pa = lds0 + wm * 32 + off, pb = lds0 + 8192 + wn * 32 + off;
+#pragma unroll
+  for (int q = 0; q < ST - 1; ++q)
+    if (q < n) issue(q);
+  for (int it = 0; it < n; ++it) {
+    if (it + ST - 2 < n) wait_dma<4 * (ST - 2)>();
+    else wait_dma<0>();
+    wg_barrier();
+    if (it + ST - 1 < n) issue((it + ST - 1) & (ST - 1));
+    const unsigned so = (unsigned)((it & (ST - 1)) * STAGE);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      half8 a[2], b[2];
+      fetch_1x1<4096>(pa + so + ks * 2048, pb + so + ks * 2048, a, b);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], acc, 0, 0, 0);
+    }
+  }
+  __syncthreads();
+  // image of the tile: [orientation][plane][4 blocks][64 rows][16]
+  _Float16* img = reinterpret_cast<_Float16*>(smem);
+  const bool diag = bi == bj;
+  const int j = wn + l31;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int i = wm + 8 * q + 4 * (lane >> 5);
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = acc[4 * q + e] * jb.mul;
+    if (jb.quad) {                                   // A[i][j] from A[j][i]: four neighbours
+      const long at = cat(Mp, bj * CT + j, bi * CT + i);
+      const half4 h = *reinterpret_cast<const half4*>(A + at), l = *reinterpret_cast<const half4*>(A + pl + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] += NS_B * ((float)h[e] + (float)l[e]);
+        if (diag && i + e == j) v[e] += NS_A * (float)(1 << SG);
       }
     }
-    put_sym(C, pl, m.Mp, gi, gj, bi == bj, u);
-  });
+    half4 hh, ll;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      _Float16 h, l;
+      split16(v[e], h, l);
+      hh[e] = h; ll[e] = l;
+      if (!diag || i + e >= j) {
+        const int at = (int)cat(64, i + e, j);
+        img[at] = h; img[4096 + at] = l;
+      }
+      if (diag && i + e > j) {
+        const int at = (int)cat(64, j, i + e);
+        img[at] = h; img[4096 + at] = l;
+      }
+    }
+    if (!diag) {
+      const int at = (int)cat(64, j, i);
+      *reinterpret_cast<half4*>(img + 8192 + at) = hh;
+      *reinterpret_cast<half4*>(img + 12288 + at) = ll;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int x = q * 256 + tid, im = x >> 9, blk = (x >> 7) & 3, in = x & 127;
+    if (im >= 2 && diag) break;
+    const int rb = im < 2 ? bi : bj, cb = im < 2 ? bj : bi;
+    *reinterpret_cast<uint4*>(C + (im & 1) * pl + ((cb * 4 + blk) * Mp + rb * CT) * 16 + in * 8) =
+        *reinterpret_cast<const uint4*>(img + im * 4096 + blk * 1024 + in * 8);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- X <- P X
@@ -622,6 +690,11 @@ __device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned 
 
 // A tile is 128 rows x 256 columns: 4 waves side by side, 128 x 64 each (per K step 12 KB of LDS reads for 24 MFMAs; 64 x 64 would need
 // two thirds more), K steps of 16 through three stages: 72 KB, two workgroups per CU, whose epilogues run under each other's products.
+__device__ __forceinline__ void muon_update(const NsStep& s, long at, float keep, float step, float o) {
+  const float p = s.p[at] * keep - step * o;
+  s.p[at] = p;
+  if (s.pb) s.pb[at] = (bf16_t)(ns_pack_bf16(p, 0.f) & 0xffffu);
+}
 template <int PX, int OUT>
 __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int total, const ApplyK k) {
   constexpr int A_BYTES = AI * 2 * 32, B_BYTES = 16 * AJ * 2 * PX, STAGE = A_BYTES + B_BYTES, ST = 3;
@@ -645,13 +718,13 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  // P: 32 rows of two chunks per transfer; X: two rows of 32 chunks, chunk c of row k at slot c ^ ((k & 3) << 2) for the transposing reads.
+  // P: 32 rows of a block per transfer; X: two rows of 32 chunks, chunk c of row k at slot c ^ ((k & 3) << 2) for the transposing reads.
   // Rows and columns behind the matrix read its last ones: products that nobody stores.
   const _Float16* as[PA];
 #pragma unroll
   for (int q = 0; q < PA; ++q) {
     const int row = (q * 4 + wave) * 32 + (lane >> 1), plane = row / AI, lr = min(i0 + row - plane * AI, m.Mp - 1);
-    as[q] = P + plane * pl + (long)lr * m.Mp + ((lane & 1) ^ swz<2>(row)) * 8;
+    as[q] = P + plane * pl + (long)lr * 16 + ((lane & 1) ^ swz<2>(row)) * 8;
   }
   const _Float16* bs[PB];
 #pragma unroll
@@ -660,10 +733,10 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
     const int col = min(j0 + (((lane & 31) ^ ((kr & 3) << 2)) * 8), m.Np - 8);
     bs[q] = X + plane * xpl + (long)kr * m.Np + col;
   }
-  const long bstep = 16L * m.Np;
+  const long astep = 16L * m.Mp, bstep = 16L * m.Np;
   auto issue = [&](int st) {
 #pragma unroll
-    for (int q = 0; q < PA; ++q) { dma16(as[q], smem + st * STAGE + (q * 4 + wave) * 1024); as[q] += 16; }
+    for (int q = 0; q < PA; ++q) { dma16(as[q], smem + st * STAGE + (q * 4 + wave) * 1024); as[q] += astep; }
 #pragma unroll
     for (int q = 0; q < PB; ++q) { dma16(bs[q], smem + st * STAGE + A_BYTES + (q * 4 + wave) * 1024); bs[q] += bstep; }
   };
@@ -695,53 +768,114 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][j], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][i], b[0][j], acc[i][j], 0, 0, 0);
-        if constexpr (PX == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[1][j], acc[i][j], 0, 0, 0);
+        // the transposed product: a lane holds one row of the result and runs of four of its columns
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[0][j], a[0][i], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[0][j], a[1][i], acc[i][j], 0, 0, 0);
+        if constexpr (PX == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[1][j], a[0][i], acc[i][j], 0, 0, 0);
       }
     cur = cur == ST - 1 ? 0 : cur + 1;
     nxt = nxt == ST - 1 ? 0 : nxt + 1;
   }
   const float f = (k.cfac ? k.cfac[r.id] : k.cconst) * k.mul;
   const float keep = 1.f - k.s.lr * k.s.wd, step = k.s.lr * m.scale;
+  if (OUT != 0 && m.tall) {
+    // the stored row is the long side: 32 neighbouring lanes hold 32 neighbours of a stored row
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int gj = j0 + wn + j * 32 + (lane & 31);
-    if constexpr (OUT == 0) {
-      if (gj >= m.Np) continue;
-    } else {
-      if (gj >= m.N) continue;
+    for (int i = 0; i < 4; ++i) {
+      const int gi = i0 + i * 32 + (lane & 31);
+      if (gi >= m.M) continue;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int gj = j0 + wn + j * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+          if (gj >= m.N) continue;
+          const float v = acc[i][j][e] * f;
+          if constexpr (OUT == 1) reinterpret_cast<float*>(k.out)[r.out + (long)gj * k.ldo + gi] = v;
+          else if constexpr (OUT == 2) reinterpret_cast<bf16_t*>(k.out)[r.out + (long)gj * k.ldo + gi] = (bf16_t)(ns_pack_bf16(v, 0.f) & 0xffffu);
+          else muon_update(k.s, ns_at(m, gj, gi), keep, step, v);
+        }
     }
-    // wide: the column is the lane's for all rows; tall: it is the stored row
-    const long cbase = OUT == 0 ? (long)gj : m.tall ? 0L : ns_at(m, 0, gj);
+    return;
+  }
+  // 32 rows at a time through LDS (rows of 264 floats: both the writes and the reads meet every bank once): a wave then handles whole rows, four
+  // neighbours per lane
+  float* buf = reinterpret_cast<float*>(smem);
+  const int c = lane * 4, gj = j0 + c;
+  const long cbase = OUT == 3 && gj < m.N ? ns_at(m, 0, gj) : 0;
+  const bool four = gj + 4 <= m.N && (OUT != 3 || (m.cols & 3) == 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4; ++i) {
+    float4 p[8];
+    if constexpr (OUT == 3) {
+      if (four) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int ii = i0 + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-        const float v = acc[i][j][e] * f;
-        if constexpr (OUT == 0) {
-          if (ii < m.Mp) {
-            _Float16 h, l;
-            split16(v, h, l);
-            _Float16* o = k.wso + m.x + (long)ii * m.Np + gj;
-            o[0] = h; o[xpl] = l;
-          }
-        } else {
-          if (ii < m.M) {
-            if constexpr (OUT == 3) {
-              const long at = m.tall ? ns_at(m, gj, ii) : cbase + (long)ii * m.ld;
-              const float p = k.s.p[at] * keep - step * v;
-              k.s.p[at] = p;
-              if (k.s.pb) k.s.pb[at] = (bf16_t)(ns_pack_bf16(p, 0.f) & 0xffffu);
-            } else {
-              const long at = r.out + (m.tall ? (long)gj * k.ldo + ii : (long)ii * k.ldo + gj);
-              if constexpr (OUT == 1) reinterpret_cast<float*>(k.out)[at] = v;
-              else reinterpret_cast<bf16_t*>(k.out)[at] = (bf16_t)(ns_pack_bf16(v, 0.f) & 0xffffu);
-            }
+        for (int t = 0; t < 8; ++t) {
+          const int gi = i0 + i * 32 + wave * 8 + t;
+          if (gi < m.M) {
+            const NsU4 u = *reinterpret_cast<const NsU4*>(k.s.p + cbase + (long)gi * m.ld);
+            p[t] = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
           }
         }
       }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<float4*>(buf + (lane & 31) * 264 + wn + j * 32 + 8 * q + 4 * (lane >> 5)) =
+            make_float4(acc[i][j][4 * q] * f, acc[i][j][4 * q + 1] * f, acc[i][j][4 * q + 2] * f, acc[i][j][4 * q + 3] * f);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const int gi = i0 + i * 32 + wave * 8 + t;
+      const float4 v = *reinterpret_cast<const float4*>(buf + (wave * 8 + t) * 264 + c);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      if constexpr (OUT == 0) {
+        if (gi < m.Mp && gj < m.Np) {
+          half4 h, l;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { _Float16 th, tl; split16(x[e], th, tl); h[e] = th; l[e] = tl; }
+          _Float16* o = k.wso + m.x + (long)gi * m.Np + gj;
+          *reinterpret_cast<half4*>(o) = h;
+          *reinterpret_cast<half4*>(o + xpl) = l;
+        }
+      } else if (gi < m.M && four) {
+        if constexpr (OUT == 3) {
+          const long at = cbase + (long)gi * m.ld;
+          const float y[4] = {p[t].x * keep - step * x[0], p[t].y * keep - step * x[1], p[t].z * keep - step * x[2], p[t].w * keep - step * x[3]};
+          NsU4 u;
+          u.x = __float_as_uint(y[0]); u.y = __float_as_uint(y[1]); u.z = __float_as_uint(y[2]); u.w = __float_as_uint(y[3]);
+          *reinterpret_cast<NsU4*>(k.s.p + at) = u;
+          if (k.s.pb) {
+            NsU2 b;
+            b.x = ns_pack_bf16(y[0], y[1]); b.y = ns_pack_bf16(y[2], y[3]);
+            *reinterpret_cast<NsU2*>(k.s.pb + at) = b;
+          }
+        } else {
+          const long at = r.out + (long)gi * k.ldo + gj;
+          if constexpr (OUT == 1) {
+            NsU4 u;
+            u.x = __float_as_uint(x[0]); u.y = __float_as_uint(x[1]); u.z = __float_as_uint(x[2]); u.w = __float_as_uint(x[3]);
+            *reinterpret_cast<NsU4*>(reinterpret_cast<float*>(k.out) + at) = u;
+          } else {
+            NsU2 b;
+            b.x = ns_pack_bf16(x[0], x[1]); b.y = ns_pack_bf16(x[2], x[3]);
+            *reinterpret_cast<NsU2*>(reinterpret_cast<bf16_t*>(k.out) + at) = b;
+          }
+        }
+      } else if (gi < m.M) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (gj + e >= m.N) break;
+          const long at = r.out + (long)gi * k.ldo + gj + e;
+          if constexpr (OUT == 1) reinterpret_cast<float*>(k.out)[at] = x[e];
+          else if constexpr (OUT == 2) reinterpret_cast<bf16_t*>(k.out)[at] = (bf16_t)(ns_pack_bf16(x[e], 0.f) & 0xffffu);
+          else muon_update(k.s, ns_at(m, gi, gj + e), keep, step, x[e]);
+        }
+      }
+    }
   }
 }
 
@@ -772,7 +906,7 @@ struct NsCounts { long n0, n1, ng, nr, nc, na, x, g, part; };
 static NsCounts ns_counts(NsMat& m, long others, bool flat) {
   NsCounts c;
   const long n = (long)m.taps * m.rows * m.cols;
-  c.n0 = flat ? cdiv(n, K0_ELEMS) : cdiv((long)m.rows * cdiv(m.cols, 8), K0_ELEMS / 8);
+  c.n0 = flat ? cdiv(n, k0_elems(n)) : cdiv((long)m.rows * cdiv(m.cols, 8), SQ_RUNS);
   m.np = (int)c.n0;
   if (m.kind == 1) { c.n1 = c.ng = c.nr = c.nc = c.na = c.x = c.g = c.part = 0; return c; }
   c.n1 = m.tall ? (long)(m.Mp / 64) * (m.Np / 64) : cdiv((long)m.Mp * m.Np / 8, 1024);
