@@ -19,8 +19,11 @@
 // is 2^-25 of the rms.  |G|, |Q G| <= 1.5, |Q| <= 3.45, |P| <= 3.45^3 = 41 bound the others' scales.  A bf16 input is one fp16 value exactly (8 bits): one plane.
 //
 // Layout.  A matrix is stored by the caller as [taps][rows][cols] with row and tap strides (a packed convolution weight is one matrix
-// [rows, taps * cols]); the planes here are [M][N], M <= N the short side, both padded with zeros to multiples of 64: no product checks
-// a bound along K, and padding stays zero through every step.  All matrices of a call share every launch (a device table of tile ranges).
+// [rows, taps * cols]).  The planes here are M x N, M <= N the short side, both padded with zeros to multiples of 64: no product checks
+// a bound along K, and padding stays zero through every step.  They (and the m x m matrices) are stored in blocks of 16 columns,
+// [column / 16][row][16], the rows of a block padded by 8: what a product needs next of any run of rows is contiguous, and neighbouring blocks
+// begin on different L2 channels.  (Row-major planes, whose rows lie a large power of two apart, held every product at 6.5 TB/s of operands.)
+// All matrices of a call share every launch (a device table of tile ranges).
 #include "common.h"
 #include <math.h>
 #include <vector>
@@ -46,22 +49,24 @@ struct NsMat {
   int np;                       // partial sums of squares
   float scale;
   long x, g, part;              // offsets in the workspace: X planes and chain planes (halves), Gram partials (floats)
-  int b0, b1, bg, br, bc, ba;   // first workgroup in: momentum, split, Gram, its join, chain, apply
+  int sq0;                      // first partial sum of squares
 };
+enum { F_MOM, F_SPLIT, F_GRAM, F_JOIN, F_CHAIN, F_APPLY, F_N };       // launches
 struct NsGroup {                // matrices of one call: a device table, or (tab = nullptr) `n` equal ones
   const NsMat* tab;
+  const int* first;             // [F_N][n]: the first workgroup of each record
   int n;
   NsMat u;                      // the single record of equal matrices: offsets of number 0
   long src_step, out_step, x_step, g_step, part_step;
-  int n0, n1, ng, nr, nc, na;   // workgroups per matrix
+  int per[F_N];                 // workgroups per matrix
 };
 struct NsRef { NsMat m; int id, tile; long out; };
 
-template <int NsMat::*FIRST, int NsGroup::*PER>
+template <int F>
 __device__ __forceinline__ NsRef ns_find(const NsGroup& gr, int b) {
   NsRef r;
   if (gr.tab == nullptr) {
-    const int per = gr.*PER;
+    const int per = gr.per[F];
     r.id = b / per;
     r.tile = b - r.id * per;
     r.m = gr.u;
@@ -70,15 +75,17 @@ __device__ __forceinline__ NsRef ns_find(const NsGroup& gr, int b) {
     r.m.x += (long)r.id * gr.x_step; r.m.g += (long)r.id * gr.g_step; r.m.part += (long)r.id * gr.part_step;
     return r;
   }
-  int lo = 0, hi = gr.n - 1;    // the last record whose range begins at or before b
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (gr.tab[mid].*FIRST <= b) lo = mid;
-    else hi = mid - 1;
+  // the last record whose range begins at or before b: 64 at a time, one load and a vote
+  int id = -1;
+  for (int c = 0; c < gr.n; c += 64) {
+    const int i = c + (int)(threadIdx.x & 63);
+    const unsigned long long vote = __ballot(i < gr.n && gr.first[F * gr.n + i] <= b);
+    id += __popcll(vote);
+    if (~vote) break;
   }
-  r.id = lo;
-  r.m = gr.tab[lo];
-  r.tile = b - r.m.*FIRST;
+  r.id = __builtin_amdgcn_readfirstlane(id);
+  r.m = gr.tab[r.id];
+  r.tile = b - gr.first[F * gr.n + r.id];
   r.out = r.m.src;
   return r;
 }
@@ -103,11 +110,13 @@ __device__ __forceinline__ double block_sum_d256(double v, double* red) {
 }
 
 // ---------------------------------------------------------------------------------------------- table upload
-struct NsChunk { NsMat m[16]; };
-__global__ void ns_table_kernel(NsChunk c, NsMat* tab, int n) {
+// the table travels in kernel arguments: nothing of the caller's memory is read after the call, and a captured graph keeps its copy
+struct NsChunk { NsMat m[16]; int first[F_N][16]; };
+__global__ void ns_table_kernel(NsChunk c, NsMat* tab, int* first, int at, int n, int total) {
   const int words = (int)(sizeof(NsMat) / 4);
-  for (int i = threadIdx.x; i < n * words; i += 64)
-    reinterpret_cast<unsigned*>(tab)[i] = reinterpret_cast<const unsigned*>(&c)[i];
+  for (int i = threadIdx.x; i < n * words; i += 256)
+    reinterpret_cast<unsigned*>(tab + at)[i] = reinterpret_cast<const unsigned*>(&c)[i];
+  for (int i = threadIdx.x; i < n * F_N; i += 256) first[(i / n) * total + at + i % n] = c.first[i / n][i % n];
 }
 
 // ---------------------------------------------------------------------------------------------- momentum, Adam, sums of squares
@@ -126,7 +135,7 @@ __device__ __forceinline__ float ns_update(const NsStep& s, float g, float m1) {
 // one workgroup = k0_elems consecutive elements of a tensor; 28 bytes / element for Adam's, 12 for a matrix's
 __global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, const NsStep s, double* sq) {
   __shared__ double red[4];
-  const NsRef r = ns_find<&NsMat::b0, &NsGroup::n0>(gr, blockIdx.x);
+  const NsRef r = ns_find<F_MOM>(gr, blockIdx.x);
   const long n = (long)r.m.taps * r.m.rows * r.m.cols;
   const long e0 = (long)r.tile * k0_elems(n), e1 = min(n, e0 + k0_elems(n));
   const long base = r.m.src;
@@ -247,7 +256,7 @@ constexpr int SQ_RUNS = 512;
 template <int SRC>
 __global__ __launch_bounds__(256) void ns_sumsq_kernel(const NsGroup gr, const void* x, double* sq) {
   __shared__ double red[4];
-  const NsRef r = ns_find<&NsMat::b0, &NsGroup::n0>(gr, blockIdx.x);
+  const NsRef r = ns_find<F_MOM>(gr, blockIdx.x);
   const unsigned rpr = (unsigned)(r.m.cols + 7) / 8u;
   const unsigned n = (unsigned)r.m.rows * rpr;
   const unsigned e0 = (unsigned)r.tile * SQ_RUNS, e1 = min(n, e0 + SQ_RUNS);
@@ -264,6 +273,11 @@ __global__ __launch_bounds__(256) void ns_sumsq_kernel(const NsGroup gr, const v
   if (threadIdx.x == 0) sq[blockIdx.x] = acc;
 }
 
+// element (i, j) of a plane in blocks of 16 columns; planes of X and of an m x m matrix
+__device__ __forceinline__ long cat(int Mp, int i, int j) { return ((long)(j >> 4) * (Mp + 8) + i) * 16 + (j & 15); }
+__device__ __forceinline__ long xplane(const NsMat& m) { return (long)m.Np * (m.Mp + 8); }
+__device__ __forceinline__ long cplane(const NsMat& m) { return (long)m.Mp * (m.Mp + 8); }
+
 // ---------------------------------------------------------------------------------------------- split into fp16 planes
 // every workgroup joins its matrix's partial sums of squares itself (a few hundred doubles); the first one publishes
 // c = 2^k / (|U| + eps), the factor from the planes' units to X0's
@@ -273,11 +287,11 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
   __shared__ double red[4];
   __shared__ float tile[64][65];
   constexpr bool ONE = SRC == 1;
-  const NsRef r = ns_find<&NsMat::b1, &NsGroup::n1>(gr, blockIdx.x);
+  const NsRef r = ns_find<F_SPLIT>(gr, blockIdx.x);
   const NsMat& m = r.m;
   const long n = (long)m.taps * m.rows * m.cols;
   const int np = m.np;
-  const int first = gr.tab ? m.b0 : r.id * gr.n0;
+  const int first = gr.tab ? m.sq0 : r.id * gr.per[F_MOM];
   double a = 0.0;
   for (int i = threadIdx.x; i < np; i += 256) a += sq[first + i];
   a = block_sum_d256(a, red);
@@ -289,16 +303,15 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
   const float f = (float)ldexp(1.0, -k);
   if (r.tile == 0 && threadIdx.x == 0) cfac[r.id] = norm == 0.0 ? 0.f : (float)(ldexp(1.0, k) / (norm + (double)eps));
   _Float16* hi = ws + m.x;
-  _Float16* lo = hi + (long)m.Mp * m.Np;
+  _Float16* lo = hi + xplane(m);
   if (!m.tall) {
-    // 1024 chunks of 8 plane elements per workgroup
-    const int cpr = m.Np / 8;
-    const long nch = (long)m.Mp * cpr;
+    // 64 rows x 128 columns: 8 plane elements per thread and trip, 1 KB runs per wave
+    const int tr = m.Mp / 64;
+    const int i = (r.tile % tr) * 64 + ((threadIdx.x >> 1) & 63), jt = (r.tile / tr) * 128 + (threadIdx.x & 1) * 8 + (threadIdx.x >> 7) * 16;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const long ch = (long)r.tile * 1024 + q * 256 + threadIdx.x;
-      if (ch >= nch) break;
-      const int i = (int)(ch / cpr), j = (int)(ch - (long)i * cpr) * 8;
+      const int j = jt + q * 32;
+      if (j >= m.Np) break;
       float v[8];
       if (i < m.M && j < m.N) {
         ns_load8<SRC>(m, x, s, i, j, v);
@@ -309,8 +322,8 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
       half8 h, l;
 #pragma unroll
       for (int e = 0; e < 8; ++e) { _Float16 th, tl; split16(v[e] * f, th, tl); h[e] = th; l[e] = tl; }
-      *reinterpret_cast<half8*>(hi + (long)i * m.Np + j) = h;
-      if constexpr (!ONE) *reinterpret_cast<half8*>(lo + (long)i * m.Np + j) = l;
+      *reinterpret_cast<half8*>(hi + cat(m.Mp, i, j)) = h;
+      if constexpr (!ONE) *reinterpret_cast<half8*>(lo + cat(m.Mp, i, j)) = l;
     }
   } else {
     // 64 x 64 tile through LDS: plane row i = stored flat column, plane column j = stored row
@@ -324,12 +337,12 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int c = q * 256 + threadIdx.x, i = c >> 3, j = (c & 7) * 8;
+      const int c = q * 256 + threadIdx.x, i = (c >> 1) & 63, j = (c & 1) * 8 + (c >> 7) * 16;
       half8 h, l;
 #pragma unroll
       for (int e = 0; e < 8; ++e) { _Float16 th, tl; split16(tile[j + e][i] * f, th, tl); h[e] = th; l[e] = tl; }
-      *reinterpret_cast<half8*>(hi + (long)(i0 + i) * m.Np + j0 + j) = h;
-      if constexpr (!ONE) *reinterpret_cast<half8*>(lo + (long)(i0 + i) * m.Np + j0 + j) = l;
+      *reinterpret_cast<half8*>(hi + cat(m.Mp, i0 + i, j0 + j)) = h;
+      if constexpr (!ONE) *reinterpret_cast<half8*>(lo + cat(m.Mp, i0 + i, j0 + j)) = l;
     }
   }
 }
@@ -348,8 +361,8 @@ __device__ __forceinline__ int xcd_tile(int b, int total, int grp) {
   return (r >> 3) < g2 && t < total ? t : -1;
 }
 
-// LDS image of an operand with K contiguous: rows of BK halves = CH 16-byte chunks; chunk c of row r at slot c ^ ((r CH / 16) % CH): the 16
-// lanes that a ds_read_b128 serves at a time (16 consecutive rows, one chunk) then cover the 256 bytes of a bank row once.
+// LDS image of an operand: blocks of [rows][16], a row = two 16-byte chunks, chunk c of row r at slot c ^ ((r >> 3) & 1): the 16 lanes
+// that a ds_read_b128 serves at a time (16 consecutive rows, one chunk) then cover the 256 bytes of a bank row once.
 // Tiles go global -> LDS without registers (one instruction = 64 lanes x 16 bytes = 1 KB in LDS order), ST stages deep; the operand
 // reads of a K step and their wait are ONE asm block: the compiler, which would wait for every transfer in flight before any LDS
 // read, does not see them, and nothing can come between a read and its wait.  The other waves of the SIMD cover that wait.
@@ -362,106 +375,107 @@ __device__ __forceinline__ void wg_barrier() {
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
 }
-template <int CH>
-__device__ __forceinline__ int swz(int row) { return (row * CH / 16) % CH; }
+__device__ __forceinline__ int swz(int row) { return (row >> 3) & 1; }
 
-// one K step (16) of TM + TN fragments: rows 32 apart (RB bytes each), planes PS bytes apart
+// one K step (16) of T + T fragments, 32 rows (1 KB) apart, planes PS bytes apart
 #define NS_RD "ds_read_b128 "
 template <int PS>
-__device__ __forceinline__ void fetch_1x1(unsigned pa, unsigned pb, half8 (&a)[2], half8 (&b)[2]) {
+__device__ __forceinline__ void fetch_nt(unsigned pa, unsigned pb, half8 (&a)[2][1], half8 (&b)[2][1]) {
   asm volatile(NS_RD "%0, %4\n\t" NS_RD "%2, %5\n\t" NS_RD "%1, %4 offset:%6\n\t" NS_RD "%3, %5 offset:%6\n\t" "s_waitcnt lgkmcnt(0)"
-               : "=&v"(a[0]), "=&v"(a[1]), "=&v"(b[0]), "=&v"(b[1]) : "v"(pa), "v"(pb), "n"(PS) : "memory");
+               : "=&v"(a[0][0]), "=&v"(a[1][0]), "=&v"(b[0][0]), "=&v"(b[1][0]) : "v"(pa), "v"(pb), "n"(PS) : "memory");
 }
-template <int RB, int PSA, int PSB>
-__device__ __forceinline__ void fetch_2x2(unsigned pa, unsigned pb, half8 (&a)[2][2], half8 (&b)[2][2]) {
-  asm volatile(NS_RD "%0, %8\n\t" NS_RD "%4, %9\n\t" NS_RD "%1, %8 offset:%10\n\t" NS_RD "%5, %9 offset:%10\n\t"
-               NS_RD "%2, %8 offset:%11\n\t" NS_RD "%3, %8 offset:%12\n\t" NS_RD "%6, %9 offset:%13\n\t" NS_RD "%7, %9 offset:%14\n\t"
+template <int PS>
+__device__ __forceinline__ void fetch_nt(unsigned pa, unsigned pb, half8 (&a)[2][2], half8 (&b)[2][2]) {
+  asm volatile(NS_RD "%0, %8\n\t" NS_RD "%4, %9\n\t" NS_RD "%1, %8 offset:1024\n\t" NS_RD "%5, %9 offset:1024\n\t"
+               NS_RD "%2, %8 offset:%10\n\t" NS_RD "%3, %8 offset:%11\n\t" NS_RD "%6, %9 offset:%10\n\t" NS_RD "%7, %9 offset:%11\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(b[0][0]), "=&v"(b[0][1]), "=&v"(b[1][0]), "=&v"(b[1][1])
-               : "v"(pa), "v"(pb), "n"(32 * RB), "n"(PSA), "n"(PSA + 32 * RB), "n"(PSB), "n"(PSB + 32 * RB) : "memory");
+               : "v"(pa), "v"(pb), "n"(PS), "n"(PS + 1024) : "memory");
 }
-template <int RB>
-__device__ __forceinline__ void fetch_2x2(unsigned pa, unsigned pb, half8 (&a)[1][2], half8 (&b)[1][2]) {
-  asm volatile(NS_RD "%0, %4\n\t" NS_RD "%2, %5\n\t" NS_RD "%1, %4 offset:%6\n\t" NS_RD "%3, %5 offset:%6\n\t" "s_waitcnt lgkmcnt(0)"
-               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(b[0][0]), "=&v"(b[0][1]) : "v"(pa), "v"(pb), "n"(32 * RB) : "memory");
+template <int PS>
+__device__ __forceinline__ void fetch_nt(unsigned pa, unsigned pb, half8 (&a)[1][2], half8 (&b)[1][2]) {
+  asm volatile(NS_RD "%0, %4\n\t" NS_RD "%2, %5\n\t" NS_RD "%1, %4 offset:1024\n\t" NS_RD "%3, %5 offset:1024\n\t" "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(b[0][0]), "=&v"(b[0][1]) : "v"(pa), "v"(pb) : "memory");
 }
 
-// C[BM][BN] = sum_k A[i][k] B[j][k], operands as PL fp16 planes; 4 waves (2 x 2), K in steps of BK, ST LDS stages.
-// Rows behind a_rows / b_rows read the last one instead: their products belong to rows and columns that nobody stores.
-template <int BM, int BN, int PL, int BK, int ST>
+// C[BM][BM] = sum_k A[i][k] B[j][k] over columns k0 .. k1 - 1 (multiples of 32), operands as PL fp16 planes in blocks; 4 waves (2 x 2), two
+// blocks per stage, ST stages.  `same`: A and B are the same rows, moved once.  Rows behind a_rows / b_rows read the last one instead:
+// their products belong to rows and columns that nobody stores.
+template <int BM, int PL, int ST>
 struct NtCore {
-  static constexpr int TM = BM / 64, TN = BN / 64, CH = BK / 8, RB = BK * 2, RPI = 1024 / RB;
-  static constexpr int A_BYTES = BM * PL * RB, STAGE = (BM + BN) * PL * RB;
-  static constexpr int NI = STAGE / 1024 / 4;                       // transfers per wave and stage
+  static constexpr int T = BM / 64, BLK = BM * 32, OP = PL * 2 * BLK, STAGE = 2 * OP;      // [operand][plane][block][BM][16]
+  static constexpr int NI = STAGE / 4096;                           // transfers per wave and stage
   static constexpr int LDS_BYTES = ST * STAGE;
-  static_assert(TM == 2 && TN == 2 && (BM % RPI) == 0 && (BN % RPI) == 0 && LDS_BYTES <= 80 * 1024, "tile");
-  f32x16 acc[TM][TN];
+  static_assert((T == 1 || T == 2) && LDS_BYTES <= 128 * 1024, "tile");
+  f32x16 acc[T][T];
 
-  __device__ __forceinline__ void run(char* smem, const _Float16* A, long a_plane, long lda, int a_rows, const _Float16* B, long b_plane,
-                                      long ldb, int b_rows, int k0, int k1) {
+  __device__ __forceinline__ void run(char* smem, const _Float16* A, int a_rows, const _Float16* B, int b_rows, long plane, int pitch, bool same,
+                                      int k0, int k1) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+    const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BM / 2);
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < T; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
+      for (int j = 0; j < T; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     const _Float16* src[NI];
 #pragma unroll
-    for (int q = 0; q < NI; ++q) {
-      const int row = (q * 4 + wave) * RPI + lane / CH, slot = lane % CH;
-      const bool isA = row < BM * PL;
-      const int rr = isA ? row : row - BM * PL;
-      const int pl = rr / (isA ? BM : BN), lr = rr - pl * (isA ? BM : BN);
-      const int c = slot ^ swz<CH>(row);
-      src[q] = (isA ? A + pl * a_plane + (long)min(lr, a_rows - 1) * lda : B + pl * b_plane + (long)min(lr, b_rows - 1) * ldb) + c * 8 + k0;
+    for (int q = 0; q < NI; ++q) {                   // transfer x of a stage: operand, plane, block, 32 rows
+      const int x = q * 4 + wave, op = x / (NI * 2), y = x % (BM / 32), z = x / (BM / 32) % (PL * 2);
+      const int row = y * 32 + (lane >> 1);
+      src[q] = (op ? B : A) + (z >> 1) * plane + ((long)(k0 / 16 + (z & 1)) * pitch + min(row, (op ? b_rows : a_rows) - 1)) * 16 +
+               ((lane & 1) ^ swz(row)) * 8;
     }
+    const long step = 32L * pitch;
     auto issue = [&](int st) {
 #pragma unroll
-      for (int q = 0; q < NI; ++q) { dma16(src[q], smem + st * STAGE + (q * 4 + wave) * 1024); src[q] += BK; }
+      for (int q = 0; q < NI; ++q) {
+        if (q == NI / 2 && same) break;
+        dma16(src[q], smem + st * STAGE + (q * 4 + wave) * 1024);
+        src[q] += step;
+      }
     };
-    const int n = (k1 - k0) / BK;
+    const int n = (k1 - k0) / 32;
     const unsigned lds0 = (unsigned)(size_t)smem;
     const int r = lane & 31;
-    const unsigned off0 = (unsigned)(((lane >> 5) ^ swz<CH>(r)) << 4);
-    const unsigned pa = lds0 + (wm + r) * RB + off0, pb = lds0 + A_BYTES + (wn + r) * RB + off0;
+    const unsigned off = (unsigned)(r * 32 + (((lane >> 5) ^ swz(r)) << 4));
+    const unsigned pa = lds0 + wm * 32 + off, pb = lds0 + (same ? 0 : OP) + wn * 32 + off;
 #pragma unroll
     for (int q = 0; q < ST - 1; ++q)
       if (q < n) issue(q);
     int cur = 0, nxt = ST - 1;
     for (int it = 0; it < n; ++it) {
-      if (it + ST - 2 < n) wait_dma<NI * (ST - 2)>();
-      else wait_dma<0>();
+      if (it + ST - 2 >= n) wait_dma<0>();
+      else if (same) wait_dma<NI / 2 * (ST - 2)>();
+      else wait_dma<NI * (ST - 2)>();
       wg_barrier();
       if (it + ST - 1 < n) issue(nxt);
       const unsigned so = (unsigned)(cur * STAGE);
 #pragma unroll
-      for (int ks = 0; ks < BK / 16; ++ks) {
-        half8 a[PL][TM], b[PL][TN];
-        const unsigned qa = ((pa ^ (unsigned)(ks << 5)) + so), qb = ((pb ^ (unsigned)(ks << 5)) + so);
-        if constexpr (PL == 2) fetch_2x2<RB, BM * RB, BN * RB>(qa, qb, a, b);
-        else fetch_2x2<RB>(qa, qb, a, b);
+      for (int ks = 0; ks < 2; ++ks) {
+        half8 a[PL][T], b[PL][T];
+        fetch_nt<2 * BLK>(pa + so + ks * BLK, pb + so + ks * BLK, a, b);
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < T; ++i)
 #pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][j], acc[i][j], 0, 0, 0);
-            if constexpr (PL == 2) {
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[1][j], acc[i][j], 0, 0, 0);
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][i], b[0][j], acc[i][j], 0, 0, 0);
-            }
-          }
+          for (int j = 0; j < T; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[0][j], acc[i][j], 0, 0, 0);
+        if constexpr (PL == 2) {
+#pragma unroll
+          for (int i = 0; i < T; ++i)
+#pragma unroll
+            for (int j = 0; j < T; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][i], b[PL - 1][j], acc[i][j], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < T; ++i)
+#pragma unroll
+            for (int j = 0; j < T; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[PL - 1][i], b[0][j], acc[i][j], 0, 0, 0);
+        }
       }
       cur = cur + 1 == ST ? 0 : cur + 1;
       nxt = nxt + 1 == ST ? 0 : nxt + 1;
     }
   }
 };
-
-// Chain matrices are stored in blocks of 16 columns, [column / 16][row][16]: a K step of any run of rows is contiguous, so that the
-// transfers to LDS move whole kilobytes (row by row they took 32 or 64 bytes of a line at a time: chain launches of 10 us, apply 337 us)
-__device__ __forceinline__ long cat(long Mp, int i, int j) { return ((long)(j >> 4) * Mp + i) * 16 + (j & 15); }
 
 // tile number of the lower triangle (bi >= bj), row by row
 __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
@@ -475,20 +489,19 @@ __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
 // G = X X^T over one slice of the long side: fp32 partial tiles, in the order of the accumulators (one float4 = four rows of a column)
 template <int PL>
 __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int total, const _Float16* ws, float* part) {
-  typedef NtCore<GT, GT, PL, 32, 2> Core;
+  typedef NtCore<GT, PL, 2> Core;
   __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
   const int b = xcd_tile(blockIdx.x, total, 10);
   if (b < 0) return;
-  const NsRef r = ns_find<&NsMat::bg, &NsGroup::ng>(gr, b);
+  const NsRef r = ns_find<F_GRAM>(gr, b);
   const NsMat& m = r.m;
   const int nt = (m.Mp + GT - 1) / GT, ntri = nt * (nt + 1) / 2;
   const int split = r.tile / ntri, t = r.tile - split * ntri;
   int bi, bj;
   tri(t, bi, bj);
   const _Float16* X = ws + m.x;
-  const long plane = (long)m.Mp * m.Np;
   Core c;
-  c.run(smem, X + (long)bi * GT * m.Np, plane, m.Np, m.Mp - bi * GT, X + (long)bj * GT * m.Np, plane, m.Np, m.Mp - bj * GT,
+  c.run(smem, X + (long)bi * GT * 16, m.Mp - bi * GT, X + (long)bj * GT * 16, m.Mp - bj * GT, xplane(m), m.Mp + 8, bi == bj,
         split * m.kc, min(m.Np, (split + 1) * m.kc));
   float4* out = reinterpret_cast<float4*>(part + m.part + (long)r.tile * (GT * GT));
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -504,7 +517,7 @@ __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int t
 
 // join of the slices, in order; both triangles of G from the lower one.  One workgroup = one 32 x 32 block, a float4 per thread
 __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, const float* part, const float* cfac, float cconst, _Float16* ws) {
-  const NsRef r = ns_find<&NsMat::br, &NsGroup::nr>(gr, blockIdx.x);
+  const NsRef r = ns_find<F_JOIN>(gr, blockIdx.x);
   const NsMat& m = r.m;
   int bi, bj;
   tri(r.tile, bi, bj);                               // in units of 32
@@ -522,7 +535,7 @@ __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, con
     v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
   }
   const int i0 = bi * 32 + 8 * q + 4 * (lane >> 5), j0 = bj * 32 + (lane & 31);
-  const long pl = (long)m.Mp * m.Mp;
+  const long pl = cplane(m);
   _Float16* G = ws + m.g;
   half4 hh, ll;
 #pragma unroll
@@ -544,66 +557,34 @@ __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, con
 
 // chain planes of a matrix: 0 G, 1 Q, 2 Q G, 3 P, 4 the other P  (hi and lo each)
 // C = A B of commuting symmetric matrices: the lower triangle of 64 x 64 tiles, mirrored.  `quad`: C = a I + b A + c A A
-// 4 waves of 32 x 32; K in steps of 32 (two blocks) through four LDS stages of 16 KB, two workgroups per CU: such a product is a
-// few microseconds of latency, the depth covers it.  The tile leaves through LDS in both orientations, 2 KB runs.
+// 4 waves of 32 x 32.  Such a product is a few microseconds of latency: ST = 4 stages (64 KB, two workgroups per CU), 8 where there is
+// at most one workgroup per CU.  The tile leaves through LDS in both orientations, 2 KB runs.
 struct ChainJob { int a, b, c; float mul; int quad; };
-__global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
-  constexpr int ST = 4, STAGE = 16384;               // [operand][plane][block][64 rows][16]
-  __shared__ __attribute__((aligned(1024))) char smem[ST * STAGE];
+template <int ST>
+__global__ __launch_bounds__(256, ST == 4 ? 2 : 1) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
+  typedef NtCore<CT, 2, ST> Core;
+  __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
   const int t = xcd_tile(blockIdx.x, total, 36);
   if (t < 0) return;
   const ChainJob jb = t >= tiles ? j1 : j0;          // two jobs: the second one's tiles come behind the first one's
-  const NsRef r = ns_find<&NsMat::bc, &NsGroup::nc>(gr, t >= tiles ? t - tiles : t);
+  const NsRef r = ns_find<F_CHAIN>(gr, t >= tiles ? t - tiles : t);
   const NsMat& m = r.m;
   int bi, bj;
   tri(r.tile, bi, bj);
-  const long Mp = m.Mp, pl = Mp * Mp;
+  const int Mp = m.Mp;
+  const long pl = cplane(m);
   const _Float16* A = ws + m.g + jb.a * 2 * pl;
   const _Float16* B = ws + m.g + jb.b * 2 * pl;
   _Float16* C = ws + m.g + jb.c * 2 * pl;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-  const _Float16* src[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {                      // transfer x of a stage: operand x >> 3, plane, block, half of the rows
-    const int x = q * 4 + wave, row = (x & 1) * 32 + (lane >> 1);
-    src[q] = ((x >> 3) ? B : A) + ((x >> 2) & 1) * pl + (((x >> 1) & 1) * Mp + ((x >> 3) ? bj : bi) * CT + row) * 16 +
-             ((lane & 1) ^ swz<2>(row)) * 8;
-  }
-  const long step = 32 * Mp;
-  auto issue = [&](int st) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) { dma16(src[q], smem + st * STAGE + (q * 4 + wave) * 1024); src[q] += step; }
-  };
-  f32x16 acc;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-  const int n = m.Mp / 32;
-  const unsigned lds0 = (unsigned)(size_t)smem;
-  const int l31 = lane & 31;
-  const unsigned off = (unsigned)(l31 * 32 + (((lane >> 5) ^ swz<2>(l31)) << 4));
-  const unsigned pa = lds0 + wm * 32 + off, pb = lds0 + 8192 + wn * 32 + off;
-#pragma unroll
-  for (int q = 0; q < ST - 1; ++q)
-    if (q < n) issue(q);
-  for (int it = 0; it < n; ++it) {
-    if (it + ST - 2 < n) wait_dma<4 * (ST - 2)>();
-    else wait_dma<0>();
-    wg_barrier();
-    if (it + ST - 1 < n) issue((it + ST - 1) & (ST - 1));
-    const unsigned so = (unsigned)((it & (ST - 1)) * STAGE);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      half8 a[2], b[2];
-      fetch_1x1<4096>(pa + so + ks * 2048, pb + so + ks * 2048, a, b);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], acc, 0, 0, 0);
-    }
-  }
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32, l31 = lane & 31;
+  Core core;
+  core.run(smem, A + (long)bi * CT * 16, CT, B + (long)bj * CT * 16, CT, pl, Mp + 8, bi == bj && jb.a == jb.b, 0, Mp);
+  const f32x16& acc = core.acc[0][0];
   __syncthreads();
   // image of the tile: [orientation][plane][4 blocks][64 rows][16]
   _Float16* img = reinterpret_cast<_Float16*>(smem);
+  auto im64 = [](int i, int j) { return ((j >> 4) * 64 + i) * 16 + (j & 15); };
   const bool diag = bi == bj;
   const int j = wn + l31;
 #pragma unroll
@@ -628,16 +609,16 @@ __global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, Chai
       split16(v[e], h, l);
       hh[e] = h; ll[e] = l;
       if (!diag || i + e >= j) {
-        const int at = (int)cat(64, i + e, j);
+        const int at = im64(i + e, j);
         img[at] = h; img[4096 + at] = l;
       }
       if (diag && i + e > j) {
-        const int at = (int)cat(64, j, i + e);
+        const int at = im64(j, i + e);
         img[at] = h; img[4096 + at] = l;
       }
     }
     if (!diag) {
-      const int at = (int)cat(64, j, i);
+      const int at = im64(j, i);
       *reinterpret_cast<half4*>(img + 8192 + at) = hh;
       *reinterpret_cast<half4*>(img + 12288 + at) = ll;
     }
@@ -648,7 +629,7 @@ __global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, Chai
     const int x = q * 256 + tid, im = x >> 9, blk = (x >> 7) & 3, in = x & 127;
     if (im >= 2 && diag) break;
     const int rb = im < 2 ? bi : bj, cb = im < 2 ? bj : bi;
-    *reinterpret_cast<uint4*>(C + (im & 1) * pl + ((cb * 4 + blk) * Mp + rb * CT) * 16 + in * 8) =
+    *reinterpret_cast<uint4*>(C + (im & 1) * pl + cat(Mp, rb * CT, (cb * 4 + blk) * 16) + in * 8) =
         *reinterpret_cast<const uint4*>(img + im * 4096 + blk * 1024 + in * 8);
   }
 }
@@ -663,15 +644,16 @@ struct ApplyK {
   void* out; long ldo;
   NsStep s;
 };
-// one K step of the apply product: P rows 32 bytes each (one K step per stage), 4 fragments of 32 rows; X rows (K) of 256 columns through
-// the transposing read: in a group of 16 lanes lane 4 r + c gives the address of four columns of row r and gets one column of four
-// rows; two of them make a fragment
+// one K step of the apply product: 4 fragments of 32 rows of P; X (K step = 16 of its rows, [column / 16][16 rows][16]) through the
+// transposing read: in a group of 16 lanes lane 4 r + c gives the address of four columns of row r and gets one column of four
+// rows; two of them make a fragment.  Odd blocks hold their rows in the order 4..7 0..3 12..15 8..11, so that the two blocks a
+// 32-lane half reads lie in different banks: the second read's address is the first one's ^ 128.
 #define NS_TR "ds_read_b64_tr_b16 "
 __device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][4], half4 (&b)[2][2][2]) {
-  asm volatile(NS_RD "%0, %16\n\t" NS_TR "%8, %17\n\t" NS_TR "%9, %17 offset:2048\n\t" NS_RD "%1, %16 offset:1024\n\t"
-               NS_TR "%10, %18\n\t" NS_TR "%11, %18 offset:2048\n\t" NS_RD "%2, %16 offset:2048\n\t" NS_RD "%3, %16 offset:3072\n\t"
+  asm volatile(NS_RD "%0, %16\n\t" NS_TR "%8, %17\n\t" NS_TR "%9, %18\n\t" NS_RD "%1, %16 offset:1024\n\t"
+               NS_TR "%10, %17 offset:1024\n\t" NS_TR "%11, %18 offset:1024\n\t" NS_RD "%2, %16 offset:2048\n\t" NS_RD "%3, %16 offset:3072\n\t"
                NS_RD "%4, %16 offset:4096\n\t" NS_RD "%5, %16 offset:5120\n\t" NS_RD "%6, %16 offset:6144\n\t" NS_RD "%7, %16 offset:7168\n\t"
-               NS_TR "%12, %17 offset:8192\n\t" NS_TR "%13, %17 offset:10240\n\t" NS_TR "%14, %18 offset:8192\n\t" NS_TR "%15, %18 offset:10240\n\t"
+               NS_TR "%12, %17 offset:8192\n\t" NS_TR "%13, %18 offset:8192\n\t" NS_TR "%14, %17 offset:9216\n\t" NS_TR "%15, %18 offset:9216\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[0][2]), "=&v"(a[0][3]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(a[1][2]), "=&v"(a[1][3]),
                  "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1]),
@@ -679,8 +661,8 @@ __device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned 
                : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
 }
 __device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][4], half4 (&b)[1][2][2]) {
-  asm volatile(NS_RD "%0, %12\n\t" NS_TR "%8, %13\n\t" NS_TR "%9, %13 offset:2048\n\t" NS_RD "%1, %12 offset:1024\n\t"
-               NS_TR "%10, %14\n\t" NS_TR "%11, %14 offset:2048\n\t" NS_RD "%2, %12 offset:2048\n\t" NS_RD "%3, %12 offset:3072\n\t"
+  asm volatile(NS_RD "%0, %12\n\t" NS_TR "%8, %13\n\t" NS_TR "%9, %14\n\t" NS_RD "%1, %12 offset:1024\n\t"
+               NS_TR "%10, %13 offset:1024\n\t" NS_TR "%11, %14 offset:1024\n\t" NS_RD "%2, %12 offset:2048\n\t" NS_RD "%3, %12 offset:3072\n\t"
                NS_RD "%4, %12 offset:4096\n\t" NS_RD "%5, %12 offset:5120\n\t" NS_RD "%6, %12 offset:6144\n\t" NS_RD "%7, %12 offset:7168\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[0][2]), "=&v"(a[0][3]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(a[1][2]), "=&v"(a[1][3]),
@@ -702,11 +684,11 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
   __shared__ __attribute__((aligned(1024))) char smem[ST * STAGE];
   const int bt = xcd_tile(blockIdx.x, total, 4);
   if (bt < 0) return;
-  const NsRef r = ns_find<&NsMat::ba, &NsGroup::na>(gr, bt);
+  const NsRef r = ns_find<F_APPLY>(gr, bt);
   const NsMat& m = r.m;
   const int ti = (m.Mp + AI - 1) / AI;
   const int i0 = (r.tile % ti) * AI, j0 = (r.tile / ti) * AJ;
-  const long pl = (long)m.Mp * m.Mp, xpl = (long)m.Mp * m.Np;
+  const long pl = cplane(m), xpl = xplane(m);
   const _Float16* P = k.wsg + m.g + k.pbuf * 2 * pl;
   const _Float16* X = k.wsx + m.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -718,34 +700,32 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  // P: 32 rows of a block per transfer; X: two rows of 32 chunks, chunk c of row k at slot c ^ ((k & 3) << 2) for the transposing reads.
-  // Rows and columns behind the matrix read its last ones: products that nobody stores.
+  // P: 32 rows of a block per transfer; X: 16 rows of two blocks.  Rows and blocks behind the matrix read its last ones: products that
+  // nobody stores.
   const _Float16* as[PA];
 #pragma unroll
   for (int q = 0; q < PA; ++q) {
     const int row = (q * 4 + wave) * 32 + (lane >> 1), plane = row / AI, lr = min(i0 + row - plane * AI, m.Mp - 1);
-    as[q] = P + plane * pl + (long)lr * 16 + ((lane & 1) ^ swz<2>(row)) * 8;
+    as[q] = P + plane * pl + (long)lr * 16 + ((lane & 1) ^ swz(row)) * 8;
   }
   const _Float16* bs[PB];
 #pragma unroll
   for (int q = 0; q < PB; ++q) {
-    const int row = (q * 4 + wave) * 2 + (lane >> 5), plane = row >> 4, kr = row & 15;
-    const int col = min(j0 + (((lane & 31) ^ ((kr & 3) << 2)) * 8), m.Np - 8);
-    bs[q] = X + plane * xpl + (long)kr * m.Np + col;
+    const int x = q * 4 + wave, plane = x >> 3, blk = min((j0 >> 4) + (x & 7) * 2 + (lane >> 5), m.Np / 16 - 1);
+    const int kr = ((lane >> 1) & 15) ^ ((lane >> 5) << 2);
+    bs[q] = X + plane * xpl + ((long)blk * (m.Mp + 8) + kr) * 16 + (lane & 1) * 8;
   }
-  const long astep = 16L * m.Mp, bstep = 16L * m.Np;
+  const long astep = 16L * (m.Mp + 8);
   auto issue = [&](int st) {
 #pragma unroll
     for (int q = 0; q < PA; ++q) { dma16(as[q], smem + st * STAGE + (q * 4 + wave) * 1024); as[q] += astep; }
 #pragma unroll
-    for (int q = 0; q < PB; ++q) { dma16(bs[q], smem + st * STAGE + A_BYTES + (q * 4 + wave) * 1024); bs[q] += bstep; }
+    for (int q = 0; q < PB; ++q) { dma16(bs[q], smem + st * STAGE + A_BYTES + (q * 4 + wave) * 1024); bs[q] += 256; }
   };
   const unsigned lds0 = (unsigned)(size_t)smem;
   const int r4 = (lane >> 2) & 3, cq = lane & 3, mb = (lane >> 4) & 1, kh = lane >> 5;
-  const unsigned pa = lds0 + (lane & 31) * 32 + ((kh ^ swz<2>(lane & 31)) << 4);
-  const int chunk = (wn >> 3) + 2 * mb + (cq >> 1);
-  const unsigned pb0 = lds0 + A_BYTES + (8 * kh + r4) * (AJ * 2) + ((chunk ^ (r4 << 2)) << 4) + ((cq & 1) << 3);
-  const unsigned pb1 = lds0 + A_BYTES + (8 * kh + r4) * (AJ * 2) + (((chunk + 4) ^ (r4 << 2)) << 4) + ((cq & 1) << 3);
+  const unsigned pa = lds0 + (lane & 31) * 32 + ((kh ^ swz(lane & 31)) << 4);
+  const unsigned pb0 = lds0 + A_BYTES + ((wn >> 4) + mb) * 512 + (8 * kh + r4 + 4 * mb) * 32 + cq * 8, pb1 = pb0 ^ 128;
   const int n = m.Mp / 16;
   issue(0);
   issue(1);
@@ -827,21 +807,29 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
         *reinterpret_cast<float4*>(buf + (lane & 31) * 264 + wn + j * 32 + 8 * q + 4 * (lane >> 5)) =
             make_float4(acc[i][j][4 * q] * f, acc[i][j][4 * q + 1] * f, acc[i][j][4 * q + 2] * f, acc[i][j][4 * q + 3] * f);
     __syncthreads();
+    if constexpr (OUT == 0) {
+      // planes: 16 blocks of 32 rows, 1 KB each
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int blk = t * 4 + wave, row = lane >> 1, col = blk * 16 + (lane & 1) * 8;
+        if (i0 + i * 32 + row >= m.Mp || j0 + col >= m.Np) continue;
+        const float4 u = *reinterpret_cast<const float4*>(buf + row * 264 + col), w = *reinterpret_cast<const float4*>(buf + row * 264 + col + 4);
+        const float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+        half8 h, l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { _Float16 th, tl; split16(x[e], th, tl); h[e] = th; l[e] = tl; }
+        _Float16* o = k.wso + m.x + cat(m.Mp, i0 + i * 32 + row, j0 + col);
+        *reinterpret_cast<half8*>(o) = h;
+        *reinterpret_cast<half8*>(o + xpl) = l;
+      }
+      continue;
+    }
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       const int gi = i0 + i * 32 + wave * 8 + t;
       const float4 v = *reinterpret_cast<const float4*>(buf + (wave * 8 + t) * 264 + c);
       const float x[4] = {v.x, v.y, v.z, v.w};
-      if constexpr (OUT == 0) {
-        if (gi < m.Mp && gj < m.Np) {
-          half4 h, l;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { _Float16 th, tl; split16(x[e], th, tl); h[e] = th; l[e] = tl; }
-          _Float16* o = k.wso + m.x + (long)gi * m.Np + gj;
-          *reinterpret_cast<half4*>(o) = h;
-          *reinterpret_cast<half4*>(o + xpl) = l;
-        }
-      } else if (gi < m.M && four) {
+      if (gi < m.M && four) {
         if constexpr (OUT == 3) {
           const long at = cbase + (long)gi * m.ld;
           const float y[4] = {p[t].x * keep - step * x[0], p[t].y * keep - step * x[1], p[t].z * keep - step * x[2], p[t].w * keep - step * x[3]};
@@ -885,9 +873,10 @@ static long up(long a, long b) { return (a + b - 1) / b * b; }
 struct NsPlan {
   NsGroup gr;
   std::vector<NsMat> mats;      // the table's content (empty: equal matrices)
-  long n0, n1, ng, nr, nc, na;  // workgroups per launch
+  std::vector<int> first;       // [F_N][n]
+  long n[F_N];                  // workgroups per launch
   int nscal;
-  long off_tab, off_c, off_sq, off_x, x_halves, off_g, off_part, bytes;
+  long off_tab, off_first, off_c, off_sq, off_x, x_halves, off_g, off_part, bytes;
 };
 
 // sizes and workgroup counts of one matrix; false: a side or a product of sides out of range
@@ -902,56 +891,65 @@ static bool ns_shape(NsMat& m) {
   if ((long)m.Mp * m.Np > 0x7fffffffL) return false;
   return true;
 }
-struct NsCounts { long n0, n1, ng, nr, nc, na, x, g, part; };
-static NsCounts ns_counts(NsMat& m, long others, bool flat) {
-  NsCounts c;
+struct NsCounts { long n[F_N], x, g, part; };
+// ks: slices of the long side in the Gram product
+static NsCounts ns_counts(NsMat& m, long ks, bool flat) {
+  NsCounts c{};
   const long n = (long)m.taps * m.rows * m.cols;
-  c.n0 = flat ? cdiv(n, k0_elems(n)) : cdiv((long)m.rows * cdiv(m.cols, 8), SQ_RUNS);
-  m.np = (int)c.n0;
-  if (m.kind == 1) { c.n1 = c.ng = c.nr = c.nc = c.na = c.x = c.g = c.part = 0; return c; }
-  c.n1 = m.tall ? (long)(m.Mp / 64) * (m.Np / 64) : cdiv((long)m.Mp * m.Np / 8, 1024);
+  c.n[F_MOM] = flat ? cdiv(n, k0_elems(n)) : cdiv((long)m.rows * cdiv(m.cols, 8), SQ_RUNS);
+  m.np = (int)c.n[F_MOM];
+  if (m.kind == 1) return c;
+  c.n[F_SPLIT] = m.tall ? (long)(m.Mp / 64) * (m.Np / 64) : (long)(m.Mp / 64) * cdiv(m.Np, 128);
   const long nt = cdiv(m.Mp, GT), ntri = nt * (nt + 1) / 2;
-  // slices of the long side: enough workgroups for two per CU, at least 512 columns each
-  long ks = cdiv(512, ntri * (others > 0 ? others : 1));
-  if (ks > m.Np / 512) ks = m.Np / 512;
-  if (ks < 1) ks = 1;
-  m.kc = (int)up(cdiv(m.Np, ks), 32);
-  m.ks = (int)cdiv(m.Np, m.kc);
-  c.ng = ntri * m.ks;
+  m.ks = ks < 1 ? 1 : ks > m.Np / 256 ? (m.Np < 256 ? 1 : m.Np / 256) : (int)ks;
+  m.kc = (int)up(cdiv(m.Np, m.ks), 32);
+  m.ks = cdiv(m.Np, m.kc);
+  c.n[F_GRAM] = ntri * m.ks;
   const long n64 = m.Mp / 64, n32 = m.Mp / 32;
-  c.nc = n64 * (n64 + 1) / 2;
-  c.nr = n32 * (n32 + 1) / 2;
-  c.na = (long)cdiv(m.Mp, AI) * cdiv(m.Np, AJ);
-  c.x = 2L * m.Mp * m.Np;
-  c.g = 10L * m.Mp * m.Mp;
-  c.part = (long)c.ng * GT * GT;
+  c.n[F_CHAIN] = n64 * (n64 + 1) / 2;
+  c.n[F_JOIN] = n32 * (n32 + 1) / 2;
+  c.n[F_APPLY] = (long)cdiv(m.Mp, AI) * cdiv(m.Np, AJ);
+  c.x = 2L * m.Np * (m.Mp + 8);
+  c.g = 10L * m.Mp * (m.Mp + 8);
+  c.part = c.n[F_GRAM] * GT * GT;
   return c;
+}
+// Gram tiles of a matrix times its length: the unit in which the long side is divided
+static long ns_gram_work(const NsMat& m) {
+  const long nt = cdiv(m.Mp, GT);
+  return nt * (nt + 1) / 2 * m.Np;
 }
 static void ns_place(NsPlan& pl, int nmat, long nx, long ng, long npart) {
   auto take = [&](long& off, long bytes) { off = pl.bytes; pl.bytes += up(bytes, 256); };
   pl.bytes = 0;
   take(pl.off_tab, (long)pl.mats.size() * (long)sizeof(NsMat));
+  take(pl.off_first, (long)pl.first.size() * 4);
   take(pl.off_c, (long)nmat * 4);
-  take(pl.off_sq, pl.n0 * 8);
+  take(pl.off_sq, pl.n[F_MOM] * 8);
   pl.x_halves = up(nx, 128);
   take(pl.off_x, pl.x_halves * 2 * 2);               // two sets of planes: X and its successor
   take(pl.off_g, ng * 2);
   take(pl.off_part, npart * 4);
 }
 
+// workgroups of a Gram launch that run at once: two per CU
+constexpr long GRAM_SLOTS = 512;
+
 static const char* ns_plan_batch(NsPlan& pl, long batch, long rows, long cols, long sx, long ldx, long so) {
   NsMat m{};
   m.taps = 1; m.rows = (int)rows; m.cols = (int)cols; m.ld = ldx; m.st = 0;
   if (!ns_shape(m)) return "a matrix has more than 2^31 - 1 elements";
-  const NsCounts c = ns_counts(m, batch, false);
+  const long nt = cdiv(m.Mp, GT);
+  const NsCounts c = ns_counts(m, GRAM_SLOTS / (nt * (nt + 1) / 2 * batch), false);
   pl.gr.tab = nullptr;
   pl.gr.n = (int)batch;
   pl.gr.u = m;
   pl.gr.src_step = sx; pl.gr.out_step = so; pl.gr.x_step = c.x; pl.gr.g_step = c.g; pl.gr.part_step = c.part;
-  pl.gr.n0 = (int)c.n0; pl.gr.n1 = (int)c.n1; pl.gr.ng = (int)c.ng; pl.gr.nr = (int)c.nr; pl.gr.nc = (int)c.nc; pl.gr.na = (int)c.na;
-  pl.n0 = c.n0 * batch; pl.n1 = c.n1 * batch; pl.ng = c.ng * batch; pl.nr = c.nr * batch; pl.nc = c.nc * batch; pl.na = c.na * batch;
-  const long top = 0x3fffffffL;
-  if (pl.n0 > top || pl.n1 > top || pl.ng > top || pl.nc > top || pl.na > top) return "too many matrices for one call";
+  for (int f = 0; f < F_N; ++f) {
+    pl.gr.per[f] = (int)c.n[f];
+    pl.n[f] = c.n[f] * batch;
+    if (c.n[f] > 0x3fffffffL || pl.n[f] > 0x3fffffffL) return "too many matrices for one call";
+  }
   ns_place(pl, (int)batch, c.x * batch, c.g * batch, c.part * batch);
   return nullptr;
 }
@@ -968,21 +966,25 @@ static const char* ns_plan_table(NsPlan& pl, const pg_muon_entry_t* e, int n) {
     if ((long)m.taps * m.rows > 0x7fffffffL || (long)m.taps * m.rows * m.cols > 0x7fffffffL) return "a tensor has more than 2^31 - 1 elements";
     if (m.kind == 0) {
       if (!ns_shape(m)) return "a matrix has more than 2^31 - 1 elements";
-      work += (long)m.Mp * m.Np;
+      work += ns_gram_work(m);
     }
   }
-  long b0 = 0, b1 = 0, bg = 0, br = 0, bc = 0, ba = 0, x = 0, g = 0, part = 0;
+  pl.first.resize((size_t)n * F_N);
+  long x = 0, g = 0, part = 0;
   for (int i = 0; i < n; ++i) {
     NsMat& m = pl.mats[(size_t)i];
-    // a matrix shares the machine with the others in proportion to its size
-    const long others = m.kind == 0 ? work / ((long)m.Mp * m.Np) : 1;
-    const NsCounts c = ns_counts(m, others, true);
-    m.b0 = (int)b0; m.b1 = (int)b1; m.bg = (int)bg; m.br = (int)br; m.bc = (int)bc; m.ba = (int)ba;
+    // a matrix gets workgroups in proportion to its work, rounded down: all slices run at once, and no second round begins for a few
+    const long nt = cdiv(m.Mp, GT), share = m.kind == 0 ? GRAM_SLOTS * ns_gram_work(m) / work / (nt * (nt + 1) / 2) : 0;
+    const NsCounts c = ns_counts(m, share, true);
+    m.sq0 = (int)pl.n[F_MOM];
     m.x = x; m.g = g; m.part = part;
-    b0 += c.n0; b1 += c.n1; bg += c.ng; br += c.nr; bc += c.nc; ba += c.na; x += c.x; g += c.g; part += c.part;
-    if (b0 > 0x3fffffffL || b1 > 0x3fffffffL || bg > 0x3fffffffL || ba > 0x3fffffffL || bc > 0x3fffffffL) return "too many tensors for one call";
+    x += c.x; g += c.g; part += c.part;
+    for (int f = 0; f < F_N; ++f) {
+      pl.first[(size_t)(f * n + i)] = (int)pl.n[f];
+      pl.n[f] += c.n[f];
+      if (pl.n[f] > 0x3fffffffL) return "too many tensors for one call";
+    }
   }
-  pl.n0 = b0; pl.n1 = b1; pl.ng = bg; pl.nr = br; pl.nc = bc; pl.na = ba;
   ns_place(pl, n, x, g, part);
   pl.gr.n = n;
   return nullptr;
@@ -1001,9 +1003,9 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
   _Float16* g = reinterpret_cast<_Float16*>(w + pl.off_g);
   float* part = reinterpret_cast<float*>(w + pl.off_part);
   const dim3 blk(256);
-  if (in.kind == 0) PG_KLAUNCH((ns_split_kernel<0>), dim3((unsigned)pl.n1), blk, 0, st, gr, in.x, step, sq, eps, cfac, xin);
-  else if (in.kind == 1) PG_KLAUNCH((ns_split_kernel<1>), dim3((unsigned)pl.n1), blk, 0, st, gr, in.x, step, sq, eps, cfac, xin);
-  else PG_KLAUNCH((ns_split_kernel<2>), dim3((unsigned)pl.n1), blk, 0, st, gr, in.x, step, sq, eps, cfac, xin);
+  if (in.kind == 0) PG_KLAUNCH((ns_split_kernel<0>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, cfac, xin);
+  else if (in.kind == 1) PG_KLAUNCH((ns_split_kernel<1>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, cfac, xin);
+  else PG_KLAUNCH((ns_split_kernel<2>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, cfac, xin);
   // planes between stages: |X| <= 1.21 (the quintic's largest value on [0, 1.21]), so 2^15 X fits fp16; its rms there is >= 0.5
   const float sx = 32768.f;
   bool first = true;
@@ -1013,24 +1015,28 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     const bool last = steps == 0;
     const float* cf = first ? cfac : nullptr;
     const bool one = first && in.kind == 1;
-    if (one) PG_KLAUNCH((ns_gram_kernel<1>), dim3((unsigned)up(pl.ng, 8)), blk, 0, st, gr, (int)pl.ng, (const _Float16*)xin, part);
-    else PG_KLAUNCH((ns_gram_kernel<2>), dim3((unsigned)up(pl.ng, 8)), blk, 0, st, gr, (int)pl.ng, (const _Float16*)xin, part);
-    PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.nr), blk, 0, st, gr, (const float*)part, cf, 1.f / sx, g);
+    if (one) PG_KLAUNCH((ns_gram_kernel<1>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
+    else PG_KLAUNCH((ns_gram_kernel<2>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
+    PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.n[F_JOIN]), blk, 0, st, gr, (const float*)part, cf, 1.f / sx, g);
     // buffers: 0 G, 1 Q, 2 Q G, 3 and 4 P in turn; the first step's Q is the first P (and keeps Q's scale)
     const float q1 = 1.f / (float)(1 << SG);
     int p = 3, psc = SG;
-    const int nc = (int)pl.nc;
-    const dim3 gc((unsigned)up(pl.nc, 8));
+    const int nc = (int)pl.n[F_CHAIN];
+    auto chain = [&](const ChainJob& a, const ChainJob* b) {
+      const int total = b ? 2 * nc : nc;
+      const dim3 gd((unsigned)up(total, 8));
+      if (total <= 256) PG_KLAUNCH((ns_chain_kernel<8>), gd, blk, 0, st, gr, a, b ? *b : a, total, nc, g);
+      else PG_KLAUNCH((ns_chain_kernel<4>), gd, blk, 0, st, gr, a, b ? *b : a, total, nc, g);
+    };
     for (int k = 0; k < ns; ++k) {
       const int q = k == 0 ? 3 : 1;
       const ChainJob quad = {0, 0, q, NS_C * q1, 1};
-      PG_KLAUNCH(ns_chain_kernel, gc, blk, 0, st, gr, quad, quad, nc, nc, g);
       const ChainJob qg = {q, 0, 2, q1, 0}, qp = {q, p, 7 - p, (float)ldexp(1.0, SP - SG - psc), 0}, qqg = {q, 2, 0, q1, 0};
       const bool more = k + 1 < ns;
-      if (more && k > 0) PG_KLAUNCH(ns_chain_kernel, dim3((unsigned)up(2 * pl.nc, 8)), blk, 0, st, gr, qg, qp, 2 * nc, nc, g);
-      else if (more) PG_KLAUNCH(ns_chain_kernel, gc, blk, 0, st, gr, qg, qg, nc, nc, g);
-      else if (k > 0) PG_KLAUNCH(ns_chain_kernel, gc, blk, 0, st, gr, qp, qp, nc, nc, g);
-      if (more) PG_KLAUNCH(ns_chain_kernel, gc, blk, 0, st, gr, qqg, qqg, nc, nc, g);
+      chain(quad, nullptr);
+      if (more) chain(qg, k > 0 ? &qp : nullptr);
+      else if (k > 0) chain(qp, nullptr);
+      if (more) chain(qqg, nullptr);
       if (k > 0) { p = 7 - p; psc = SP; }
     }
     ApplyK a;
@@ -1040,8 +1046,8 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     a.mul = (float)ldexp(1.0, -psc) * (last ? 1.f : sx);
     a.out = out; a.ldo = ldo; a.s = step;
     const int o = last ? out_kind : 0;
-    const dim3 gd((unsigned)up(pl.na, 8));
-    const int na = (int)pl.na;
+    const dim3 gd((unsigned)up(pl.n[F_APPLY], 8));
+    const int na = (int)pl.n[F_APPLY];
     if (one) {
       if (o == 0) PG_KLAUNCH((ns_apply_kernel<1, 0>), gd, blk, 0, st, gr, na, a);
       else if (o == 1) PG_KLAUNCH((ns_apply_kernel<1, 1>), gd, blk, 0, st, gr, na, a);
@@ -1087,8 +1093,8 @@ extern "C" int pg_orthogonalise(const void* x, int32_t x_is_bf16, int64_t batch,
   char* w = reinterpret_cast<char*>(workspace);
   hipStream_t st = (hipStream_t)stream;
   double* sq = reinterpret_cast<double*>(w + pl.off_sq);
-  if (x_is_bf16) PG_KLAUNCH((ns_sumsq_kernel<1>), dim3((unsigned)pl.n0), dim3(256), 0, st, pl.gr, x, sq);
-  else PG_KLAUNCH((ns_sumsq_kernel<0>), dim3((unsigned)pl.n0), dim3(256), 0, st, pl.gr, x, sq);
+  if (x_is_bf16) PG_KLAUNCH((ns_sumsq_kernel<1>), dim3((unsigned)pl.n[F_MOM]), dim3(256), 0, st, pl.gr, x, sq);
+  else PG_KLAUNCH((ns_sumsq_kernel<0>), dim3((unsigned)pl.n[F_MOM]), dim3(256), 0, st, pl.gr, x, sq);
   const NsSource in = {x_is_bf16 ? 1 : 0, x};
   const NsStep none{};
   ns_run(pl, w, in, none, steps, eps, out_is_bf16 ? 2 : 1, out, (long)ldo, st);
@@ -1125,22 +1131,27 @@ extern "C" int pg_muon_step(const pg_muon_t* d, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   char* w = reinterpret_cast<char*>(d->workspace);
   NsMat* tab = reinterpret_cast<NsMat*>(w + pl.off_tab);
-  for (size_t i = 0; i < pl.mats.size(); i += 16) {
+  int* first = reinterpret_cast<int*>(w + pl.off_first);
+  for (int i = 0; i < d->n; i += 16) {
     NsChunk c;
-    const int cnt = (int)(pl.mats.size() - i < 16 ? pl.mats.size() - i : 16);
+    const int cnt = d->n - i < 16 ? d->n - i : 16;
     memset(&c, 0, sizeof(c));
-    memcpy(&c, &pl.mats[i], (size_t)cnt * sizeof(NsMat));
-    PG_KLAUNCH(ns_table_kernel, dim3(1), dim3(64), 0, st, c, tab + i, cnt);
+    for (int k = 0; k < cnt; ++k) {
+      c.m[k] = pl.mats[(size_t)(i + k)];
+      for (int f = 0; f < F_N; ++f) c.first[f][k] = pl.first[(size_t)(f * d->n + i + k)];
+    }
+    PG_KLAUNCH(ns_table_kernel, dim3(1), dim3(256), 0, st, c, tab, first, i, cnt, d->n);
   }
   pl.gr.tab = tab;
+  pl.gr.first = first;
   NsStep s{};
   s.p = d->p; s.g = d->g; s.gb = reinterpret_cast<const bf16_t*>(d->g_bf16); s.m = d->m; s.v = d->v;
   s.pb = reinterpret_cast<bf16_t*>(d->p_bf16);
   s.mu = d->momentum; s.gscale = d->grad_scale; s.lr = d->lr; s.wd = d->weight_decay; s.nesterov = d->nesterov;
   s.b1 = (float)d->beta1; s.b2 = (float)d->beta2; s.eps = d->adam_eps; s.b1d = d->beta1; s.b2d = d->beta2;
   s.step0 = (long)d->step; s.ctr = reinterpret_cast<const unsigned long long*>(d->ctr);
-  PG_KLAUNCH(muon_momentum_kernel, dim3((unsigned)pl.n0), dim3(256), 0, st, pl.gr, s, reinterpret_cast<double*>(w + pl.off_sq));
-  if (pl.ng > 0) {
+  PG_KLAUNCH(muon_momentum_kernel, dim3((unsigned)pl.n[F_MOM]), dim3(256), 0, st, pl.gr, s, reinterpret_cast<double*>(w + pl.off_sq));
+  if (pl.n[F_GRAM] > 0) {
     const NsSource in = {2, nullptr};
     ns_run(pl, w, in, s, d->steps, d->eps, 3, nullptr, 0, st);
   }
