@@ -279,6 +279,14 @@ __device__ __forceinline__ long xplane(const NsMat& m) { return (long)m.Np * (m.
 __device__ __forceinline__ long cplane(const NsMat& m) { return (long)m.Mp * (m.Mp + 8); }
 
 // ---------------------------------------------------------------------------------------------- split into fp16 planes
+// planes hold 2^-k U with an rms in 2^-0.75 .. 2^0.25: the largest element, at most sqrt(n) rms <= 2^15.5 2^0.25, fits fp16.
+// c = 2^k / (|U| + eps): from the planes' units to X0's
+__device__ __forceinline__ void ns_scale(double sumsq, long n, float eps, int& k, float& c) {
+  const double norm = sqrt(sumsq), rms = sqrt(sumsq / (double)n);
+  k = 0;
+  if (rms > 0.0 && rms < 1e300) k = max(-126, min(126, (int)rint(log2(rms) + 0.25)));
+  c = norm == 0.0 ? 0.f : (float)(ldexp(1.0, k) / (norm + (double)eps));
+}
 // every workgroup joins its matrix's partial sums of squares itself (a few hundred doubles); the first one publishes
 // c = 2^k / (|U| + eps), the factor from the planes' units to X0's
 template <int SRC>
@@ -295,13 +303,11 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
   double a = 0.0;
   for (int i = threadIdx.x; i < np; i += 256) a += sq[first + i];
   a = block_sum_d256(a, red);
-  const double norm = sqrt(a);
-  // 2^k >= rms / 2^0.75, so that the largest element, at most sqrt(n) rms, stays below 2^(15.5 + 0.75 - 0.5) ... 55200 in the planes
-  const double rms = sqrt(a / (double)n);
-  int k = 0;
-  if (rms > 0.0 && rms < 1e300) k = max(-126, min(126, (int)rint(log2(rms) + 0.25)));
+  int k;
+  float cf;
+  ns_scale(a, n, eps, k, cf);
   const float f = (float)ldexp(1.0, -k);
-  if (r.tile == 0 && threadIdx.x == 0) cfac[r.id] = norm == 0.0 ? 0.f : (float)(ldexp(1.0, k) / (norm + (double)eps));
+  if (r.tile == 0 && threadIdx.x == 0) cfac[r.id] = cf;
   _Float16* hi = ws + m.x;
   _Float16* lo = hi + xplane(m);
   if (!m.tall) {
@@ -398,20 +404,21 @@ __device__ __forceinline__ void fetch_nt(unsigned pa, unsigned pb, half8 (&a)[1]
                : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(b[0][0]), "=&v"(b[0][1]) : "v"(pa), "v"(pb) : "memory");
 }
 
-// C[BM][BM] = sum_k A[i][k] B[j][k] over columns k0 .. k1 - 1 (multiples of 32), operands as PL fp16 planes in blocks; 4 waves (2 x 2), two
-// blocks per stage, ST stages.  `same`: A and B are the same rows, moved once.  Rows behind a_rows / b_rows read the last one instead:
-// their products belong to rows and columns that nobody stores.
-template <int BM, int PL, int ST>
+// C[BM][BM] = sum_k A[i][k] B[j][k] over columns k0 .. k1 - 1 (multiples of 32), operands as PL fp16 planes in blocks.  KG groups of 4 waves
+// (2 x 2) take every KG-th step of 32 columns, ST stages deep; `join` adds the groups' sums.  `same`: A and B are the same rows, moved
+// once.  Rows behind a_rows / b_rows read the last one instead: their products belong to rows and columns that nobody stores.
+template <int BM, int PL, int ST, int KG>
 struct NtCore {
   static constexpr int T = BM / 64, BLK = BM * 32, OP = PL * 2 * BLK, STAGE = 2 * OP;      // [operand][plane][block][BM][16]
   static constexpr int NI = STAGE / 4096;                           // transfers per wave and stage
-  static constexpr int LDS_BYTES = ST * STAGE;
+  static constexpr int LDS_BYTES = KG * ST * STAGE;
   static_assert((T == 1 || T == 2) && LDS_BYTES <= 128 * 1024, "tile");
   f32x16 acc[T][T];
 
   __device__ __forceinline__ void run(char* smem, const _Float16* A, int a_rows, const _Float16* B, int b_rows, long plane, int pitch, bool same,
                                       int k0, int k1) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = wv & 3, grp = wv >> 2;
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BM / 2);
 #pragma unroll
     for (int i = 0; i < T; ++i)
@@ -419,25 +426,27 @@ struct NtCore {
       for (int j = 0; j < T; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    char* const base = smem + grp * (ST * STAGE);
     const _Float16* src[NI];
 #pragma unroll
     for (int q = 0; q < NI; ++q) {                   // transfer x of a stage: operand, plane, block, 32 rows
       const int x = q * 4 + wave, op = x / (NI * 2), y = x % (BM / 32), z = x / (BM / 32) % (PL * 2);
       const int row = y * 32 + (lane >> 1);
-      src[q] = (op ? B : A) + (z >> 1) * plane + ((long)(k0 / 16 + (z & 1)) * pitch + min(row, (op ? b_rows : a_rows) - 1)) * 16 +
+      src[q] = (op ? B : A) + (z >> 1) * plane + ((long)(k0 / 16 + grp * 2 + (z & 1)) * pitch + min(row, (op ? b_rows : a_rows) - 1)) * 16 +
                ((lane & 1) ^ swz(row)) * 8;
     }
-    const long step = 32L * pitch;
+    const long step = 32L * KG * pitch;
     auto issue = [&](int st) {
 #pragma unroll
       for (int q = 0; q < NI; ++q) {
         if (q == NI / 2 && same) break;
-        dma16(src[q], smem + st * STAGE + (q * 4 + wave) * 1024);
+        dma16(src[q], base + st * STAGE + (q * 4 + wave) * 1024);
         src[q] += step;
       }
     };
-    const int n = (k1 - k0) / 32;
-    const unsigned lds0 = (unsigned)(size_t)smem;
+    const int all = (k1 - k0) / 32, trips = (all + KG - 1) / KG;       // every wave meets every barrier
+    const int n = all > grp ? (all - grp + KG - 1) / KG : 0;
+    const unsigned lds0 = (unsigned)(size_t)base;
     const int r = lane & 31;
     const unsigned off = (unsigned)(r * 32 + (((lane >> 5) ^ swz(r)) << 4));
     const unsigned pa = lds0 + wm * 32 + off, pb = lds0 + (same ? 0 : OP) + wn * 32 + off;
@@ -445,12 +454,13 @@ struct NtCore {
     for (int q = 0; q < ST - 1; ++q)
       if (q < n) issue(q);
     int cur = 0, nxt = ST - 1;
-    for (int it = 0; it < n; ++it) {
+    for (int it = 0; it < trips; ++it) {
       if (it + ST - 2 >= n) wait_dma<0>();
       else if (same) wait_dma<NI / 2 * (ST - 2)>();
       else wait_dma<NI * (ST - 2)>();
       wg_barrier();
       if (it + ST - 1 < n) issue(nxt);
+      if (KG > 1 && it >= n) break;                                    // the last trip: no barrier follows
       const unsigned so = (unsigned)(cur * STAGE);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -475,6 +485,31 @@ struct NtCore {
       nxt = nxt + 1 == ST ? 0 : nxt + 1;
     }
   }
+  // the groups' sums, in order, to group 0 (T = 1); every wave calls it.  LDS is free afterwards
+  __device__ __forceinline__ void join(char* smem) {
+    static_assert(T == 1, "join");
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    float4* buf = reinterpret_cast<float4*>(smem);
+    __syncthreads();
+    if (KG > 1) {
+      if (wv >= 4) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          buf[((wv - 4) * 4 + q) * 64 + lane] = make_float4(acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]);
+      }
+      __syncthreads();
+      if (wv < 4) {
+#pragma unroll
+        for (int g = 1; g < KG; ++g)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4 f = buf[((g * 4 - 4 + wv) * 4 + q) * 64 + lane];
+            acc[0][0][4 * q] += f.x; acc[0][0][4 * q + 1] += f.y; acc[0][0][4 * q + 2] += f.z; acc[0][0][4 * q + 3] += f.w;
+          }
+      }
+      __syncthreads();
+    }
+  }
 };
 
 // tile number of the lower triangle (bi >= bj), row by row
@@ -489,7 +524,7 @@ __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
 // G = X X^T over one slice of the long side: fp32 partial tiles, in the order of the accumulators (one float4 = four rows of a column)
 template <int PL>
 __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int total, const _Float16* ws, float* part) {
-  typedef NtCore<GT, PL, 2> Core;
+  typedef NtCore<GT, PL, 2, 1> Core;
   __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
   const int b = xcd_tile(blockIdx.x, total, 10);
   if (b < 0) return;
@@ -557,12 +592,14 @@ __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, con
 
 // chain planes of a matrix: 0 G, 1 Q, 2 Q G, 3 P, 4 the other P  (hi and lo each)
 // C = A B of commuting symmetric matrices: the lower triangle of 64 x 64 tiles, mirrored.  `quad`: C = a I + b A + c A A
-// 4 waves of 32 x 32.  Such a product is a few microseconds of latency: ST = 4 stages (64 KB, two workgroups per CU), 8 where there is
-// at most one workgroup per CU.  The tile leaves through LDS in both orientations, 2 KB runs.
+// Tiles of 64 x 64.  Such a product is a few microseconds of latency (LDS read, three dependent MFMAs, barrier: 0.36 us per 32 columns
+// with 4 waves), so KG groups of 4 waves divide the columns: 4 groups (128 KB of stages) where there is at most one workgroup per CU, 2
+// (two workgroups per CU) otherwise.  The tile leaves through LDS in both orientations, 2 KB runs.
 struct ChainJob { int a, b, c; float mul; int quad; };
-template <int ST>
-__global__ __launch_bounds__(256, ST == 4 ? 2 : 1) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
-  typedef NtCore<CT, 2, ST> Core;
+template <int KG>
+__global__ __launch_bounds__(256 * KG, KG == 2 ? 4 : 4) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles,
+                                                                            _Float16* ws) {
+  typedef NtCore<CT, 2, 2, KG> Core;
   __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
   const int t = xcd_tile(blockIdx.x, total, 36);
   if (t < 0) return;
@@ -577,16 +614,17 @@ __global__ __launch_bounds__(256, ST == 4 ? 2 : 1) void ns_chain_kernel(const Ns
   const _Float16* B = ws + m.g + jb.b * 2 * pl;
   _Float16* C = ws + m.g + jb.c * 2 * pl;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32, l31 = lane & 31;
+  const int wm = ((wave >> 1) & 1) * 32, wn = (wave & 1) * 32, l31 = lane & 31;
   Core core;
   core.run(smem, A + (long)bi * CT * 16, CT, B + (long)bj * CT * 16, CT, pl, Mp + 8, bi == bj && jb.a == jb.b, 0, Mp);
+  core.join(smem);
   const f32x16& acc = core.acc[0][0];
-  __syncthreads();
   // image of the tile: [orientation][plane][4 blocks][64 rows][16]
   _Float16* img = reinterpret_cast<_Float16*>(smem);
   auto im64 = [](int i, int j) { return ((j >> 4) * 64 + i) * 16 + (j & 15); };
   const bool diag = bi == bj;
   const int j = wn + l31;
+  if (wave < 4) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int i = wm + 8 * q + 4 * (lane >> 5);
@@ -623,10 +661,11 @@ __global__ __launch_bounds__(256, ST == 4 ? 2 : 1) void ns_chain_kernel(const Ns
       *reinterpret_cast<half4*>(img + 12288 + at) = ll;
     }
   }
+  }
   __syncthreads();
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const int x = q * 256 + tid, im = x >> 9, blk = (x >> 7) & 3, in = x & 127;
+  for (int q = 0; q < 8 / KG; ++q) {
+    const int x = q * (256 * KG) + tid, im = x >> 9, blk = (x >> 7) & 3, in = x & 127;
     if (im >= 2 && diag) break;
     const int rb = im < 2 ? bi : bj, cb = im < 2 ? bj : bi;
     *reinterpret_cast<uint4*>(C + (im & 1) * pl + cat(Mp, rb * CT, (cb * 4 + blk) * 16) + in * 8) =
@@ -867,6 +906,304 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
   }
 }
 
+// ---------------------------------------------------------------------------------------------- small matrices
+// The chain of a matrix with a short side of at most MP (64, 128) in ONE workgroup: (MP / 32)^2 waves, each with one 32 x 32 block of every
+// matrix in its registers; two LDS buffers hold the operands of the product under way (fp16 pairs, [plane][block][MP rows][16]).
+// A launch of the tiled form costs 5 us whatever its size, a product here 0.6 (64) to 1.2 us (128).
+template <int MP>
+struct SmallChain {
+  static constexpr int W = MP / 32, BUF = MP * MP * 4, PS = MP * MP * 2;
+  int lane, wi, wj;
+  unsigned fa, fb;
+  __device__ __forceinline__ SmallChain(int wave) {
+    lane = threadIdx.x & 63; wi = wave / W; wj = wave % W;
+    const int r = lane & 31;
+    const unsigned off = (unsigned)(r * 32 + (((lane >> 5) ^ swz(r)) << 4));
+    fa = (unsigned)(wi * 1024) + off; fb = (unsigned)(wj * 1024) + off;
+  }
+  // the transposed block of a symmetric matrix: four neighbours of a row at a time
+  __device__ __forceinline__ void put(char* buf, const f32x16& v) const {
+    const int row = wj * 32 + (lane & 31);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int col = wi * 32 + 8 * q + 4 * (lane >> 5);
+      half4 h, l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { _Float16 th, tl; split16(v[4 * q + e], th, tl); h[e] = th; l[e] = tl; }
+      char* at = buf + ((col >> 4) * MP + row) * 32 + ((((col >> 3) & 1) ^ swz(row)) << 4) + (col & 7) * 2;
+      *reinterpret_cast<half4*>(at) = h;
+      *reinterpret_cast<half4*>(at + PS) = l;
+    }
+  }
+  __device__ __forceinline__ f32x16 mul(const char* a, const char* b) const {
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+    const unsigned pa = (unsigned)(size_t)a + fa, pb = (unsigned)(size_t)b + fb;
+#pragma unroll
+    for (int ks = 0; ks < MP / 16; ++ks) {
+      half8 x[2][1], y[2][1];
+      fetch_nt<PS>(pa + ks * (MP * 32), pb + ks * (MP * 32), x, y);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0][0], y[0][0], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0][0], y[1][0], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[1][0], y[0][0], acc, 0, 0, 0);
+    }
+    return acc;
+  }
+  // g: this wave's block of G (scale 2^SG).  Returns its block of P, scale 2^(steps > 1 ? SP : SG).  `on`: this wave has a block; every
+  // wave of the workgroup calls it
+  __device__ __forceinline__ f32x16 run(bool on, f32x16 g, int steps, char* b1, char* b2) const {
+    const float q1 = 1.f / (float)(1 << SG);
+    f32x16 P, y;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) P[e] = 0.f;
+    __syncthreads();
+    if (on) put(b1, g);
+    __syncthreads();
+    for (int k = 0; k < steps; ++k) {
+      const bool more = k + 1 < steps;
+      f32x16 q;
+      if (on) {
+        q = mul(b1, b1);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          q[e] = q[e] * (NS_C * q1) + NS_B * g[e];
+          if (wi == wj && 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31)) q[e] += NS_A * (float)(1 << SG);
+        }
+        put(b2, q);
+      }
+      __syncthreads();
+      if (on && more) y = mul(b2, b1) * q1;
+      if (k == 0) {
+        P = q;
+      } else {
+        __syncthreads();
+        if (on) put(b1, P);
+        __syncthreads();
+        if (on) P = mul(b2, b1) * (k == 1 ? 1.f / (float)(1 << (2 * SG - SP)) : q1);
+      }
+      if (more) {
+        __syncthreads();
+        if (on) put(b1, y);
+        __syncthreads();
+        if (on) g = mul(b2, b1) * q1;
+        __syncthreads();
+        if (on) put(b1, g);
+        __syncthreads();
+      }
+    }
+    return P;
+  }
+};
+
+// the join of the Gram slices and the whole chain of one stage: one workgroup per matrix, P to buffer 3
+template <int MP>
+__global__ __launch_bounds__(64 * (MP / 32) * (MP / 32)) void ns_chain_small_kernel(const NsGroup gr, const float* part, const float* cfac, float cconst,
+                                                                                  int steps, _Float16* ws) {
+  typedef SmallChain<MP> Sc;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * Sc::BUF];
+  const int id = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  NsMat m = gr.tab ? gr.tab[id] : gr.u;
+  if (m.kind == 1) return;
+  if (!gr.tab) { m.g += (long)id * gr.g_step; m.part += (long)id * gr.part_step; }
+  const Sc sc(wave);
+  const int frag = ((sc.wi >> 1) * 2 + (sc.wj >> 1)) * 4 + (sc.wi & 1) * 2 + (sc.wj & 1);
+  const float4* src = reinterpret_cast<const float4*>(part + m.part) + frag * 256 + lane;
+  const float c1 = cfac ? cfac[id] : cconst;
+  const float c2 = c1 * c1 * (float)(1 << SG);
+  f32x16 g;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) g[e] = 0.f;
+  if (sc.wi * 32 < m.Mp && sc.wj * 32 < m.Mp) {
+#pragma unroll 4
+    for (int s = 0; s < m.ks; ++s)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 f = src[(long)s * (GT * GT / 4) + q * 64];
+        g[4 * q] += f.x; g[4 * q + 1] += f.y; g[4 * q + 2] += f.z; g[4 * q + 3] += f.w;
+      }
+    g = g * c2;
+  }
+  const f32x16 P = sc.run(true, g, steps, smem, smem + Sc::BUF);
+  const int row = sc.wj * 32 + (lane & 31);
+  if (sc.wi * 32 >= m.Mp || sc.wj * 32 >= m.Mp) return;
+  const long pl = cplane(m);
+  _Float16* out = ws + m.g + 6 * pl;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    half4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { _Float16 th, tl; split16(P[4 * q + e], th, tl); h[e] = th; l[e] = tl; }
+    _Float16* at = out + cat(m.Mp, row, sc.wi * 32 + 8 * q + 4 * (lane >> 5));
+    *reinterpret_cast<half4*>(at) = h;
+    *reinterpret_cast<half4*>(at + pl) = l;
+  }
+}
+
+// Everything in one launch for matrices of at most 64 x NX: X stays in LDS from the first load to the result.  8 waves: the Gram product
+// divides the columns among two groups of four, the chain takes four waves, P X goes by strips of 32 columns, in place.
+template <int NX, int SRC, int OUT>
+__global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void* x, long src_step, void* outp, long out_step, long ldo, int steps, float eps) {
+  constexpr int XP = NX * 64 * 2;                     // bytes of a plane: [NX / 16][64 rows][16]
+  typedef SmallChain<64> Sc;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * XP + 2 * Sc::BUF];
+  __shared__ double red[8];
+  char* const X = smem;
+  char* const b1 = smem + 2 * XP;
+  char* const b2 = b1 + Sc::BUF;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  NsMat mm = m;
+  mm.src += (long)blockIdx.x * src_step;
+  const NsStep none{};
+  // runs of eight stored neighbours: at most 64 x NX / 8
+  constexpr int RUNS = 64 * NX / 8 / 512;
+  const int rpr = (m.cols + 7) / 8, nrun = m.rows * rpr;
+  float v[RUNS][8];
+  double a = 0.0;
+#pragma unroll
+  for (int t = 0; t < RUNS; ++t) {
+    const int c = t * 512 + tid;
+    if (c < nrun) {
+      const int row = c / rpr;
+      ns_load8<SRC>(mm, x, none, row, (c - row * rpr) * 8, v[t]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a = fma((double)v[t][e], (double)v[t][e], a);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 2 * XP / 16 / 512; ++t) *reinterpret_cast<uint4*>(X + (t * 512 + tid) * 16) = make_uint4(0u, 0u, 0u, 0u);
+  a = wave_sum_d(a);
+  if (lane == 0) red[wave] = a;
+  __syncthreads();
+  a = 0.0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) a += red[w];
+  int k;
+  float cf;
+  ns_scale(a, (long)m.rows * m.cols, eps, k, cf);
+  const float f = (float)ldexp(1.0, -k);
+#pragma unroll
+  for (int t = 0; t < RUNS; ++t) {
+    const int c = t * 512 + tid;
+    if (c >= nrun) continue;
+    const int row = c / rpr, col = (c - row * rpr) * 8;
+    half8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { _Float16 th, tl; split16(v[t][e] * f, th, tl); h[e] = th; l[e] = tl; }
+    if (!m.tall) {
+      char* at = X + ((col >> 4) * 64 + row) * 32 + ((((col >> 3) & 1) ^ swz(row)) << 4);
+      *reinterpret_cast<half8*>(at) = h;
+      *reinterpret_cast<half8*>(at + XP) = l;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = col + e, j = row;
+        if (i >= m.M) break;
+        _Float16* at = reinterpret_cast<_Float16*>(X + ((j >> 4) * 64 + i) * 32 + ((((j >> 3) & 1) ^ swz(i)) << 4) + (j & 7) * 2);
+        at[0] = h[e];
+        at[XP / 2] = l[e];
+      }
+    }
+  }
+  const bool on = wave < 4;
+  const Sc sc(wave & 3);
+  const int r4 = (lane >> 2) & 3, cq = lane & 3, mb = (lane >> 4) & 1, kh = lane >> 5;
+  const int nblk = m.Np / 16;
+  float c1 = cf;
+  while (steps > 0) {
+    const int ns = steps < 3 ? steps : 3;
+    steps -= ns;
+    __syncthreads();
+    f32x16 g;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) g[e] = 0.f;
+    for (int b = wave >> 2; b < nblk; b += 2) {
+      half8 p[2][1], q[2][1];
+      const unsigned at = (unsigned)(size_t)X + b * 2048;
+      fetch_nt<XP>(at + sc.fa, at + sc.fb, p, q);
+      g = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0][0], q[0][0], g, 0, 0, 0);
+      g = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0][0], q[1][0], g, 0, 0, 0);
+      g = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[1][0], q[0][0], g, 0, 0, 0);
+    }
+    float4* buf = reinterpret_cast<float4*>(b1);
+    if (!on) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) buf[((wave - 4) * 4 + q) * 64 + lane] = make_float4(g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]);
+    }
+    __syncthreads();
+    if (on) {
+      const float c2 = c1 * c1 * (float)(1 << SG);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 u = buf[(wave * 4 + q) * 64 + lane];
+        g[4 * q] = (g[4 * q] + u.x) * c2; g[4 * q + 1] = (g[4 * q + 1] + u.y) * c2;
+        g[4 * q + 2] = (g[4 * q + 2] + u.z) * c2; g[4 * q + 3] = (g[4 * q + 3] + u.w) * c2;
+      }
+    }
+    const f32x16 P = sc.run(on, g, ns, b1, b2);
+    __syncthreads();
+    if (on) sc.put(b1, P);
+    __syncthreads();
+    const bool last = steps == 0;
+    const float mul = c1 * (ns > 1 ? 1.f / (float)(1 << SP) : 1.f / (float)(1 << SG)) * (last ? 1.f : 32768.f);
+    for (int s = wave; s < m.Np / 32; s += 8) {       // a strip of 32 columns: all of its rows are this wave's
+      f32x16 acc[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        half8 p[2][2];
+        half4 t[2][2];
+        const int r = lane & 31;
+        const unsigned pa = (unsigned)(size_t)b1 + ks * 2048 + r * 32 + ((kh ^ swz(r)) << 4);
+        const unsigned pb = (unsigned)(size_t)X + (s * 2 + mb) * 2048 + (ks * 16 + 8 * kh + r4) * 32 + (((cq >> 1) ^ kh) << 4) + (cq & 1) * 8;
+        asm volatile(NS_RD "%0, %8\n\t" NS_RD "%1, %8 offset:1024\n\t" NS_RD "%2, %8 offset:%10\n\t" NS_RD "%3, %8 offset:%11\n\t"
+                     NS_TR "%4, %9\n\t" NS_TR "%5, %9 offset:128\n\t" NS_TR "%6, %9 offset:%12\n\t" NS_TR "%7, %9 offset:%13\n\t" "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(p[0][0]), "=&v"(p[0][1]), "=&v"(p[1][0]), "=&v"(p[1][1]), "=&v"(t[0][0]), "=&v"(t[0][1]), "=&v"(t[1][0]), "=&v"(t[1][1])
+                     : "v"(pa), "v"(pb), "n"(Sc::PS), "n"(Sc::PS + 1024), "n"(XP), "n"(XP + 128) : "memory");
+        const half8 y0 = __builtin_shufflevector(t[0][0], t[0][1], 0, 1, 2, 3, 4, 5, 6, 7);
+        const half8 y1 = __builtin_shufflevector(t[1][0], t[1][1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y0, p[0][i], acc[i], 0, 0, 0);
+          acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y0, p[1][i], acc[i], 0, 0, 0);
+          acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y1, p[0][i], acc[i], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = i * 32 + (lane & 31);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int col = s * 32 + 8 * q + 4 * kh;
+          float o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = acc[i][4 * q + e] * mul;
+          if (!last) {
+            half4 h, l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { _Float16 th, tl; split16(o[e], th, tl); h[e] = th; l[e] = tl; }
+            char* at = X + ((col >> 4) * 64 + row) * 32 + ((((col >> 3) & 1) ^ swz(row)) << 4) + (col & 7) * 2;
+            *reinterpret_cast<half4*>(at) = h;
+            *reinterpret_cast<half4*>(at + XP) = l;
+          } else if (row < m.M) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (col + e >= m.N) break;
+              const long at = (long)blockIdx.x * out_step + (m.tall ? (long)(col + e) * ldo + row : (long)row * ldo + col + e);
+              if constexpr (OUT == 1) reinterpret_cast<float*>(outp)[at] = o[e];
+              else reinterpret_cast<bf16_t*>(outp)[at] = (bf16_t)(ns_pack_bf16(o[e], 0.f) & 0xffffu);
+            }
+          }
+        }
+      }
+    }
+    c1 = 1.f / 32768.f;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- host side
 static long up(long a, long b) { return (a + b - 1) / b * b; }
 
@@ -875,7 +1212,7 @@ struct NsPlan {
   std::vector<NsMat> mats;      // the table's content (empty: equal matrices)
   std::vector<int> first;       // [F_N][n]
   long n[F_N];                  // workgroups per launch
-  int nscal;
+  int top;                      // largest padded short side
   long off_tab, off_first, off_c, off_sq, off_x, x_halves, off_g, off_part, bytes;
 };
 
@@ -941,6 +1278,7 @@ static const char* ns_plan_batch(NsPlan& pl, long batch, long rows, long cols, l
   if (!ns_shape(m)) return "a matrix has more than 2^31 - 1 elements";
   const long nt = cdiv(m.Mp, GT);
   const NsCounts c = ns_counts(m, GRAM_SLOTS / (nt * (nt + 1) / 2 * batch), false);
+  pl.top = m.Mp;
   pl.gr.tab = nullptr;
   pl.gr.n = (int)batch;
   pl.gr.u = m;
@@ -967,6 +1305,7 @@ static const char* ns_plan_table(NsPlan& pl, const pg_muon_entry_t* e, int n) {
     if (m.kind == 0) {
       if (!ns_shape(m)) return "a matrix has more than 2^31 - 1 elements";
       work += ns_gram_work(m);
+      if (m.Mp > pl.top) pl.top = m.Mp;
     }
   }
   pl.first.resize((size_t)n * F_N);
@@ -1017,16 +1356,22 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     const bool one = first && in.kind == 1;
     if (one) PG_KLAUNCH((ns_gram_kernel<1>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
     else PG_KLAUNCH((ns_gram_kernel<2>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
-    PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.n[F_JOIN]), blk, 0, st, gr, (const float*)part, cf, 1.f / sx, g);
     // buffers: 0 G, 1 Q, 2 Q G, 3 and 4 P in turn; the first step's Q is the first P (and keeps Q's scale)
     const float q1 = 1.f / (float)(1 << SG);
     int p = 3, psc = SG;
     const int nc = (int)pl.n[F_CHAIN];
+    if (pl.top <= 128) {
+      const dim3 gm((unsigned)gr.n);
+      if (pl.top == 64) PG_KLAUNCH((ns_chain_small_kernel<64>), gm, blk, 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
+      else PG_KLAUNCH((ns_chain_small_kernel<128>), gm, dim3(1024), 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
+      psc = ns > 1 ? SP : SG;
+    } else {
+    PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.n[F_JOIN]), blk, 0, st, gr, (const float*)part, cf, 1.f / sx, g);
     auto chain = [&](const ChainJob& a, const ChainJob* b) {
       const int total = b ? 2 * nc : nc;
       const dim3 gd((unsigned)up(total, 8));
-      if (total <= 256) PG_KLAUNCH((ns_chain_kernel<8>), gd, blk, 0, st, gr, a, b ? *b : a, total, nc, g);
-      else PG_KLAUNCH((ns_chain_kernel<4>), gd, blk, 0, st, gr, a, b ? *b : a, total, nc, g);
+      if (total <= 256) PG_KLAUNCH((ns_chain_kernel<4>), gd, dim3(1024), 0, st, gr, a, b ? *b : a, total, nc, g);
+      else PG_KLAUNCH((ns_chain_kernel<2>), gd, dim3(512), 0, st, gr, a, b ? *b : a, total, nc, g);
     };
     for (int k = 0; k < ns; ++k) {
       const int q = k == 0 ? 3 : 1;
@@ -1038,6 +1383,7 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
       else if (k > 0) chain(qp, nullptr);
       if (more) chain(qqg, nullptr);
       if (k > 0) { p = 7 - p; psc = SP; }
+    }
     }
     ApplyK a;
     memset(&a, 0, sizeof(a));
@@ -1067,9 +1413,21 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
 
 using namespace pg;
 
+namespace pg {
+// the one-launch form: short side <= 64, long side <= 384
+static bool ns_is_small(int64_t rows, int64_t cols) { return (rows < cols ? rows : cols) <= 64 && (rows < cols ? cols : rows) <= 384; }
+template <int SRC, int OUT>
+static void ns_small(const NsMat& m, const void* x, long xs, void* out, long os, long ldo, int steps, float eps, unsigned batch, hipStream_t st) {
+  if (m.Np <= 64) PG_KLAUNCH((ns_small_kernel<64, SRC, OUT>), dim3(batch), dim3(512), 0, st, m, x, xs, out, os, ldo, steps, eps);
+  else if (m.Np <= 192) PG_KLAUNCH((ns_small_kernel<192, SRC, OUT>), dim3(batch), dim3(512), 0, st, m, x, xs, out, os, ldo, steps, eps);
+  else PG_KLAUNCH((ns_small_kernel<384, SRC, OUT>), dim3(batch), dim3(512), 0, st, m, x, xs, out, os, ldo, steps, eps);
+}
+}  // namespace pg
+
 extern "C" int64_t pg_orthogonalise_workspace(int64_t batch, int64_t rows, int64_t cols) {
   if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
   if (batch > 0x3fffffff || rows > 0x7fffffff || cols > 0x7fffffff) return -1;
+  if (ns_is_small(rows, cols)) return 0;
   NsPlan pl{};
   return ns_plan_batch(pl, batch, rows, cols, 0, cols, 0) ? -1 : pl.bytes;
 }
@@ -1086,6 +1444,19 @@ extern "C" int pg_orthogonalise(const void* x, int32_t x_is_bf16, int64_t batch,
   PG_REQUIRE(((size_t)x & (x_is_bf16 ? 1 : 3)) == 0 && ((size_t)out & (out_is_bf16 ? 1 : 3)) == 0 && ((size_t)workspace & 255) == 0,
              "pg_orthogonalise: x / out aligned to their element, workspace to 256 bytes");
   PG_REQUIRE(batch <= 0x3fffffff && rows <= 0x7fffffff && cols <= 0x7fffffff, "pg_orthogonalise: sizes out of range");
+  if (ns_is_small(rows, cols)) {
+    NsMat m{};
+    m.taps = 1; m.rows = (int)rows; m.cols = (int)cols; m.ld = (long)ldx;
+    ns_shape(m);
+    hipStream_t st = (hipStream_t)stream;
+    const unsigned nb = (unsigned)batch;
+    if (x_is_bf16 && out_is_bf16) ns_small<1, 2>(m, x, (long)x_batch, out, (long)out_batch, (long)ldo, steps, eps, nb, st);
+    else if (x_is_bf16) ns_small<1, 1>(m, x, (long)x_batch, out, (long)out_batch, (long)ldo, steps, eps, nb, st);
+    else if (out_is_bf16) ns_small<0, 2>(m, x, (long)x_batch, out, (long)out_batch, (long)ldo, steps, eps, nb, st);
+    else ns_small<0, 1>(m, x, (long)x_batch, out, (long)out_batch, (long)ldo, steps, eps, nb, st);
+    PG_LAUNCH_OK("pg_orthogonalise");
+    return 0;
+  }
   NsPlan pl{};
   const char* bad = ns_plan_batch(pl, batch, rows, cols, x_batch, ldx, out_batch);
   PG_REQUIRE(bad == nullptr, "pg_orthogonalise: %s", bad);

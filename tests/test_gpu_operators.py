@@ -181,7 +181,7 @@ def close(got, ref, steps=5):
 
 
 SHAPES = [(1, 1, 1), (1, 1, 7), (1, 7, 1), (2, 2, 2), (3, 64, 64), (2, 65, 63), (1, 128, 300), (2, 300, 130), (1, 257, 1025), (1, 33, 4099),
-          (1, 4099, 33), (5, 16, 200), (1, 192, 9216), (1, 640, 700)]
+          (1, 4099, 33), (5, 16, 200), (1, 192, 9216), (1, 640, 700), (3, 50, 384), (2, 384, 64), (2, 64, 385), (2, 100, 2000)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
