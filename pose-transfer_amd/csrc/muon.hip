@@ -39,7 +39,7 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int SG = 12, SP = 10;                 // log2 of the scales of G, Q, Q G and of P
 // elements per workgroup of the momentum / square-sum pass: small tensors give few workgroups, large ones many partial sums
 __host__ __device__ constexpr int k0_elems(long n) { return n < (1L << 21) ? 4096 : 16384; }
-constexpr int GT = 128, CT = 64, AI = 128, AJ = 256;      // tiles: Gram, chain, apply (rows, columns)
+constexpr int GT = 128, AI = 128, AJ = 256;      // tiles: Gram; apply (rows, columns)
 
 struct NsMat {
   long src, ld, st;             // the caller's storage: element offset, row stride, tap stride
@@ -51,7 +51,7 @@ struct NsMat {
   long x, g, part;              // offsets in the workspace: X planes and chain planes (halves), Gram partials (floats)
   int sq0;                      // first partial sum of squares
 };
-enum { F_MOM, F_SPLIT, F_GRAM, F_JOIN, F_CHAIN, F_APPLY, F_N };       // launches
+enum { F_MOM, F_SPLIT, F_GRAM, F_JOIN, F_CHAIN, F_APPLY, F_N };       // launches (F_JOIN also: the chain's tiles of 32)
 struct NsGroup {                // matrices of one call: a device table, or (tab = nullptr) `n` equal ones
   const NsMat* tab;
   const int* first;             // [F_N][n]: the first workgroup of each record
@@ -404,21 +404,20 @@ __device__ __forceinline__ void fetch_nt(unsigned pa, unsigned pb, half8 (&a)[1]
                : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(b[0][0]), "=&v"(b[0][1]) : "v"(pa), "v"(pb) : "memory");
 }
 
-// C[BM][BM] = sum_k A[i][k] B[j][k] over columns k0 .. k1 - 1 (multiples of 32), operands as PL fp16 planes in blocks.  KG groups of 4 waves
-// (2 x 2) take every KG-th step of 32 columns, ST stages deep; `join` adds the groups' sums.  `same`: A and B are the same rows, moved
-// once.  Rows behind a_rows / b_rows read the last one instead: their products belong to rows and columns that nobody stores.
-template <int BM, int PL, int ST, int KG>
+// C[BM][BM] = sum_k A[i][k] B[j][k] over columns k0 .. k1 - 1 (multiples of 32), operands as PL fp16 planes in blocks; 4 waves (2 x 2), two
+// blocks per stage, ST stages.  `same`: A and B are the same rows, moved once.  Rows behind a_rows / b_rows read the last one instead:
+// their products belong to rows and columns that nobody stores.
+template <int BM, int PL, int ST>
 struct NtCore {
   static constexpr int T = BM / 64, BLK = BM * 32, OP = PL * 2 * BLK, STAGE = 2 * OP;      // [operand][plane][block][BM][16]
   static constexpr int NI = STAGE / 4096;                           // transfers per wave and stage
-  static constexpr int LDS_BYTES = KG * ST * STAGE;
-  static_assert((T == 1 || T == 2) && LDS_BYTES <= 128 * 1024, "tile");
+  static constexpr int LDS_BYTES = ST * STAGE;
+  static_assert((T == 1 || T == 2) && LDS_BYTES <= 64 * 1024, "tile");
   f32x16 acc[T][T];
 
   __device__ __forceinline__ void run(char* smem, const _Float16* A, int a_rows, const _Float16* B, int b_rows, long plane, int pitch, bool same,
                                       int k0, int k1) {
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wave = wv & 3, grp = wv >> 2;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BM / 2);
 #pragma unroll
     for (int i = 0; i < T; ++i)
@@ -426,27 +425,25 @@ struct NtCore {
       for (int j = 0; j < T; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    char* const base = smem + grp * (ST * STAGE);
     const _Float16* src[NI];
 #pragma unroll
     for (int q = 0; q < NI; ++q) {                   // transfer x of a stage: operand, plane, block, 32 rows
       const int x = q * 4 + wave, op = x / (NI * 2), y = x % (BM / 32), z = x / (BM / 32) % (PL * 2);
       const int row = y * 32 + (lane >> 1);
-      src[q] = (op ? B : A) + (z >> 1) * plane + ((long)(k0 / 16 + grp * 2 + (z & 1)) * pitch + min(row, (op ? b_rows : a_rows) - 1)) * 16 +
+      src[q] = (op ? B : A) + (z >> 1) * plane + ((long)(k0 / 16 + (z & 1)) * pitch + min(row, (op ? b_rows : a_rows) - 1)) * 16 +
                ((lane & 1) ^ swz(row)) * 8;
     }
-    const long step = 32L * KG * pitch;
+    const long step = 32L * pitch;
     auto issue = [&](int st) {
 #pragma unroll
       for (int q = 0; q < NI; ++q) {
         if (q == NI / 2 && same) break;
-        dma16(src[q], base + st * STAGE + (q * 4 + wave) * 1024);
+        dma16(src[q], smem + st * STAGE + (q * 4 + wave) * 1024);
         src[q] += step;
       }
     };
-    const int all = (k1 - k0) / 32, trips = (all + KG - 1) / KG;       // every wave meets every barrier
-    const int n = all > grp ? (all - grp + KG - 1) / KG : 0;
-    const unsigned lds0 = (unsigned)(size_t)base;
+    const int n = (k1 - k0) / 32;
+    const unsigned lds0 = (unsigned)(size_t)smem;
     const int r = lane & 31;
     const unsigned off = (unsigned)(r * 32 + (((lane >> 5) ^ swz(r)) << 4));
     const unsigned pa = lds0 + wm * 32 + off, pb = lds0 + (same ? 0 : OP) + wn * 32 + off;
@@ -454,13 +451,12 @@ struct NtCore {
     for (int q = 0; q < ST - 1; ++q)
       if (q < n) issue(q);
     int cur = 0, nxt = ST - 1;
-    for (int it = 0; it < trips; ++it) {
+    for (int it = 0; it < n; ++it) {
       if (it + ST - 2 >= n) wait_dma<0>();
       else if (same) wait_dma<NI / 2 * (ST - 2)>();
       else wait_dma<NI * (ST - 2)>();
       wg_barrier();
       if (it + ST - 1 < n) issue(nxt);
-      if (KG > 1 && it >= n) break;                                    // the last trip: no barrier follows
       const unsigned so = (unsigned)(cur * STAGE);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -485,31 +481,6 @@ struct NtCore {
       nxt = nxt + 1 == ST ? 0 : nxt + 1;
     }
   }
-  // the groups' sums, in order, to group 0 (T = 1); every wave calls it.  LDS is free afterwards
-  __device__ __forceinline__ void join(char* smem) {
-    static_assert(T == 1, "join");
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    float4* buf = reinterpret_cast<float4*>(smem);
-    __syncthreads();
-    if (KG > 1) {
-      if (wv >= 4) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          buf[((wv - 4) * 4 + q) * 64 + lane] = make_float4(acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]);
-      }
-      __syncthreads();
-      if (wv < 4) {
-#pragma unroll
-        for (int g = 1; g < KG; ++g)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4 f = buf[((g * 4 - 4 + wv) * 4 + q) * 64 + lane];
-            acc[0][0][4 * q] += f.x; acc[0][0][4 * q + 1] += f.y; acc[0][0][4 * q + 2] += f.z; acc[0][0][4 * q + 3] += f.w;
-          }
-      }
-      __syncthreads();
-    }
-  }
 };
 
 // tile number of the lower triangle (bi >= bj), row by row
@@ -524,7 +495,7 @@ __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
 // G = X X^T over one slice of the long side: fp32 partial tiles, in the order of the accumulators (one float4 = four rows of a column)
 template <int PL>
 __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int total, const _Float16* ws, float* part) {
-  typedef NtCore<GT, PL, 2, 1> Core;
+  typedef NtCore<GT, PL, 2> Core;
   __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
   const int b = xcd_tile(blockIdx.x, total, 10);
   if (b < 0) return;
@@ -592,14 +563,12 @@ __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, con
 
 // chain planes of a matrix: 0 G, 1 Q, 2 Q G, 3 P, 4 the other P  (hi and lo each)
 // C = A B of commuting symmetric matrices: the lower triangle of 64 x 64 tiles, mirrored.  `quad`: C = a I + b A + c A A
-// Tiles of 64 x 64.  Such a product is a few microseconds of latency (LDS read, three dependent MFMAs, barrier: 0.36 us per 32 columns
-// with 4 waves), so KG groups of 4 waves divide the columns: 4 groups (128 KB of stages) where there is at most one workgroup per CU, 2
-// (two workgroups per CU) otherwise.  The tile leaves through LDS in both orientations, 2 KB runs.
 struct ChainJob { int a, b, c; float mul; int quad; };
-template <int KG>
-__global__ __launch_bounds__(256 * KG, KG == 2 ? 4 : 4) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles,
-                                                                            _Float16* ws) {
-  typedef NtCore<CT, 2, 2, KG> Core;
+
+// Tiles of 64 x 64 (many matrices): four stages of 16 KB, two workgroups per CU.  The result leaves through LDS: written four
+// neighbours at a time as the mirrored tile, which is copied out as it is and, by transposing reads, turned.
+__global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
+  typedef NtCore<64, 2, 4> Core;
   __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
   const int t = xcd_tile(blockIdx.x, total, 36);
   if (t < 0) return;
@@ -614,17 +583,13 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 4 : 4) void ns_chain_kernel(con
   const _Float16* B = ws + m.g + jb.b * 2 * pl;
   _Float16* C = ws + m.g + jb.c * 2 * pl;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = ((wave >> 1) & 1) * 32, wn = (wave & 1) * 32, l31 = lane & 31;
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
   Core core;
-  core.run(smem, A + (long)bi * CT * 16, CT, B + (long)bj * CT * 16, CT, pl, Mp + 8, bi == bj && jb.a == jb.b, 0, Mp);
-  core.join(smem);
+  core.run(smem, A + (long)bi * 64 * 16, 64, B + (long)bj * 64 * 16, 64, pl, Mp + 8, bi == bj && jb.a == jb.b, 0, Mp);
   const f32x16& acc = core.acc[0][0];
-  // image of the tile: [orientation][plane][4 blocks][64 rows][16]
-  _Float16* img = reinterpret_cast<_Float16*>(smem);
-  auto im64 = [](int i, int j) { return ((j >> 4) * 64 + i) * 16 + (j & 15); };
   const bool diag = bi == bj;
-  const int j = wn + l31;
-  if (wave < 4) {
+  const int j = wn + (lane & 31);
+  __syncthreads();
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int i = wm + 8 * q + 4 * (lane >> 5);
@@ -632,7 +597,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 4 : 4) void ns_chain_kernel(con
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = acc[4 * q + e] * jb.mul;
     if (jb.quad) {                                   // A[i][j] from A[j][i]: four neighbours
-      const long at = cat(Mp, bj * CT + j, bi * CT + i);
+      const long at = cat(Mp, bj * 64 + j, bi * 64 + i);
       const half4 h = *reinterpret_cast<const half4*>(A + at), l = *reinterpret_cast<const half4*>(A + pl + at);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -642,35 +607,130 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 4 : 4) void ns_chain_kernel(con
     }
     half4 hh, ll;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      _Float16 h, l;
-      split16(v[e], h, l);
-      hh[e] = h; ll[e] = l;
-      if (!diag || i + e >= j) {
-        const int at = im64(i + e, j);
-        img[at] = h; img[4096 + at] = l;
-      }
-      if (diag && i + e > j) {
-        const int at = im64(j, i + e);
-        img[at] = h; img[4096 + at] = l;
-      }
-    }
-    if (!diag) {
-      const int at = im64(j, i);
-      *reinterpret_cast<half4*>(img + 8192 + at) = hh;
-      *reinterpret_cast<half4*>(img + 12288 + at) = ll;
-    }
-  }
+    for (int e = 0; e < 4; ++e) { _Float16 h, l; split16(v[e], h, l); hh[e] = h; ll[e] = l; }
+    char* at = smem + (i >> 4) * 2048 + j * 32 + (i & 15) * 2;       // [plane][block of i][64 rows j][16]
+    *reinterpret_cast<half4*>(at) = hh;
+    *reinterpret_cast<half4*>(at + 8192) = ll;
   }
   __syncthreads();
+  const unsigned lds0 = (unsigned)(size_t)smem;
 #pragma unroll
-  for (int q = 0; q < 8 / KG; ++q) {
-    const int x = q * (256 * KG) + tid, im = x >> 9, blk = (x >> 7) & 3, in = x & 127;
-    if (im >= 2 && diag) break;
-    const int rb = im < 2 ? bi : bj, cb = im < 2 ? bj : bi;
-    *reinterpret_cast<uint4*>(C + (im & 1) * pl + cat(Mp, rb * CT, (cb * 4 + blk) * 16) + in * 8) =
-        *reinterpret_cast<const uint4*>(img + im * 4096 + blk * 1024 + in * 8);
+  for (int q = 0; q < 4; ++q) {                      // plane q >> 1
+    const int x = (q & 1) * 256 + tid, blk = x >> 7, in = x & 127;
+    *reinterpret_cast<uint4*>(C + (q >> 1) * pl + cat(Mp, bj * 64, bi * 64 + blk * 16) + in * 8) =
+        *reinterpret_cast<const uint4*>(smem + (q >> 1) * 8192 + blk * 2048 + in * 16);
+    if (diag) continue;
+    // 16 lanes: 16 neighbours i, eight neighbours jc * 8 .. of each
+    const int ib = lane >> 4, jc = (q & 1) * 4 + wave, l = lane & 15;
+    half4 u, w;
+    asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:128\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(u), "=&v"(w) : "v"(lds0 + (unsigned)((q >> 1) * 8192 + ib * 2048 + (jc * 8 + (l >> 2)) * 32 + (l & 3) * 8)) : "memory");
+    *reinterpret_cast<half8*>(C + (q >> 1) * pl + cat(Mp, bi * 64 + ib * 16 + l, bj * 64 + jc * 8)) =
+        __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
   }
+}
+
+// Tiles of 32 x 32 (few matrices: at most two per CU).  Such a product is latency alone: launch, one round of transfers, a few dependent
+// MFMAs.  A workgroup brings the whole of its rows (KC columns at a time, 128 KB for 512) in one go; each of its 4 waves moves and
+// multiplies every fourth block, with no barrier before the sums are joined.
+template <int KC>
+__global__ __launch_bounds__(256) void ns_chain32_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
+  constexpr int NB = KC / 64;                        // blocks per wave and round
+  __shared__ __attribute__((aligned(1024))) char smem[4 * NB * 4096];
+  const int t = xcd_tile(blockIdx.x, total, (total + 7) / 8);
+  if (t < 0) return;
+  const ChainJob jb = t >= tiles ? j1 : j0;
+  const NsRef r = ns_find<F_JOIN>(gr, t >= tiles ? t - tiles : t);
+  const NsMat& m = r.m;
+  int bi, bj;
+  tri(r.tile, bi, bj);
+  const int Mp = m.Mp;
+  const long pl = cplane(m);
+  const _Float16* A = ws + m.g + jb.a * 2 * pl;
+  const _Float16* B = ws + m.g + jb.b * 2 * pl;
+  _Float16* C = ws + m.g + jb.c * 2 * pl;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool diag = bi == bj;
+  const int row = lane >> 1;
+  const long step = 64L * (Mp + 8);                  // four blocks
+  const long own = (long)wave * 16 * (Mp + 8) + row * 16 + ((lane & 1) ^ swz(row)) * 8;
+  const _Float16* pa = A + (long)bi * 32 * 16 + own;
+  const _Float16* pb = B + (long)bj * 32 * 16 + own;
+  // this wave's LDS: [block][A hi, A lo, B hi, B lo][32 rows][16]
+  char* const base = smem + wave * (NB * 4096);
+  const unsigned lds0 = (unsigned)(size_t)base + (lane & 31) * 32 + (((lane >> 5) ^ swz(lane & 31)) << 4);
+  // the four values of A that a quadratic form needs, on their way early
+  const int i = 8 * wave + 4 * (lane >> 5), j = lane & 31;
+  half4 gh = {0, 0, 0, 0}, gl = {0, 0, 0, 0};
+  if (jb.quad) {
+    const long at = cat(Mp, bj * 32 + j, bi * 32 + i);
+    gh = *reinterpret_cast<const half4*>(A + at);
+    gl = *reinterpret_cast<const half4*>(A + pl + at);
+  }
+  f32x16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  int left = Mp / 64;                                // blocks of this wave
+  while (left > 0) {
+    const int nb = min(left, NB);
+    left -= nb;
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      if (u >= nb) break;
+      dma16(pa, base + u * 4096);
+      dma16(pa + pl, base + u * 4096 + 1024);
+      dma16(pb, base + u * 4096 + 2048);
+      dma16(pb + pl, base + u * 4096 + 3072);
+      pa += step; pb += step;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < NB; ++s) {                   // block s - (NB - nb): behind it 4 (NB - 1 - s) transfers are in flight
+      const int u = s - (NB - nb);
+      if (u < 0) continue;
+      switch (NB - 1 - s) {
+        case 7: wait_dma<28>(); break;
+        case 6: wait_dma<24>(); break;
+        case 5: wait_dma<20>(); break;
+        case 4: wait_dma<16>(); break;
+        case 3: wait_dma<12>(); break;
+        case 2: wait_dma<8>(); break;
+        case 1: wait_dma<4>(); break;
+        default: wait_dma<0>(); break;
+      }
+      half8 a[2][1], b[2][1];
+      const unsigned q = lds0 + u * 4096;
+      fetch_nt<1024>(q, q + 2048, a, b);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][0], b[0][0], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][0], b[1][0], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][0], b[0][0], acc, 0, 0, 0);
+    }
+  }
+  // sums of the four waves, in order: wave w finishes rows 8 w .. 8 w + 7
+  __syncthreads();
+  float4* buf = reinterpret_cast<float4*>(smem);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) buf[(wave * 4 + q) * 64 + lane] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+  __syncthreads();
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float4 f = buf[(w * 4 + wave) * 64 + lane];
+    v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+  }
+  const int gi = bi * 32 + i, gj = bj * 32 + j;
+  half4 hh, ll;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] *= jb.mul;
+    if (jb.quad) v[e] += NS_B * ((float)gh[e] + (float)gl[e]) + (gi + e == gj ? NS_A * (float)(1 << SG) : 0.f);
+    _Float16 h, l;
+    split16(v[e], h, l);
+    hh[e] = h; ll[e] = l;
+    if (!diag) { C[cat(Mp, gi + e, gj)] = h; C[pl + cat(Mp, gi + e, gj)] = l; }
+  }
+  *reinterpret_cast<half4*>(C + cat(Mp, gj, gi)) = hh;
+  *reinterpret_cast<half4*>(C + pl + cat(Mp, gj, gi)) = ll;
 }
 
 // ---------------------------------------------------------------------------------------------- X <- P X
@@ -1359,7 +1419,8 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     // buffers: 0 G, 1 Q, 2 Q G, 3 and 4 P in turn; the first step's Q is the first P (and keeps Q's scale)
     const float q1 = 1.f / (float)(1 << SG);
     int p = 3, psc = SG;
-    const int nc = (int)pl.n[F_CHAIN];
+    const bool many = pl.n[F_JOIN] > 512;
+    const int nc = (int)pl.n[many ? F_CHAIN : F_JOIN];
     if (pl.top <= 128) {
       const dim3 gm((unsigned)gr.n);
       if (pl.top == 64) PG_KLAUNCH((ns_chain_small_kernel<64>), gm, blk, 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
@@ -1370,8 +1431,10 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     auto chain = [&](const ChainJob& a, const ChainJob* b) {
       const int total = b ? 2 * nc : nc;
       const dim3 gd((unsigned)up(total, 8));
-      if (total <= 256) PG_KLAUNCH((ns_chain_kernel<4>), gd, dim3(1024), 0, st, gr, a, b ? *b : a, total, nc, g);
-      else PG_KLAUNCH((ns_chain_kernel<2>), gd, dim3(512), 0, st, gr, a, b ? *b : a, total, nc, g);
+      const ChainJob b1 = b ? *b : a;
+      if (many) PG_KLAUNCH(ns_chain_kernel, gd, blk, 0, st, gr, a, b1, total, nc, g);
+      else if (pl.top <= 256) PG_KLAUNCH((ns_chain32_kernel<256>), gd, blk, 0, st, gr, a, b1, total, nc, g);
+      else PG_KLAUNCH((ns_chain32_kernel<512>), gd, blk, 0, st, gr, a, b1, total, nc, g);
     };
     for (int k = 0; k < ns; ++k) {
       const int q = k == 0 ? 3 : 1;
