@@ -297,11 +297,12 @@ struct RmsBwdK {
 };
 
 // A group of LPR lanes walks rows; every lane keeps the dgamma sums of its own columns in registers, the workgroup's groups are
-// joined in LDS, the workgroups by rms_dgamma_kernel (one workgroup: written here).  No atomics: the order is fixed.
-template <typename T, int LPR, int NCH>
-__global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdK p) {
-  constexpr int V = RmsV<T>::N, G = 256 / LPR;
-  __shared__ float red[256 * NCH * V];
+// joined in LDS, the workgroups by rms_dgamma_kernel (one workgroup: written here).  No atomics: the order is fixed.  WG: 256 lanes, or 1024
+// for the few rows that one workgroup handles by itself (a second launch costs more than the rows).
+template <typename T, int LPR, int NCH, int WG>
+__global__ __launch_bounds__(WG) void rms_bwd_kernel(const RmsBwdK p) {
+  constexpr int V = RmsV<T>::N, G = WG / LPR;
+  __shared__ float red[WG * NCH * V];
   const int ln = threadIdx.x % LPR, grp = threadIdx.x / LPR;
   float acc[NCH][V], gain[NCH][V];
 #pragma unroll
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdK p) {
 #pragma unroll
     for (int e = 0; e < V; ++e) red[(grp * NCH + i) * LPR * V + ln * V + e] = acc[i][e];
   __syncthreads();
-  for (int c = threadIdx.x; c < p.C; c += 256) {
+  for (int c = threadIdx.x; c < p.C; c += WG) {
     float t = 0.f;
     for (int k = 0; k < G; ++k) t += red[k * NCH * LPR * V + c];
     if (gridDim.x == 1) p.dgamma[c] = p.accumulate ? p.dgamma[c] + t : t;
@@ -431,11 +432,13 @@ static void rms_shape(int C, int V, int group, int& lpr, int& nch) {
   while (nch * lpr * V < C) nch *= 2;
   if (nch * V > 32) nch = 0;
 }
-static long rms_bwd_blocks(long rows, int lpr) {
+// at most eight rows per group of a workgroup of 1024 lanes: it writes dgamma itself
+static bool rms_bwd_single(long rows, int lpr, int nch) { return nch == 1 && rows <= 8 * (1024 / lpr); }
+static long rms_bwd_blocks(long rows, int lpr, int nch) {
+  if (rms_bwd_single(rows, lpr, nch)) return 1;
   const long g = 256 / lpr;
   long b = (rows + g - 1) / g;
-  // few rows: one workgroup that writes dgamma itself; otherwise at least two rows per group, at most 4 workgroups per CU
-  if (b <= 16) return 1;
+  // otherwise at least two rows per group, at most 4 workgroups per CU
   b = (b + 1) / 2;
   return b > 1024 ? 1024 : b;
 }
@@ -511,7 +514,7 @@ extern "C" int64_t pg_rms_norm_bwd_workspace(int64_t rows, int32_t C, int32_t io
   if (rows <= 0 || C <= 0) return 0;
   int lpr, nch;
   rms_shape(C, io_flags ? 8 : 4, 0, lpr, nch);
-  const long nb = nch ? rms_bwd_blocks(rows, lpr) : rms_long_slices(rows);
+  const long nb = nch ? rms_bwd_blocks(rows, lpr, nch) : rms_long_slices(rows);
   return nch && nb == 1 ? 0 : (int64_t)nb * C * 4;
 }
 
@@ -535,30 +538,37 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
   }
   int lpr, nch;
   rms_shape(C, io_flags ? 8 : 4, 0, lpr, nch);
-  const long nb = nch ? rms_bwd_blocks(rows, lpr) : rms_long_slices(rows);
+  const long nb = nch ? rms_bwd_blocks(rows, lpr, nch) : rms_long_slices(rows);
   PG_REQUIRE(nch || rows < (1L << 31), "pg_rms_norm_bwd: too many rows");
   PG_REQUIRE(nch || (dx != dy && dx != dh && dx != h), "pg_rms_norm_bwd: rows of more than 2048 channels are read twice: dx must not be an input");
   PG_REQUIRE(dx != dy || lddy == C, "pg_rms_norm_bwd: dx in place of dy needs lddy == C");
   RmsBwdK k = {dy, dh, h, rstd, gamma, (long)rows, C, (long)lddy, dx, (float*)workspace, dgamma, accumulate};
-#define PG_RB1(T, L, N) PG_KLAUNCH((rms_bwd_kernel<T, L, N>), dim3((unsigned)nb), dim3(256), 0, st, k)
+  const bool single = rms_bwd_single(rows, lpr, nch);
+#define PG_RBN(T, L, N) PG_KLAUNCH((rms_bwd_kernel<T, L, N, 256>), dim3((unsigned)nb), dim3(256), 0, st, k)
+#define PG_RB1(T, L)                                                                                               \
+  do {                                                                                                             \
+    if (single) PG_KLAUNCH((rms_bwd_kernel<T, L, 1, 1024>), dim3(1), dim3(1024), 0, st, k);                        \
+    else PG_RBN(T, L, 1);                                                                                          \
+  } while (0)
 #define PG_RB(T)                                                                                                   \
   do {                                                                                                             \
     if (nch == 0) {                                                                                                \
       PG_KLAUNCH((rms_bwd_long_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, k);                             \
       PG_KLAUNCH((rms_dgamma_long_kernel<T>), dim3((C + 255) / 256, (unsigned)nb), dim3(256), 0, st, k);           \
     }                                                                                                              \
-    else if (lpr == 8) PG_RB1(T, 8, 1);                                                                            \
-    else if (lpr == 16) PG_RB1(T, 16, 1);                                                                          \
-    else if (lpr == 32) PG_RB1(T, 32, 1);                                                                          \
-    else if (nch == 1) PG_RB1(T, 64, 1);                                                                           \
-    else if (nch == 2) PG_RB1(T, 64, 2);                                                                           \
-    else if (nch == 4) PG_RB1(T, 64, 4);                                                                           \
-    else PG_RB1(T, 64, 32 / RmsV<T>::N);                                                                           \
+    else if (lpr == 8) PG_RB1(T, 8);                                                                               \
+    else if (lpr == 16) PG_RB1(T, 16);                                                                             \
+    else if (lpr == 32) PG_RB1(T, 32);                                                                             \
+    else if (nch == 1) PG_RB1(T, 64);                                                                              \
+    else if (nch == 2) PG_RBN(T, 64, 2);                                                                           \
+    else if (nch == 4) PG_RBN(T, 64, 4);                                                                           \
+    else PG_RBN(T, 64, 32 / RmsV<T>::N);                                                                           \
   } while (0)
   if (io_flags == 0) PG_RB(float);
   else PG_RB(bf16_t);
 #undef PG_RB
 #undef PG_RB1
+#undef PG_RBN
   if (!(nch && nb == 1))
     PG_KLAUNCH(rms_dgamma_kernel, dim3((C + 31) / 32), dim3(1024), 0, st, (const float*)workspace, (int)nb, C, dgamma, accumulate);
   PG_LAUNCH_OK("pg_rms_norm_bwd");

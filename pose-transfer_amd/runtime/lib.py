@@ -227,6 +227,11 @@ def stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def current_device():
+    """index of torch's current device"""
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
+
+
 def ptr(t):
     """device pointer of a tensor (None -> NULL)."""
     if t is None:

@@ -22,11 +22,13 @@ _IO = {torch.float32: 0, torch.bfloat16: 3}
 class _On:
     """the tensors' device as the current one while a call enqueues (a no-op where it already is)"""
 
-    def __init__(self, device):
-        self.prev, self.idx = None, device.index
+    __slots__ = ("prev", "idx")
+
+    def __init__(self, t):
+        self.prev, self.idx = None, t.get_device()
 
     def __enter__(self):
-        cur = torch.cuda.current_device()
+        cur = L.current_device()
         if cur != self.idx:
             self.prev = cur
             torch.cuda.set_device(self.idx)
@@ -42,39 +44,47 @@ def _need(cond, msg):
         raise ValueError(msg)
 
 
-def _rows(t, name, dtype, device, shape=None):
-    """a 2-D tensor with unit column stride; its row stride"""
-    _need(torch.is_tensor(t) and t.dim() == 2, "%s: a 2-D tensor [rows, channels] is required" % name)
-    _need(t.dtype == dtype and t.device == device, "%s: %s on %s expected, got %s on %s" % (name, dtype, device, t.dtype, t.device))
-    _need(shape is None or tuple(t.shape) == tuple(shape), "%s: shape %s expected, got %s" % (name, shape and tuple(shape), tuple(t.shape)))
-    _need(t.shape[1] <= 1 or t.stride(1) == 1, "%s: channels must be contiguous" % name)
-    ld = t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
-    _need(ld >= t.shape[1], "%s: rows overlap" % name)
-    return ld
+# (the messages are formatted only when raised: these checks are most of a small call's host time)
+def _rows(t, name, like, shape):
+    """row stride of a 2-D tensor [rows, channels] of like's type and device with unit column stride"""
+    if not (torch.is_tensor(t) and t.dtype == like.dtype and t.device == like.device and t.shape == shape and len(shape) == 2):
+        raise ValueError("%s: %s %s on %s expected" % (name, like.dtype, tuple(shape), like.device))
+    s0, s1 = t.stride()
+    rows, ch = shape
+    if s1 != 1 and ch > 1:
+        raise ValueError("%s: channels must be contiguous" % name)
+    if rows <= 1:
+        return ch if ch > 0 else 1
+    if s0 < ch:
+        raise ValueError("%s: rows overlap" % name)
+    return s0
+
+
+def _vector(t, name, like, n):
+    if not (torch.is_tensor(t) and t.dtype == torch.float32 and t.device == like.device and t.dim() == 1 and t.shape[0] == n
+            and (n <= 1 or t.stride(0) == 1)):
+        raise ValueError("%s: a contiguous fp32 vector of %d on %s expected" % (name, n, like.device))
 
 
 def _norm_args(x, gamma, residual):
-    _need(torch.is_tensor(x) and x.is_cuda and x.dtype in _IO, "rms_norm: x must be an fp32 or bf16 tensor on the GPU")
-    ldx = _rows(x, "x", x.dtype, x.device)
-    rows, ch = x.shape
-    _need(ch > 0, "rms_norm: no channels")
-    _need(torch.is_tensor(gamma) and gamma.dtype == torch.float32 and gamma.device == x.device and tuple(gamma.shape) == (ch,)
-          and (ch == 1 or gamma.stride(0) == 1), "rms_norm: gamma must be a contiguous fp32 [%d] on x's device" % ch)
-    ldr = 0 if residual is None else _rows(residual, "residual", x.dtype, x.device, x.shape)
-    return rows, ch, ldx, ldr
+    if not (torch.is_tensor(x) and x.is_cuda and x.dtype in _IO and x.dim() == 2 and x.shape[1] > 0):
+        raise ValueError("rms_norm: x must be an fp32 or bf16 [rows, channels] tensor on the GPU")
+    shape = x.shape
+    _vector(gamma, "gamma", x, shape[1])
+    return shape[0], shape[1], _rows(x, "x", x, shape), 0 if residual is None else _rows(residual, "residual", x, shape)
 
 
 def rms_norm(x, gamma, residual=None, eps=1e-6):
     """y = h * rstd * gamma with h = x + residual (rounded to x's type), rstd = (mean_c h^2 + eps)^-1/2.
     Returns (y, h, rstd); h is x where there is no residual.  x [rows, C] fp32 or bf16, rows may be strided; gamma fp32 [C]."""
     rows, ch, ldx, ldr = _norm_args(x, gamma, residual)
-    with _On(x.device):
-        y = torch.empty((rows, ch), dtype=x.dtype, device=x.device)
-        h = torch.empty_like(y) if residual is not None else None
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    with _On(x):
+        y = x.new_empty((rows, ch))
+        h = None if residual is None else torch.empty_like(y)
+        rstd = gamma.new_empty(rows)
         if rows:
-            L.call("pg_rms_norm_fwd", L.ptr(x), L.ptr(residual), L.ptr(gamma), rows, ch, ldx, ldr, eps, _IO[x.dtype], L.ptr(h),
-                   L.ptr(y), ch, None, None, 0, L.ptr(rstd), L.stream())
+            L.call("pg_rms_norm_fwd", x.data_ptr(), L.ptr(residual), gamma.data_ptr(), rows, ch, ldx, ldr, eps, _IO[x.dtype], L.ptr(h),
+                   y.data_ptr(), ch, None, None, 0, rstd.data_ptr(), L.stream())
     return y, (x if h is None else h), rstd
 
 
@@ -82,37 +92,40 @@ def rms_norm_q8(x, gamma, residual=None, eps=1e-6, group=0):
     """the norm's output in 8 bits: (q, scale, h, rstd), q float8_e4m3fn [rows, C], value = q * scale with one fp32 scale per
     `group` channels (0: per row; scale [rows, ceil(C / group)])."""
     rows, ch, ldx, ldr = _norm_args(x, gamma, residual)
-    _need(group in GROUPS, "rms_norm_q8: group must be one of %s" % (GROUPS,))
-    with _On(x.device):
-        q = torch.empty((rows, ch), dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty((rows, -(-ch // group) if group else 1), dtype=torch.float32, device=x.device)
-        h = torch.empty((rows, ch), dtype=x.dtype, device=x.device) if residual is not None else None
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if group not in GROUPS:
+        raise ValueError("rms_norm_q8: group must be one of %s" % (GROUPS,))
+    with _On(x):
+        q = x.new_empty((rows, ch), dtype=torch.float8_e4m3fn)
+        scale = gamma.new_empty((rows, -(-ch // group) if group else 1))
+        h = None if residual is None else x.new_empty((rows, ch))
+        rstd = gamma.new_empty(rows)
         if rows:
-            L.call("pg_rms_norm_fwd", L.ptr(x), L.ptr(residual), L.ptr(gamma), rows, ch, ldx, ldr, eps, _IO[x.dtype], L.ptr(h), None,
-                   0, L.ptr(q), L.ptr(scale), group, L.ptr(rstd), L.stream())
+            L.call("pg_rms_norm_fwd", x.data_ptr(), L.ptr(residual), gamma.data_ptr(), rows, ch, ldx, ldr, eps, _IO[x.dtype], L.ptr(h), None,
+                   0, q.data_ptr(), scale.data_ptr(), group, rstd.data_ptr(), L.stream())
     return q, scale, (x if h is None else h), rstd
 
 
 def rms_norm_bwd(dy, h, rstd, gamma, dh=None):
     """(dx, dgamma) of ``rms_norm``: dx is also the residual's gradient; dh: the gradient that reaches h past the norm."""
-    _need(torch.is_tensor(h) and h.is_cuda and h.dtype in _IO, "rms_norm_bwd: h must be an fp32 or bf16 tensor on the GPU")
-    rows, ch = h.shape if h.dim() == 2 else (0, 0)
-    _need(ch > 0 and _rows(h, "h", h.dtype, h.device) == ch, "rms_norm_bwd: h must be a packed [rows, C] tensor")
-    lddy = _rows(dy, "dy", h.dtype, h.device, h.shape)
-    _need(dh is None or _rows(dh, "dh", h.dtype, h.device, h.shape) == ch, "rms_norm_bwd: dh must be packed")
-    for name, t, n in (("rstd", rstd, rows), ("gamma", gamma, ch)):
-        _need(torch.is_tensor(t) and t.dtype == torch.float32 and t.device == h.device and tuple(t.shape) == (n,)
-              and (n <= 1 or t.stride(0) == 1), "rms_norm_bwd: %s must be a contiguous fp32 [%d] on h's device" % (name, n))
-    with _On(h.device):
-        dx = torch.empty((rows, ch), dtype=h.dtype, device=h.device)
-        dgamma = torch.empty(ch, dtype=torch.float32, device=h.device)
+    if not (torch.is_tensor(h) and h.is_cuda and h.dtype in _IO and h.dim() == 2 and h.shape[1] > 0):
+        raise ValueError("rms_norm_bwd: h must be an fp32 or bf16 [rows, channels] tensor on the GPU")
+    shape = h.shape
+    rows, ch = shape
+    if _rows(h, "h", h, shape) != ch or (dh is not None and _rows(dh, "dh", h, shape) != ch):
+        raise ValueError("rms_norm_bwd: h and dh must be packed")
+    lddy = _rows(dy, "dy", h, shape)
+    _vector(rstd, "rstd", h, rows)
+    _vector(gamma, "gamma", h, ch)
+    with _On(h):
+        dx = torch.empty_like(h)
+        dgamma = torch.empty_like(gamma)
         if rows == 0:
             return dx, dgamma.zero_()
-        need = L.load().pg_rms_norm_bwd_workspace(rows, ch, _IO[h.dtype])
+        io = _IO[h.dtype]
+        need = L.load().pg_rms_norm_bwd_workspace(rows, ch, io)
         ws = torch.empty(need, dtype=torch.uint8, device=h.device) if need else None
-        L.call("pg_rms_norm_bwd", L.ptr(dy), lddy, L.ptr(dh), L.ptr(h), L.ptr(rstd), L.ptr(gamma), rows, ch, _IO[h.dtype], L.ptr(dx),
-               L.ptr(dgamma), 0, L.ptr(ws), need, L.stream())
+        L.call("pg_rms_norm_bwd", dy.data_ptr(), lddy, L.ptr(dh), h.data_ptr(), rstd.data_ptr(), gamma.data_ptr(), rows, ch, io,
+               dx.data_ptr(), dgamma.data_ptr(), 0, L.ptr(ws), need, L.stream())
     return dx, dgamma
 
 
@@ -127,12 +140,12 @@ def orthogonalise(x, steps=5, eps=1e-7, out_dtype=None):
     b, r, c = x3.shape
     if c > 1 and x3.stride(2) != 1 or r > 1 and x3.stride(1) < c or b > 1 and x3.stride(0) < 0:
         x3 = x3.contiguous()
-    with _On(x.device):
+    with _On(x):
         out = torch.empty((b, r, c), dtype=out_dtype, device=x.device)
         if out.numel():
             need = L.load().pg_orthogonalise_workspace(b, r, c)
             _need(need >= 0, "orthogonalise: sizes out of range")
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
             L.call("pg_orthogonalise", L.ptr(x3), int(x.dtype == torch.bfloat16), b, r, c, x3.stride(0) if b > 1 else 0,
                    x3.stride(1) if r > 1 else c, L.ptr(out), int(out_dtype == torch.bfloat16), r * c, c, steps, eps, L.ptr(ws), need,
                    L.stream())
@@ -160,17 +173,17 @@ def muon_step(p, g, m, v, table, lr, momentum=0.95, nesterov=True, weight_decay=
         if t is None and name in ("v", "p_bf16"):
             continue
         _need(torch.is_tensor(t) and t.dtype in dts and t.device == p.device and t.shape == p.shape and t.is_contiguous(),
-              "muon_step: %s must be a contiguous arena like p" % name)
+              "muon_step: g, m, v and p_bf16 must be contiguous arenas like p (g fp32 or bf16, m and v fp32, p_bf16 bf16)")
     _need(ctr is None or (torch.is_tensor(ctr) and ctr.dtype == torch.int64 and ctr.device == p.device and ctr.numel() >= 1),
           "muon_step: ctr must be an int64 tensor on p's device")
     if len(table) == 0:
         return
-    with _On(p.device):
+    with _On(p):
         need = muon_workspace(table)
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=p.device)
-        _need(workspace.dtype == torch.uint8 and workspace.device == p.device and workspace.is_contiguous() and workspace.numel() >= need,
-              "muon_step: workspace must be a contiguous uint8 tensor of %d bytes on p's device" % need)
+        if not (workspace.dtype == torch.uint8 and workspace.device == p.device and workspace.is_contiguous() and workspace.numel() >= need):
+            raise ValueError("muon_step: workspace must be a contiguous uint8 tensor of %d bytes on p's device" % need)
         d = L.MuonDesc(p=L.ptr(p), m=L.ptr(m), v=L.ptr(v), p_bf16=L.ptr(p_bf16), entries=table.ctypes.data, total=p.numel(),
                        n=len(table), nesterov=int(bool(nesterov)), steps=ns_steps, lr=lr, momentum=momentum, weight_decay=weight_decay,
                        grad_scale=grad_scale, eps=ns_eps, beta1=betas[0], beta2=betas[1], adam_eps=eps, step=step, ctr=L.ptr(ctr),
