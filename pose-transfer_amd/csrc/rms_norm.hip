@@ -28,59 +28,120 @@ __device__ __forceinline__ void rms_st1(bf16_t* p, float v) { *p = (bf16_t)(rms_
 __device__ __forceinline__ float rms_round(float v, const float*) { return v; }
 __device__ __forceinline__ float rms_round(float v, const bf16_t*) { return __uint_as_float(rms_pack_bf16(v, 0.f) << 16); }
 
-struct __attribute__((packed, aligned(2))) RmsU4 { unsigned x, y, z, w; };     // 16 bytes at the alignment of one element
+struct __attribute__((packed, aligned(2))) RmsU4 { unsigned x, y, z, w; };     // 16, 8, 4 bytes at the alignment of one element
+struct __attribute__((packed, aligned(2))) RmsU2 { unsigned x, y; };
+struct __attribute__((packed, aligned(2))) RmsU1 { unsigned x; };
 struct __attribute__((packed, aligned(4))) RmsF4 { float x, y, z, w; };
+struct __attribute__((packed, aligned(4))) RmsF2 { float x, y; };
 struct __attribute__((packed, aligned(1))) RmsB8 { unsigned x, y; };
 struct __attribute__((packed, aligned(1))) RmsB4 { unsigned x; };
+struct __attribute__((packed, aligned(1))) RmsB2 { unsigned short x; };
 
 template <typename T> struct RmsV { static constexpr int N = 16 / (int)sizeof(T); };
 
-// the chunk of RmsV<T>::N elements that starts at column c of a row of C elements; zero behind the row's end
-template <typename T>
-__device__ __forceinline__ void rms_load(const T* row, int c, int C, float (&v)[RmsV<T>::N]) {
-  constexpr int V = RmsV<T>::N;
-  if (c + V <= C) {
-    const RmsU4 u = *reinterpret_cast<const RmsU4*>(row + c);
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+// A chunk that crosses the row's end is read from the row's last V elements instead and moved down by d = V - C % V places, so that every
+// load is one unconditional instruction (loads under a branch of their own were waited for one by one).  d is the same for all lanes.
+__device__ __forceinline__ void rms_down(unsigned (&w)[4], int d, const bf16_t*) {
+  if (d & 4) { w[0] = w[2]; w[1] = w[3]; w[2] = w[3] = 0u; }
+  if (d & 2) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = 0u; }
+  if (d & 1) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (V == 4) v[e] = __uint_as_float(w[e]);
-      else { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
-    }
-  } else {
+    for (int k = 0; k < 3; ++k) w[k] = (w[k] >> 16) | (w[k + 1] << 16);
+    w[3] >>= 16;
+  }
+}
+__device__ __forceinline__ void rms_down(unsigned (&w)[4], int d, const float*) {
+  if (d & 2) { w[0] = w[2]; w[1] = w[3]; w[2] = w[3] = 0u; }
+  if (d & 1) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = 0u; }
+}
+__device__ __forceinline__ void rms_put_tail(bf16_t* q, int n, const unsigned (&w)[4]) {
+  if (n & 4) { RmsU2 u; u.x = w[0]; u.y = w[1]; *reinterpret_cast<RmsU2*>(q) = u; }
+  if (n & 2) reinterpret_cast<RmsU1*>(q + (n & 4))->x = (n & 4) ? w[2] : w[0];
+  if (n & 1) {
+    unsigned u = w[0];
+#pragma unroll
+    for (int k = 1; k < 4; ++k)
+      if (k == (n >> 1)) u = w[k];
+    q[n & 6] = (bf16_t)u;
+  }
+}
+__device__ __forceinline__ void rms_put_tail(float* q, int n, const unsigned (&w)[4]) {
+  if (n & 2) { RmsF2 u; u.x = __uint_as_float(w[0]); u.y = __uint_as_float(w[1]); *reinterpret_cast<RmsF2*>(q) = u; }
+  if (n & 1) q[n & 2] = __uint_as_float((n & 2) ? w[2] : w[0]);
+}
+// the chunk of RmsV<T>::N elements that starts at column c (a multiple of it) of a row of C elements; zero behind the row's end
+// `ex` (a constant at every call): the chunk is known to be full
+template <typename T>
+__device__ __forceinline__ void rms_load(bool ex, const T* row, int c, int C, float (&v)[RmsV<T>::N]) {
+  constexpr int V = RmsV<T>::N;
+  if (!ex && C < V) {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = (c + e < C) ? rms_ld1(row + c + e) : 0.f;
+    return;
+  }
+  const RmsU4 u = *reinterpret_cast<const RmsU4*>(row + (ex ? c : min(c, C - V)));
+  unsigned w[4] = {u.x, u.y, u.z, u.w};
+  if (!ex && (C & (V - 1))) {
+    unsigned t[4] = {u.x, u.y, u.z, u.w};
+    rms_down(t, V - (C & (V - 1)), row);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = c + V > C ? t[e] : w[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (!ex) w[e] = c < C ? w[e] : 0u;
+    if constexpr (V == 4) v[e] = __uint_as_float(w[e]);
+    else { v[2 * e] = __uint_as_float(w[e] << 16); v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
   }
 }
 template <typename T>
-__device__ __forceinline__ void rms_store(T* row, int c, int C, const float (&v)[RmsV<T>::N]) {
+__device__ __forceinline__ void rms_store(bool ex, T* row, int c, int C, const float (&v)[RmsV<T>::N]) {
   constexpr int V = RmsV<T>::N;
-  if (c + V <= C) {
+  if (!ex && c >= C) return;
+  unsigned w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (V == 4) w[e] = __float_as_uint(v[e]);
+    else w[e] = rms_pack_bf16(v[2 * e], v[2 * e + 1]);
+  }
+  if (ex || c + V <= C) {
     RmsU4 u;
-    if constexpr (V == 4) {
-      u.x = __float_as_uint(v[0]); u.y = __float_as_uint(v[1]); u.z = __float_as_uint(v[2]); u.w = __float_as_uint(v[3]);
-    } else {
-      u.x = rms_pack_bf16(v[0], v[1]); u.y = rms_pack_bf16(v[2], v[3]); u.z = rms_pack_bf16(v[4], v[5]); u.w = rms_pack_bf16(v[6], v[7]);
-    }
+    u.x = w[0]; u.y = w[1]; u.z = w[2]; u.w = w[3];
     *reinterpret_cast<RmsU4*>(row + c) = u;
   } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (c + e < C) rms_st1(row + c + e, v[e]);
+    rms_put_tail(row + c, C & (V - 1), w);
   }
 }
 template <int V>
-__device__ __forceinline__ void rms_gain(const float* g, int c, int C, float (&v)[V]) {
-  if (c + V <= C) {
-#pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      const RmsF4 f = *reinterpret_cast<const RmsF4*>(g + c + 4 * q);
-      v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
-    }
-  } else {
+__device__ __forceinline__ void rms_gain(bool ex, const float* g, int c, int C, float (&v)[V]) {
+  if (!ex && C < V) {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = (c + e < C) ? g[c + e] : 0.f;
+    return;
   }
+  const float* q = g + (ex ? c : min(c, C - V));
+#pragma unroll
+  for (int k = 0; k < V / 4; ++k) {
+    const RmsF4 f = *reinterpret_cast<const RmsF4*>(q + 4 * k);
+    v[4 * k] = f.x; v[4 * k + 1] = f.y; v[4 * k + 2] = f.z; v[4 * k + 3] = f.w;
+  }
+  if (!ex && (C & (V - 1))) {
+    const int d = V - (C & (V - 1));
+    float t[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) t[e] = v[e];
+#pragma unroll
+    for (int b = V / 2; b > 0; b >>= 1)
+      if (d & b) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[e] = e + b < V ? t[e + b] : 0.f;
+      }
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = c + V > C ? t[e] : v[e];
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (!ex) v[e] = c < C ? v[e] : 0.f;
 }
 template <int LPR>
 __device__ __forceinline__ float group_sum(float v, int lpr = LPR) {
@@ -103,7 +164,7 @@ struct Q8 {
 // round to nearest even; |t| <= 448 up to the rounding of the quotient, which the comparison takes off; NaN stays NaN
 __device__ __forceinline__ float q8_clip(float t) { return t > 448.f ? 448.f : (t < -448.f ? -448.f : t); }
 template <int V>
-__device__ __forceinline__ void q8_store(uint8_t* row, int c, int C, const float (&h)[V], const float (&g)[V], const Q8& k) {
+__device__ __forceinline__ void q8_store(bool ex, uint8_t* row, int c, int C, const float (&h)[V], const float (&g)[V], const Q8& k) {
   unsigned w[V / 4];
   float t[V];
 #pragma unroll
@@ -115,13 +176,16 @@ __device__ __forceinline__ void q8_store(uint8_t* row, int c, int C, const float
     p = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * q + 2], t[4 * q + 3], p, true);
     w[q] = (unsigned)p;
   }
-  if (c + V <= C) {
+  if (ex || c + V <= C) {
     if constexpr (V == 8) { RmsB8 b; b.x = w[0]; b.y = w[1]; *reinterpret_cast<RmsB8*>(row + c) = b; }
     else { RmsB4 b; b.x = w[0]; *reinterpret_cast<RmsB4*>(row + c) = b; }
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (c + e < C) row[c + e] = (uint8_t)(w[e / 4] >> (8 * (e & 3)));
+  } else if (c < C) {
+    const int n = C & (V - 1);
+    uint8_t* q = row + c;
+    unsigned u = w[0];
+    if (V == 8 && (n & 4)) { RmsB4 b; b.x = w[0]; *reinterpret_cast<RmsB4*>(q) = b; q += 4; u = w[V / 4 - 1]; }
+    if (n & 2) { RmsB2 b; b.x = (unsigned short)u; *reinterpret_cast<RmsB2*>(q) = b; q += 2; u >>= 16; }
+    if (n & 1) *q = (uint8_t)u;
   }
 }
 template <int V>
@@ -138,8 +202,8 @@ struct RmsFwdK {
   void* h; void* y; uint8_t* q; float* scales; int group, ngroups; float* rstd;
 };
 
-// Q: 0 = no 8-bit output, 1 = one scale per row, 2 = one scale per `group` channels (group / V a power of two <= LPR: host)
-template <typename T, int LPR, int NCH, int Q>
+// Q: an 8-bit output too, with one scale per row (group 0) or per `group` channels (group / V a power of two <= LPR: host)
+template <typename T, int LPR, int NCH, bool Q, bool EX>
 __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdK p) {
   constexpr int V = RmsV<T>::N;
   const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
@@ -148,13 +212,13 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdK p) {
   const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
   float h[NCH][V];
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) rms_load(x, (i * LPR + ln) * V, p.C, h[i]);
+  for (int i = 0; i < NCH; ++i) rms_load(EX || i < NCH - 1, x, (i * LPR + ln) * V, p.C, h[i]);
   if (p.res) {
     const T* r = reinterpret_cast<const T*>(p.res) + row * p.ldr;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       float t[V];
-      rms_load(r, (i * LPR + ln) * V, p.C, t);
+      rms_load(EX || i < NCH - 1, r, (i * LPR + ln) * V, p.C, t);
 #pragma unroll
       for (int e = 0; e < V; ++e) h[i][e] = rms_round(h[i][e] + t[e], x);
     }
@@ -168,25 +232,25 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdK p) {
   const float s = 1.f / sqrtf(ss / (float)p.C + p.eps);
   if (p.h) {
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) rms_store(reinterpret_cast<T*>(p.h) + row * p.C, (i * LPR + ln) * V, p.C, h[i]);
+    for (int i = 0; i < NCH; ++i) rms_store(EX || i < NCH - 1, reinterpret_cast<T*>(p.h) + row * p.C, (i * LPR + ln) * V, p.C, h[i]);
   }
   if (p.rstd && ln == 0) p.rstd[row] = s;
   float g[NCH][V];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    rms_gain<V>(p.gamma, (i * LPR + ln) * V, p.C, g[i]);
+    rms_gain<V>(EX || i < NCH - 1, p.gamma, (i * LPR + ln) * V, p.C, g[i]);
     if (p.y) {
       float y[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) y[e] = h[i][e] * s * g[i][e];
-      rms_store(reinterpret_cast<T*>(p.y) + row * p.ldy, (i * LPR + ln) * V, p.C, y);
+      rms_store(EX || i < NCH - 1, reinterpret_cast<T*>(p.y) + row * p.ldy, (i * LPR + ln) * V, p.C, y);
     }
   }
-  if constexpr (Q != 0) {
+  if constexpr (Q) {
     double am[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) am[i] = abs_max<V>(h[i], g[i]);
-    if constexpr (Q == 1) {
+    if (p.group == 0) {
 #pragma unroll
       for (int i = 1; i < NCH; ++i) am[0] = fmax(am[0], am[i]);
 #pragma unroll
@@ -194,7 +258,7 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdK p) {
       const Q8 k(am[0], s);
       if (ln == 0) p.scales[row] = k.scale;
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) q8_store<V>(p.q + row * p.C, (i * LPR + ln) * V, p.C, h[i], g[i], k);
+      for (int i = 0; i < NCH; ++i) q8_store<V>(EX || i < NCH - 1, p.q + row * p.C, (i * LPR + ln) * V, p.C, h[i], g[i], k);
     } else {
       const int gl = p.group / V;                       // lanes of a group
       for (int o = gl >> 1; o > 0; o >>= 1)
@@ -205,7 +269,7 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdK p) {
         const int c = (i * LPR + ln) * V;
         const Q8 k(am[i], s);
         if ((ln & (gl - 1)) == 0 && c < p.C) p.scales[row * p.ngroups + c / p.group] = k.scale;
-        q8_store<V>(p.q + row * p.C, c, p.C, h[i], g[i], k);
+        q8_store<V>(EX || i < NCH - 1, p.q + row * p.C, c, p.C, h[i], g[i], k);
       }
     }
   }
@@ -229,15 +293,15 @@ __device__ __forceinline__ double block_max_d(double v, double* red) {
 }
 template <typename T>
 __device__ __forceinline__ void rms_sum_chunk(const T* x, const T* r, int c, int C, float (&h)[RmsV<T>::N]) {
-  rms_load(x, c, C, h);
+  rms_load(false, x, c, C, h);
   if (r) {
     float t[RmsV<T>::N];
-    rms_load(r, c, C, t);
+    rms_load(false, r, c, C, t);
 #pragma unroll
     for (int e = 0; e < RmsV<T>::N; ++e) h[e] = rms_round(h[e] + t[e], x);
   }
 }
-template <typename T, int Q>
+template <typename T, bool Q>
 __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwdK p) {
   constexpr int V = RmsV<T>::N;
   __shared__ double red[4];
@@ -259,15 +323,15 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwdK p) {
   for (long c = (long)threadIdx.x * V; c < p.C; c += 256 * V) {
     float h[V], g[V];
     rms_sum_chunk(x, r, (int)c, p.C, h);
-    if (p.h) rms_store(reinterpret_cast<T*>(p.h) + row * p.C, (int)c, p.C, h);
-    rms_gain<V>(p.gamma, (int)c, p.C, g);
-    if constexpr (Q == 1) am = fmax(am, abs_max<V>(h, g));
+    if (p.h) rms_store(false, reinterpret_cast<T*>(p.h) + row * p.C, (int)c, p.C, h);
+    rms_gain<V>(false, p.gamma, (int)c, p.C, g);
+    if (Q && p.group == 0) am = fmax(am, abs_max<V>(h, g));
 #pragma unroll
     for (int e = 0; e < V; ++e) h[e] = h[e] * s * g[e];
-    if (p.y) rms_store(reinterpret_cast<T*>(p.y) + row * p.ldy, (int)c, p.C, h);
+    if (p.y) rms_store(false, reinterpret_cast<T*>(p.y) + row * p.ldy, (int)c, p.C, h);
   }
-  if constexpr (Q != 0) {
-    if constexpr (Q == 1) {
+  if constexpr (Q) {
+    if (Q && p.group == 0) {
       am = block_max_d(am, red);
       if (threadIdx.x == 0) p.scales[row] = Q8(am, s).scale;
     }
@@ -278,14 +342,14 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwdK p) {
       const int c = cl < p.C ? (int)cl : p.C;
       float h[V], g[V];
       rms_sum_chunk(x, r, c, p.C, h);
-      rms_gain<V>(p.gamma, c, p.C, g);
-      if constexpr (Q == 2) {
+      rms_gain<V>(false, p.gamma, c, p.C, g);
+      if (p.group) {
         am = abs_max<V>(h, g);
         const int gl = p.group / V;
         for (int o = gl >> 1; o > 0; o >>= 1) am = fmax(am, __shfl_xor(am, o, 64));
         if ((threadIdx.x & (gl - 1)) == 0 && c < p.C) p.scales[row * p.ngroups + c / p.group] = Q8(am, s).scale;
       }
-      if (c < p.C) q8_store<V>(p.q + row * p.C, c, p.C, h, g, Q8(am, s));
+      if (c < p.C) q8_store<V>(false, p.q + row * p.C, c, p.C, h, g, Q8(am, s));
     }
   }
 }
@@ -299,7 +363,7 @@ struct RmsBwdK {
 // A group of LPR lanes walks rows; every lane keeps the dgamma sums of its own columns in registers, the workgroup's groups are
 // joined in LDS, the workgroups by rms_dgamma_kernel (one workgroup: written here).  No atomics: the order is fixed.  WG: 256 lanes, or 1024
 // for the few rows that one workgroup handles by itself (a second launch costs more than the rows).
-template <typename T, int LPR, int NCH, int WG>
+template <typename T, int LPR, int NCH, int WG, bool EX>
 __global__ __launch_bounds__(WG) void rms_bwd_kernel(const RmsBwdK p) {
   constexpr int V = RmsV<T>::N, G = WG / LPR;
   __shared__ float red[WG * NCH * V];
@@ -307,7 +371,7 @@ __global__ __launch_bounds__(WG) void rms_bwd_kernel(const RmsBwdK p) {
   float acc[NCH][V], gain[NCH][V];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
-    rms_gain<V>(p.gamma, (i * LPR + ln) * V, p.C, gain[i]);
+    rms_gain<V>(EX || i < NCH - 1, p.gamma, (i * LPR + ln) * V, p.C, gain[i]);
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[i][e] = 0.f;
   }
@@ -316,10 +380,10 @@ __global__ __launch_bounds__(WG) void rms_bwd_kernel(const RmsBwdK p) {
     const T* h = reinterpret_cast<const T*>(p.h) + row * p.C;
     float a[NCH][V], b[NCH][V], d[NCH][V];
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) { rms_load(dy, (i * LPR + ln) * V, p.C, a[i]); rms_load(h, (i * LPR + ln) * V, p.C, b[i]); }
+    for (int i = 0; i < NCH; ++i) { rms_load(EX || i < NCH - 1, dy, (i * LPR + ln) * V, p.C, a[i]); rms_load(EX || i < NCH - 1, h, (i * LPR + ln) * V, p.C, b[i]); }
     if (p.dh) {
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) rms_load(reinterpret_cast<const T*>(p.dh) + row * p.C, (i * LPR + ln) * V, p.C, d[i]);
+      for (int i = 0; i < NCH; ++i) rms_load(EX || i < NCH - 1, reinterpret_cast<const T*>(p.dh) + row * p.C, (i * LPR + ln) * V, p.C, d[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
@@ -342,7 +406,7 @@ __global__ __launch_bounds__(WG) void rms_bwd_kernel(const RmsBwdK p) {
     for (int i = 0; i < NCH; ++i) {
 #pragma unroll
       for (int e = 0; e < V; ++e) a[i][e] = (a[i][e] - b[i][e] * dot) * s + d[i][e];
-      rms_store(reinterpret_cast<T*>(p.dx) + row * p.C, (i * LPR + ln) * V, p.C, a[i]);
+      rms_store(EX || i < NCH - 1, reinterpret_cast<T*>(p.dx) + row * p.C, (i * LPR + ln) * V, p.C, a[i]);
     }
   }
   // red[group][column]
@@ -390,8 +454,8 @@ __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwdK p) {
   double dot = 0.0;
   for (long c = (long)threadIdx.x * V; c < p.C; c += 256 * V) {
     float a[V], b[V], g[V], t = 0.f;
-    rms_load(dy, (int)c, p.C, a); rms_load(h, (int)c, p.C, b);
-    rms_gain<V>(p.gamma, (int)c, p.C, g);
+    rms_load(false, dy, (int)c, p.C, a); rms_load(false, h, (int)c, p.C, b);
+    rms_gain<V>(false, p.gamma, (int)c, p.C, g);
 #pragma unroll
     for (int e = 0; e < V; ++e) t = fmaf(a[e] * g[e], b[e] * s, t);
     dot += (double)t;
@@ -399,16 +463,16 @@ __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwdK p) {
   const float m = (float)(block_sum_d(dot, red) / (double)p.C);
   for (long c = (long)threadIdx.x * V; c < p.C; c += 256 * V) {
     float a[V], b[V], g[V], d[V];
-    rms_load(dy, (int)c, p.C, a); rms_load(h, (int)c, p.C, b);
-    rms_gain<V>(p.gamma, (int)c, p.C, g);
-    if (dh) rms_load(dh, (int)c, p.C, d);
+    rms_load(false, dy, (int)c, p.C, a); rms_load(false, h, (int)c, p.C, b);
+    rms_gain<V>(false, p.gamma, (int)c, p.C, g);
+    if (dh) rms_load(false, dh, (int)c, p.C, d);
     else {
 #pragma unroll
       for (int e = 0; e < V; ++e) d[e] = 0.f;
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) a[e] = (a[e] * g[e] - b[e] * s * m) * s + d[e];
-    rms_store(reinterpret_cast<T*>(p.dx) + row * p.C, (int)c, p.C, a);
+    rms_store(false, reinterpret_cast<T*>(p.dx) + row * p.C, (int)c, p.C, a);
   }
 }
 // ... and dgamma's partial sums by column strips (256 columns) x row ranges
@@ -424,13 +488,28 @@ __global__ __launch_bounds__(256) void rms_dgamma_long_kernel(const RmsBwdK p) {
   p.part[(long)blockIdx.y * p.C + c] = (float)t;
 }
 
-// lanes and chunks per lane that hold a row of C elements (V per chunk); nch = 0: it takes the long-row form
-static void rms_shape(int C, int V, int group, int& lpr, int& nch) {
-  lpr = 8;
-  while (lpr < 64 && (lpr * V < C || lpr * V < group)) lpr *= 2;
-  nch = 1;
-  while (nch * lpr * V < C) nch *= 2;
-  if (nch * V > 32) nch = 0;
+// lanes and chunks per lane that hold a row of C elements (V per chunk), nch = 0: it takes the long-row form; all chunks of a lane but the
+// last are full.  Rows that fill a power of two of lanes to the last element take one chunk per lane, or several with 64 lanes
+// (`ex`: no masks at all).  Others: few rows, and the bf16 backward pass, which keeps most registers, the fewest chunks; otherwise what
+// fills the lanes of a wave best, several rows to a wave (300 bf16 channels: 172 -> 116 us per 63 M elements).
+// A group of the 8-bit output must lie within one turn of the lanes.
+struct RmsShape { int lpr, nch; bool ex; };
+static RmsShape rms_shape(long rows, int C, int V, int group, bool bwd) {
+  for (int l = 8; l <= 64; l *= 2)
+    if (l * V == C) return {l, 1, true};
+  for (int n = 2; n * V <= 32; ++n)
+    if (64 * V * n == C) return {64, n, true};
+  static const int shapes[][2] = {{8, 1}, {8, 2}, {8, 3}, {16, 1}, {16, 2}, {16, 3}, {32, 1}, {32, 2}, {32, 3}, {64, 1}, {64, 2}, {64, 3}, {64, 4}, {64, 5},
+                                  {64, 6}, {64, 7}, {64, 8}};
+  RmsShape best = {64, 0, false};
+  float cost = 1e30f;
+  for (const auto& q : shapes) {
+    if (q[0] * q[1] * V < C || q[0] * V < group || q[1] * V > 32) continue;
+    if (q[0] * (q[1] - 1) * V >= C) continue;
+    const float c = rows <= 2048 || (bwd && V == 8) ? (float)(q[1] * 64 + q[0]) : ((float)q[1] + 1.f) * (float)q[0];
+    if (c < cost) { cost = c; best = {q[0], q[1], false}; }
+  }
+  return best;
 }
 // at most eight rows per group of a workgroup of 1024 lanes: it writes dgamma itself
 static bool rms_bwd_single(long rows, int lpr, int nch) { return nch == 1 && rows <= 8 * (1024 / lpr); }
@@ -464,10 +543,9 @@ extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamm
              "pg_rms_norm_fwd: a pointer is not aligned to its element");
   if (rows == 0) return 0;
   const int V = io_flags ? 8 : 4;
-  const int grp = q ? group : 0;
-  const int Q = !q ? 0 : (group == 0 ? 1 : 2);
-  int lpr, nch;
-  rms_shape(C, V, grp, lpr, nch);
+  const int grp = q && group < C ? group : 0;          // a group that is the whole row
+  const RmsShape sh = rms_shape((long)rows, C, V, grp, false);
+  const int lpr = sh.lpr, nch = sh.nch;
   const long blocks = nch ? (rows + 256 / lpr - 1) / (256 / lpr) : rows;
   PG_REQUIRE(blocks < (1L << 31), "pg_rms_norm_fwd: too many rows");
   PG_REQUIRE(nch || ((h == nullptr || (h != x && h != res)) && (y == nullptr || (y != x && y != res && y != h))),
@@ -475,36 +553,55 @@ extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamm
   PG_REQUIRE((h == nullptr || ((h != x || ldx == C) && (h != res || ldr == C))) &&
              (y == nullptr || ((y != x || ldy == ldx) && (y != res || ldy == ldr) && (y != h || ldy == C))),
              "pg_rms_norm_fwd: an output in place of an input needs the same row stride");
-  RmsFwdK k = {x, res, gamma, (long)rows, C, (long)ldx, (long)ldr, (long)ldy, eps, h, y, (uint8_t*)q, scales, group,
-               group ? (C + group - 1) / group : 1, rstd};
+  RmsFwdK k = {x, res, gamma, (long)rows, C, (long)ldx, (long)ldr, (long)ldy, eps, h, y, (uint8_t*)q, scales, grp,
+               grp ? (C + grp - 1) / grp : 1, rstd};
   hipStream_t st = (hipStream_t)stream;
-#define PG_RF1(T, L, N)                                                                                            \
+  const dim3 grid((unsigned)blocks), wg(256);
+#define PG_RF1(T, L, N, EX)                                                                                        \
   do {                                                                                                             \
-    if (Q == 0) PG_KLAUNCH((rms_fwd_kernel<T, L, N, 0>), dim3((unsigned)blocks), dim3(256), 0, st, k);             \
-    else if (Q == 1) PG_KLAUNCH((rms_fwd_kernel<T, L, N, 1>), dim3((unsigned)blocks), dim3(256), 0, st, k);        \
-    else PG_KLAUNCH((rms_fwd_kernel<T, L, N, 2>), dim3((unsigned)blocks), dim3(256), 0, st, k);                    \
-  } while (0)
-#define PG_RFL(T)                                                                                                  \
-  do {                                                                                                             \
-    if (Q == 0) PG_KLAUNCH((rms_fwd_long_kernel<T, 0>), dim3((unsigned)blocks), dim3(256), 0, st, k);              \
-    else if (Q == 1) PG_KLAUNCH((rms_fwd_long_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, st, k);         \
-    else PG_KLAUNCH((rms_fwd_long_kernel<T, 2>), dim3((unsigned)blocks), dim3(256), 0, st, k);                     \
+    if (q) PG_KLAUNCH((rms_fwd_kernel<T, L, N, true, EX>), grid, wg, 0, st, k);                                    \
+    else PG_KLAUNCH((rms_fwd_kernel<T, L, N, false, EX>), grid, wg, 0, st, k);                                     \
   } while (0)
 #define PG_RF(T)                                                                                                   \
   do {                                                                                                             \
-    if (nch == 0) PG_RFL(T);                                                                                       \
-    else if (lpr == 8) PG_RF1(T, 8, 1);                                                                            \
-    else if (lpr == 16) PG_RF1(T, 16, 1);                                                                          \
-    else if (lpr == 32) PG_RF1(T, 32, 1);                                                                          \
-    else if (nch == 1) PG_RF1(T, 64, 1);                                                                           \
-    else if (nch == 2) PG_RF1(T, 64, 2);                                                                           \
-    else if (nch == 4) PG_RF1(T, 64, 4);                                                                           \
-    else PG_RF1(T, 64, 32 / RmsV<T>::N);                                                                           \
+    switch (lpr * 32 + nch * 2 + (sh.ex ? 1 : 0)) {                                                                \
+      case 8 * 32 + 3: PG_RF1(T, 8, 1, true); break;                                                               \
+      case 16 * 32 + 3: PG_RF1(T, 16, 1, true); break;                                                             \
+      case 32 * 32 + 3: PG_RF1(T, 32, 1, true); break;                                                             \
+      case 64 * 32 + 3: PG_RF1(T, 64, 1, true); break;                                                             \
+      case 64 * 32 + 5: PG_RF1(T, 64, 2, true); break;                                                             \
+      case 64 * 32 + 7: PG_RF1(T, 64, 3, true); break;                                                             \
+      case 64 * 32 + 9: PG_RF1(T, 64, 4, true); break;                                                             \
+      case 64 * 32 + 11: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 5 : 4), true); break;                                    \
+      case 64 * 32 + 13: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 6 : 4), true); break;                                    \
+      case 64 * 32 + 15: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 7 : 4), true); break;                                    \
+      case 64 * 32 + 17: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 8 : 4), true); break;                                    \
+      case 8 * 32 + 2: PG_RF1(T, 8, 1, false); break;                                                              \
+      case 8 * 32 + 4: PG_RF1(T, 8, 2, false); break;                                                              \
+      case 8 * 32 + 6: PG_RF1(T, 8, 3, false); break;                                                              \
+      case 16 * 32 + 2: PG_RF1(T, 16, 1, false); break;                                                            \
+      case 16 * 32 + 4: PG_RF1(T, 16, 2, false); break;                                                            \
+      case 16 * 32 + 6: PG_RF1(T, 16, 3, false); break;                                                            \
+      case 32 * 32 + 2: PG_RF1(T, 32, 1, false); break;                                                            \
+      case 32 * 32 + 4: PG_RF1(T, 32, 2, false); break;                                                            \
+      case 32 * 32 + 6: PG_RF1(T, 32, 3, false); break;                                                            \
+      case 64 * 32 + 2: PG_RF1(T, 64, 1, false); break;                                                            \
+      case 64 * 32 + 4: PG_RF1(T, 64, 2, false); break;                                                            \
+      case 64 * 32 + 6: PG_RF1(T, 64, 3, false); break;                                                            \
+      case 64 * 32 + 8: PG_RF1(T, 64, 4, false); break;                                                            \
+      case 64 * 32 + 10: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 5 : 4), false); break;                                   \
+      case 64 * 32 + 12: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 6 : 4), false); break;                                   \
+      case 64 * 32 + 14: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 7 : 4), false); break;                                   \
+      case 64 * 32 + 16: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 8 : 4), false); break;                                   \
+      default:                                                                                                     \
+        if (q) PG_KLAUNCH((rms_fwd_long_kernel<T, true>), grid, wg, 0, st, k);                                     \
+        else PG_KLAUNCH((rms_fwd_long_kernel<T, false>), grid, wg, 0, st, k);                                      \
+        break;                                                                                                     \
+    }                                                                                                              \
   } while (0)
   if (io_flags == 0) PG_RF(float);
   else PG_RF(bf16_t);
 #undef PG_RF
-#undef PG_RFL
 #undef PG_RF1
   PG_LAUNCH_OK("pg_rms_norm_fwd");
   return 0;
@@ -512,8 +609,8 @@ extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamm
 
 extern "C" int64_t pg_rms_norm_bwd_workspace(int64_t rows, int32_t C, int32_t io_flags) {
   if (rows <= 0 || C <= 0) return 0;
-  int lpr, nch;
-  rms_shape(C, io_flags ? 8 : 4, 0, lpr, nch);
+  const RmsShape sh = rms_shape((long)rows, C, io_flags ? 8 : 4, 0, true);
+  const int lpr = sh.lpr, nch = sh.nch;
   const long nb = nch ? rms_bwd_blocks(rows, lpr, nch) : rms_long_slices(rows);
   return nch && nb == 1 ? 0 : (int64_t)nb * C * 4;
 }
@@ -536,33 +633,56 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
     PG_LAUNCH_OK("pg_rms_norm_bwd");
     return 0;
   }
-  int lpr, nch;
-  rms_shape(C, io_flags ? 8 : 4, 0, lpr, nch);
+  const RmsShape sh = rms_shape((long)rows, C, io_flags ? 8 : 4, 0, true);
+  const int lpr = sh.lpr, nch = sh.nch;
   const long nb = nch ? rms_bwd_blocks(rows, lpr, nch) : rms_long_slices(rows);
   PG_REQUIRE(nch || rows < (1L << 31), "pg_rms_norm_bwd: too many rows");
   PG_REQUIRE(nch || (dx != dy && dx != dh && dx != h), "pg_rms_norm_bwd: rows of more than 2048 channels are read twice: dx must not be an input");
   PG_REQUIRE(dx != dy || lddy == C, "pg_rms_norm_bwd: dx in place of dy needs lddy == C");
   RmsBwdK k = {dy, dh, h, rstd, gamma, (long)rows, C, (long)lddy, dx, (float*)workspace, dgamma, accumulate};
   const bool single = rms_bwd_single(rows, lpr, nch);
-#define PG_RBN(T, L, N) PG_KLAUNCH((rms_bwd_kernel<T, L, N, 256>), dim3((unsigned)nb), dim3(256), 0, st, k)
-#define PG_RB1(T, L)                                                                                               \
+#define PG_RBN(T, L, N, EX) PG_KLAUNCH((rms_bwd_kernel<T, L, N, 256, EX>), dim3((unsigned)nb), dim3(256), 0, st, k)
+#define PG_RB1(T, L, EX)                                                                                           \
   do {                                                                                                             \
-    if (single) PG_KLAUNCH((rms_bwd_kernel<T, L, 1, 1024>), dim3(1), dim3(1024), 0, st, k);                        \
-    else PG_RBN(T, L, 1);                                                                                          \
+    if (single) PG_KLAUNCH((rms_bwd_kernel<T, L, 1, 1024, EX>), dim3(1), dim3(1024), 0, st, k);                    \
+    else PG_RBN(T, L, 1, EX);                                                                                      \
   } while (0)
 #define PG_RB(T)                                                                                                   \
   do {                                                                                                             \
-    if (nch == 0) {                                                                                                \
-      PG_KLAUNCH((rms_bwd_long_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, k);                             \
-      PG_KLAUNCH((rms_dgamma_long_kernel<T>), dim3((C + 255) / 256, (unsigned)nb), dim3(256), 0, st, k);           \
+    switch (lpr * 32 + nch * 2 + (sh.ex ? 1 : 0)) {                                                                \
+      case 8 * 32 + 3: PG_RB1(T, 8, true); break;                                                                  \
+      case 16 * 32 + 3: PG_RB1(T, 16, true); break;                                                                \
+      case 32 * 32 + 3: PG_RB1(T, 32, true); break;                                                                \
+      case 64 * 32 + 3: PG_RB1(T, 64, true); break;                                                                \
+      case 64 * 32 + 5: PG_RBN(T, 64, 2, true); break;                                                             \
+      case 64 * 32 + 7: PG_RBN(T, 64, 3, true); break;                                                             \
+      case 64 * 32 + 9: PG_RBN(T, 64, 4, true); break;                                                             \
+      case 64 * 32 + 11: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 5 : 4), true); break;                                    \
+      case 64 * 32 + 13: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 6 : 4), true); break;                                    \
+      case 64 * 32 + 15: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 7 : 4), true); break;                                    \
+      case 64 * 32 + 17: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 8 : 4), true); break;                                    \
+      case 8 * 32 + 2: PG_RB1(T, 8, false); break;                                                                 \
+      case 8 * 32 + 4: PG_RBN(T, 8, (RmsV<T>::N == 4 ? 2 : 1), false); break;                                      \
+      case 8 * 32 + 6: PG_RBN(T, 8, (RmsV<T>::N == 4 ? 3 : 1), false); break;                                      \
+      case 16 * 32 + 2: PG_RB1(T, 16, false); break;                                                               \
+      case 16 * 32 + 4: PG_RBN(T, 16, (RmsV<T>::N == 4 ? 2 : 1), false); break;                                    \
+      case 16 * 32 + 6: PG_RBN(T, 16, (RmsV<T>::N == 4 ? 3 : 1), false); break;                                    \
+      case 32 * 32 + 2: PG_RB1(T, 32, false); break;                                                               \
+      case 32 * 32 + 4: PG_RBN(T, 32, (RmsV<T>::N == 4 ? 2 : 1), false); break;                                    \
+      case 32 * 32 + 6: PG_RBN(T, 32, (RmsV<T>::N == 4 ? 3 : 1), false); break;                                    \
+      case 64 * 32 + 2: PG_RB1(T, 64, false); break;                                                               \
+      case 64 * 32 + 4: PG_RBN(T, 64, 2, false); break;                                                            \
+      case 64 * 32 + 6: PG_RBN(T, 64, 3, false); break;                                                            \
+      case 64 * 32 + 8: PG_RBN(T, 64, 4, false); break;                                                            \
+      case 64 * 32 + 10: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 5 : 4), false); break;                                   \
+      case 64 * 32 + 12: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 6 : 4), false); break;                                   \
+      case 64 * 32 + 14: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 7 : 4), false); break;                                   \
+      case 64 * 32 + 16: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 8 : 4), false); break;                                   \
+      default:                                                                                                     \
+        PG_KLAUNCH((rms_bwd_long_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, k);                           \
+        PG_KLAUNCH((rms_dgamma_long_kernel<T>), dim3((C + 255) / 256, (unsigned)nb), dim3(256), 0, st, k);         \
+        break;                                                                                                     \
     }                                                                                                              \
-    else if (lpr == 8) PG_RB1(T, 8);                                                                               \
-    else if (lpr == 16) PG_RB1(T, 16);                                                                             \
-    else if (lpr == 32) PG_RB1(T, 32);                                                                             \
-    else if (nch == 1) PG_RB1(T, 64);                                                                              \
-    else if (nch == 2) PG_RBN(T, 64, 2);                                                                           \
-    else if (nch == 4) PG_RBN(T, 64, 4);                                                                           \
-    else PG_RBN(T, 64, 32 / RmsV<T>::N);                                                                           \
   } while (0)
   if (io_flags == 0) PG_RB(float);
   else PG_RB(bf16_t);
