@@ -15,6 +15,7 @@ import torch.nn as nn
 
 from ..runtime import engine as E
 from ..runtime import lib as L
+from ..runtime import ops as OPS
 from ..utils import synth
 
 
@@ -267,3 +268,40 @@ class Discriminator(_ArenaModule):
 
     def forward(self, x):
         return _DiscFn.apply(x, self, self._anchor)
+
+
+class _RMSNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        c = x.shape[-1]
+        y, h, rstd = OPS.rms_norm(x.reshape(-1, c), weight, None if residual is None else residual.reshape(-1, c), eps=eps)
+        h = h.contiguous()
+        ctx.save_for_backward(h, rstd, weight)
+        ctx.has_res = residual is not None
+        ctx.set_materialize_grads(False)
+        return (y.view(x.shape), h.view(x.shape)) if ctx.has_res else y.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, gy, gh=None):
+        h, rstd, weight = ctx.saved_tensors
+        if gy is None:
+            return gh, None, gh, None
+        shape = gy.shape
+        dh = None if gh is None else gh.reshape(h.shape).contiguous()
+        dx, dw = OPS.rms_norm_bwd(gy.reshape(h.shape), h, rstd, weight, dh=dh)
+        dx = dx.view(shape)
+        return dx, dw, dx if ctx.has_res else None, None
+
+
+class RMSNorm(nn.Module):
+    """Root-mean-square norm along the last dimension (the channels of pixel-major activations [N][H][W][C]) with a gain per
+    channel, next to the per-sample norm of the reference's blocks (networks.py:159,166-169).  forward(x) -> y;
+    forward(x, residual) -> (y, x + residual): a pre-norm residual block hands the sum on.  fp32 or bf16."""
+
+    def __init__(self, channels, eps=1e-6, device="cuda"):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(channels, dtype=torch.float32, device=device))
+
+    def forward(self, x, residual=None):
+        return _RMSNormFn.apply(x, self.weight, residual, self.eps)

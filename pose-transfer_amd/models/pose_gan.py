@@ -47,6 +47,31 @@ class FusedAdam:
         return {"step": a.step, "exp_avg": a.m.clone(), "exp_avg_sq": a.v.clone()}
 
 
+class FusedMuon(FusedAdam):
+    """Muon for the filters of the inner blocks — the momentum's orthogonal factor (Newton-Schulz products) in place of Adam's
+    elementwise scaling — and FusedAdam's update for every other tensor, as one library call over the arena (`--optimizer muon`;
+    the reference trains with Adam, pose_gan.py:50-51)."""
+
+    def __init__(self, module, lr, betas=(0.5, 0.999), eps=1e-8, momentum=0.95, weight_decay=0.0):
+        super().__init__(module, lr, betas, eps)
+        self.momentum, self.weight_decay = momentum, weight_decay
+
+    def step(self, grad_scale=1.0, grads_bf16=None):
+        self.module.arena.muon_step(self.lr, self.momentum, self.weight_decay, self.betas[0], self.betas[1], self.eps, grad_scale,
+                                    grads_bf16)
+
+
+def make_optimizer(module, opt):
+    """the optimiser `opt.optimizer` names (default: the reference's Adam)"""
+    kind = getattr(opt, "optimizer", "adam")
+    if kind == "adam":
+        return FusedAdam(module, opt.learning_rate)
+    if kind == "muon":
+        return FusedMuon(module, opt.learning_rate, momentum=getattr(opt, "muon_momentum", 0.95),
+                         weight_decay=getattr(opt, "muon_weight_decay", 0.0))
+    raise Exception("Invalid optimizer")
+
+
 class DeformablePose_GAN(nn.Module):
     def __init__(self, opt, device="cuda", init_seed=0):
         super().__init__()
@@ -95,9 +120,8 @@ class DeformablePose_GAN(nn.Module):
         pre = getattr(opt, "generator_checkpoint", None)
         if pre:
             self.gen.load_state_dict(torch.load(pre, map_location="cpu"))
-        lr = opt.learning_rate
-        self.disc_opt = FusedAdam(self.disc, lr)
-        self.gen_opt = FusedAdam(self._core, lr)
+        self.disc_opt = make_optimizer(self.disc, opt)
+        self.gen_opt = make_optimizer(self._core, opt)
         self.content_loss_layer = opt.content_loss_layer
         self.nn_loss_area_size = opt.nn_loss_area_size
         self.vgg_w = self.vgg_b = None
@@ -279,7 +303,7 @@ class DeformablePose_GAN(nn.Module):
             self.g_reducer.begin()
         # single process, one stage: the optimiser step runs in ranges UNDER the backward pass (engine.EagerAdam)
         eager = None
-        if (self.g_reducer is None and len(engs) == 1 and E.EAGER_ADAM and E.REPLAY_CTR is None and E.SIDE_STREAM
+        if (type(self.gen_opt) is FusedAdam and self.g_reducer is None and len(engs) == 1 and E.EAGER_ADAM and E.REPLAY_CTR is None and E.SIDE_STREAM
                 and hasattr(engs[0], "param_release_cb") and input.is_cuda):
             if getattr(self, "_eager_g", None) is None:
                 self._eager_g = E.EagerAdam(self._core.arena, self.gen_opt.lr, self.gen_opt.betas[0], self.gen_opt.betas[1],

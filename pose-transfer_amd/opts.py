@@ -1,7 +1,7 @@
 """Command-line options with the reference's flag names (reference src_deformable/opts.py:14-97).
 Only flags the hot path reads are acted upon; path/dir side effects of the reference's parse() are limited to
 the experiment directories.  New flags: --synthetic, --align_corners, --vgg_weights, --steps, --lazy_losses,
---synthetic_ring, --timing_skip."""
+--synthetic_ring, --timing_skip, --optimizer, --muon_momentum, --muon_weight_decay."""
 import argparse
 import os
 
@@ -73,6 +73,10 @@ class opts():
         p.add_argument("--save_samples", default=0, type=int, help="write train / test image grids every display_ratio iterations")
         p.add_argument("--save_at_end", default=0, type=int, help="write a checkpoint when --steps stops the run")
         p.add_argument("--deterministic_test", default=0, type=int, help="test.py: gen.eval() (no Dropout2d) before generating")
+        p.add_argument("--optimizer", default="adam", choices=["adam", "muon"],
+                       help="adam = the reference's; muon = orthogonalised momentum for the inner blocks' filters, Adam for the rest")
+        p.add_argument("--muon_momentum", default=0.95, type=float)
+        p.add_argument("--muon_weight_decay", default=0.0, type=float, help="decoupled decay of the filters that muon updates")
         p.add_argument("--precision", default="f32", choices=["f32", "bf16x3", "bf16", "bf16_data"],
                        help="contraction operand format: f32 = the reference's arithmetic (default); bf16_data = bf16 data path "
                             "(fp32 master weights / accumulation; stated bf16 tolerance, DESIGN.md)")

@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from . import lib as L
+from . import ops as OPS
 from ..utils import synth
 
 T_WARPS = 10
@@ -146,6 +147,7 @@ class ParamArena:
         self.params_bf16 = None       # bf16 data path: bf16 copy of the whole arena, kept current by Adam / load_state_dict
         self.bf16_version = -1
         self.params_bf16_t, self.bf16_t_version = None, -1      # ... and the per-tap transposed copy (bf16_params_t)
+        self._muon_table = self._muon_ws = None                 # muon_step's records and workspace, made at its first call
         ARENAS[self.params.untyped_storage().data_ptr()] = self
 
     def p(self, key):
@@ -283,6 +285,52 @@ class ParamArena:
         L.call("pg_adam_ex", L.ptr(self.params), L.ptr(self.grads), L.ptr(grads_bf16), L.ptr(self.m), L.ptr(self.v),
                self.total, b1, b2, eps, lr / bc1, math.sqrt(bc2), grad_scale, L.ptr(self.params_bf16) if want_bf16 else None,
                L.stream())
+        if want_bf16:
+            self.bf16_version = self.version()
+
+
+    def is_matrix(self, key):
+        """whether the Muon step treats a tensor as a matrix: the filters of the inner blocks with more than one output channel.
+        First and last layers, biases and norm parameters stay with Adam."""
+        ps = self.pshape[key]
+        return key.endswith(".net.1.weight") and len(ps) == 4 and ps[2] > 1
+
+    def muon_table(self):
+        """one ops.MUON_ENTRY per matrix ([Cout, taps * Cin], as packed), one per run of other tensors (their padding is zero and
+        stays zero under Adam).  Update scale 0.2 sqrt(max(rows, columns)): an rms of 0.2, so that Adam's learning rate serves both."""
+        if self._muon_table is None:
+            rec = []
+            for i, k in enumerate(self.keys):
+                end = self.off[self.keys[i + 1]] if i + 1 < len(self.keys) else self.total
+                if self.is_matrix(k):
+                    kh, kw, co, ci = self.pshape[k]
+                    rec.append((self.off[k], kh * kw, co, ci, 0, 0.2 * math.sqrt(max(co, kh * kw * ci)), 0))
+                elif rec and rec[-1][4] == 1 and rec[-1][0] + rec[-1][3] == self.off[k] and end - rec[-1][0] < 1 << 30:
+                    rec[-1] = (rec[-1][0], 1, 1, end - rec[-1][0], 1, 0.0, 0)
+                else:
+                    rec.append((self.off[k], 1, 1, end - self.off[k], 1, 0.0, 0))
+            self._muon_table = np.array(rec, dtype=OPS.MUON_ENTRY)
+        return self._muon_table
+
+    def muon_step(self, lr, momentum=0.95, weight_decay=0.0, b1=0.5, b2=0.999, eps=1e-8, grad_scale=1.0, grads_bf16=None):
+        """The step of models/pose_gan.py FusedMuon: Muon for the matrices, Adam for the other tensors, one call.  grads_bf16 and the
+        replay-safe step number as in adam_step; `m` holds both kinds' first moments."""
+        self.step += 1
+        self._bump_version()
+        step = self.step
+        if REPLAY_CTR is not None:
+            if getattr(self, "replay_base", None) is None:
+                self.replay_base = self.step
+            step = self.replay_base
+        table = self.muon_table()
+        if self._muon_ws is None:       # persistent: recorded launches (runtime/tape.py) keep its address
+            self._muon_ws = torch.empty(OPS.muon_workspace(table), dtype=torch.uint8, device=self.params.device)
+        want_bf16 = PRECISION == 3 and self.params.is_cuda
+        if want_bf16 and self.params_bf16 is None:
+            self.params_bf16 = torch.empty(self.total, dtype=torch.bfloat16, device=self.params.device)
+        OPS.muon_step(self.params, self.grads if grads_bf16 is None else grads_bf16, self.m, self.v, table, lr, momentum=momentum,
+                      weight_decay=weight_decay, betas=(float(b1), float(b2)), eps=eps, step=step, grad_scale=grad_scale, ctr=REPLAY_CTR,
+                      p_bf16=self.params_bf16 if want_bf16 else None, workspace=self._muon_ws)
         if want_bf16:
             self.bf16_version = self.version()
 

@@ -362,3 +362,139 @@ def test_operators_in_a_captured_graph():
         torch.cuda.synchronize()
         assert torch.equal(dx, want[k][0]) and torch.equal(o, want[k][1]) and torch.equal(s[0], want[k][2]), k
         assert bool(torch.isfinite(junk).all())
+
+
+# ------------------------------------------------------------------------------------------------ module and trainer
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rms_norm_module(dtype):
+    from pose_transfer_amd.models.networks import RMSNorm
+    mod = RMSNorm(48)
+    with torch.no_grad():
+        mod.weight.copy_(rnd(70, 48) + 1.0)
+    x, r = rnd(71, 2, 5, 3, 48, dtype=dtype).requires_grad_(), rnd(72, 2, 5, 3, 48, dtype=dtype).requires_grad_()
+    wy, wh = rnd(73, 2, 5, 3, 48, dtype=dtype), rnd(74, 2, 5, 3, 48, dtype=dtype)
+    y, h = mod(x, r)
+    ((y * wy).sum() + (h * wh).sum()).backward()
+    xd, rd = x.detach().double().requires_grad_(), r.detach().double().requires_grad_()
+    gd = mod.weight.detach().double().requires_grad_()
+    hd = xd + rd
+    hd = hd + (h.detach().double() - hd).detach()             # the stored sum; its gradient is the sum's
+    yd = hd / torch.sqrt((hd * hd).mean(-1, keepdim=True) + 1e-6) * gd
+    ((yd * wy.double()).sum() + (hd * wh.double()).sum()).backward()
+    # dx: a rounding of its own size, and terms of size |w| + |xh| mean|w xh| <= 60 in 64 u
+    assert bool(((x.grad.double() - xd.grad).abs() <= EPS[dtype] * 1.01 * xd.grad.abs() + 64 * U * 60).all())
+    assert torch.equal(x.grad, r.grad)
+    assert bool(((mod.weight.grad.double() - gd.grad).abs() <= 94 * U * (wy.double() * yd.detach() / gd.detach()).abs().sum((0, 1, 2))).all())
+    y = mod(x.detach().requires_grad_())
+    assert y.shape == x.shape and y.grad_fn is not None
+    (only_h,) = torch.autograd.grad(mod(x, r)[1].sum(), x)
+    assert torch.equal(only_h, torch.ones_like(x))
+
+
+def trainer(optimizer, precision=0, n=2, size=64):
+    from types import SimpleNamespace
+    from pose_transfer_amd.models.pose_gan import DeformablePose_GAN
+    from pose_transfer_amd.runtime import engine as E
+    from pose_transfer_amd.utils import synth
+    E.PRECISION = precision
+    opt = SimpleNamespace(image_size=(size, size), use_input_pose=True, pose_dim=18, batch_size=n, num_stacks=4, gen_type="baseline",
+                          dataset="fasion", warp_skip="mask", learning_rate=2e-4, content_loss_layer="none", nn_loss_area_size=1,
+                          gan_penalty_weight=1.0, l1_penalty_weight=100.0, optimizer=optimizer, muon_momentum=0.9, muon_weight_decay=0.01)
+    model = DeformablePose_GAN(opt, device="cuda:0")
+    b = [torch.from_numpy(np.ascontiguousarray(a)).cuda() for a in synth.batch(1, "muon/A", n, 18, size, size)]
+    return model, vars(opt), b
+
+
+def test_trainer_with_muon_against_the_definition():
+    """one dis_update and one gen_update: the arenas after each step against the 64-bit step on the arena's own gradients"""
+    model, od, b = trainer("muon")
+    for arena, run in ((model.disc.arena, lambda: model.dis_update(b[0], b[1], {"warps": b[2], "masks": b[3]}, b[0], b[1], od)),
+                       (model.gen.arena, lambda: model.gen_update(b[0], b[1], {"warps": b[2], "masks": b[3]}, od))):
+        for step in (1, 2):
+            p0, m0, v0 = arena.params.clone(), arena.m.clone(), arena.v.clone()
+            losses = run()
+            assert losses is not None and arena.step == step
+            table = arena.muon_table()
+            assert sum(1 for e in table if e["kind"] == 0) == sum(arena.is_matrix(k) for k in arena.keys) >= 3
+            pr, mr, vr = muon_ref(p0, arena.grads, m0, v0, table, 2e-4, 0.9, True, 0.01, 0.5, 0.999, 1e-8, step)
+            for e in table:
+                at = slice(int(e["off"]), int(e["off"]) + int(e["taps"]) * int(e["rows"]) * int(e["cols"]))
+                a, r = arena.params[at].double() - p0[at].double(), pr[at] - p0[at].double()
+                tol = (1.5 * NS[0] ** 5 * 2.0 ** -20 if e["kind"] == 0 else 0.0) + 64 * U
+                assert float((a - r).norm()) <= tol * float(r.norm()) + 2 * U * float(pr[at].norm()) + 2 * U * float(p0[at].norm())
+            assert bool(((arena.m.double() - mr).abs() <= 4 * U * (m0.double().abs() + arena.grads.double().abs())).all())
+    sd = model.gen.state_dict()
+    assert all(bool(torch.isfinite(v).all()) for v in sd.values())
+
+
+def test_trainer_with_muon_bf16_weights_follow():
+    model, od, b = trainer("muon", precision=3)
+    from pose_transfer_amd.runtime import engine as E
+    try:
+        model.dis_update(b[0], b[1], {"warps": b[2], "masks": b[3]}, b[0], b[1], od)
+        model.gen_update(b[0], b[1], {"warps": b[2], "masks": b[3]}, od)
+        for arena in (model.disc.arena, model.gen.arena):
+            assert arena.bf16_version == arena.version()
+            for k in arena.keys:
+                at = slice(arena.off[k], arena.off[k] + arena.numel[k])
+                assert torch.equal(arena.params_bf16[at], arena.params[at].bfloat16())
+    finally:
+        E.PRECISION = 0
+
+
+def test_trainer_with_muon_replayed_from_a_tape():
+    """recorded launches of the Muon step against the eager loop: same batches, same dropout masks, three iterations"""
+    from pose_transfer_amd.runtime.tape import TapedIteration
+    from pose_transfer_amd.utils import synth
+    runs = []
+    for taped in (False, True):
+        model, od, b = trainer("muon")
+        drop = [m.cuda() for m in (torch.from_numpy(np.ascontiguousarray(a)) for a in synth.dropout_masks(1, "muon/d", 2))]
+        b = [b[0], b[1], b[2].float().contiguous(), b[3]]
+        if taped:
+            t = TapedIteration(model, [b, b, b], dict(od), warmup=1, drop_masks=(drop, drop))     # one eager, one recorded
+            t.replay()
+            t.close()
+        else:
+            for _ in range(3):
+                o = {"warps": b[2], "masks": b[3], "drop_masks": drop}
+                model.dis_update(b[0], b[1], o, b[0], b[1], dict(od, lazy_losses=True))
+                model.gen_update(b[0], b[1], o, dict(od, lazy_losses=True))
+        torch.cuda.synchronize()
+        assert model.gen.arena.step == 3
+        runs.append((model.gen.arena.params.clone(), model.disc.arena.params.clone()))
+    for a, c in zip(*runs):
+        # the trainer's own gradients come from float atomics: equal up to their order, magnified by Adam's and Muon's scaling
+        assert float((a - c).norm() / c.norm()) < 1e-2
+
+
+def test_residual_block_step_uses_all_of_them():
+    """norm with the residual -> product -> its gradients -> Muon step, twice, against 64 bits"""
+    O = ops()
+    rows, C = 192, 64
+    x, r, t = rnd(80, rows, C), rnd(81, rows, C), rnd(82, rows, C)
+    table, total = table_of([(1, C, C), (C,)])
+    gain = slice(int(table[1]["off"]), int(table[1]["off"]) + C)
+    p, m, v = rnd(83, total, scale=0.1), torch.zeros(total, device="cuda"), torch.zeros(total, device="cuda")
+    p[gain] = 1.0
+    pd, md, vd = p.double(), m.double(), v.double()
+    for step in (1, 2):
+        w = p[:C * C].view(C, C)
+        y, h, rstd = O.rms_norm(x, p[gain].contiguous(), r)
+        err = y @ w.t() + h - t
+        g = torch.zeros(total, device="cuda")
+        g[:C * C] = (err.t().contiguous() @ y).reshape(-1)
+        dx, g[gain] = O.rms_norm_bwd(err @ w, h, rstd, p[gain].contiguous(), dh=err)
+        O.muon_step(p, g, m, v, table, lr=1e-2, step=step)
+        # the same in 64 bits with autograd
+        wd, gd, xd = pd[:C * C].view(C, C).clone().requires_grad_(), pd[gain].clone().requires_grad_(), x.double().requires_grad_()
+        hd = xd + r.double()
+        yd = hd / torch.sqrt((hd * hd).mean(1, keepdim=True) + 1e-6) * gd
+        loss = 0.5 * (yd @ wd.t() + hd - t.double()).square().sum()
+        loss.backward()
+        assert float((dx.double() - xd.grad).norm() / xd.grad.norm()) < 1e-5        # fp32 products of 64 terms: about 8 u of the size
+        gr = torch.zeros(total, dtype=torch.float64, device="cuda")
+        gr[:C * C], gr[gain] = wd.grad.reshape(-1), gd.grad
+        pd, md, vd = muon_ref(pd, gr, md, vd, table, 1e-2, 0.95, True, 0.0, 0.5, 0.999, 1e-8, step)
+        for at in (slice(0, C * C), gain):
+            assert float((p[at].double() - pd[at]).norm() / pd[at].norm()) < 1e-4

@@ -122,3 +122,38 @@ def test_wrappers_refuse_on_the_host():
               lambda: O.muon_step(x[0], x[0], x[0], x[0], table(GOOD), lr=0.1), lambda: O.muon_step(x[0], x[0], x[0], x[0], GOOD, lr=0.1)):
         with pytest.raises(ValueError):
             f()
+
+
+def test_muon_table_of_the_networks():
+    """every element of an arena is in exactly one record; the matrices are the inner blocks' filters"""
+    from pose_transfer_amd.runtime import engine as E
+    from pose_transfer_amd.utils import synth
+    enc, dec = synth.nfilters((256, 256))
+    gspec, dspec = synth.generator_spec(18, enc, dec), synth.discriminator_spec(42)
+    for spec, order in ((gspec, E.generator_param_order(gspec, len(enc), len(dec))), (dspec, E.discriminator_param_order(dspec))):
+        arena = E.ParamArena(spec, order, "cpu")
+        t = arena.muon_table()
+        end = 0
+        for e in t:
+            assert end <= e["off"] < end + 64
+            assert bool((arena.params[end:int(e["off"])] == 0).all())
+            end = int(e["off"]) + int(e["taps"]) * int(e["rows"]) * int(e["cols"])
+        assert end <= arena.total < end + 64
+        mats = [k for k in arena.keys if arena.is_matrix(k)]
+        assert len(mats) == sum(int(e["kind"] == 0) for e in t)
+        assert all(k.endswith(".net.1.weight") for k in mats)
+        assert sum(arena.numel[k] for k in mats) > 0.97 * sum(arena.numel.values())
+        assert O.muon_workspace(t) > 8 * sum(arena.numel[k] for k in mats)
+
+
+def test_optimizer_option():
+    from types import SimpleNamespace
+    from pose_transfer_amd.models import pose_gan as G
+    from pose_transfer_amd.opts import opts
+    o = opts().parse(["--optimizer", "muon", "--muon_momentum", "0.9", "--muon_weight_decay", "0.05"])
+    m = G.make_optimizer(None, o)
+    assert type(m) is G.FusedMuon and (m.momentum, m.weight_decay, m.lr, m.betas) == (0.9, 0.05, 2e-4, (0.5, 0.999))
+    assert type(G.make_optimizer(None, opts().parse([]))) is G.FusedAdam
+    assert type(G.make_optimizer(None, SimpleNamespace(learning_rate=1e-3))) is G.FusedAdam
+    with pytest.raises(Exception):
+        G.make_optimizer(None, SimpleNamespace(learning_rate=1e-3, optimizer="sgd"))
