@@ -39,7 +39,7 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int SG = 12, SP = 10;                 // log2 of the scales of G, Q, Q G and of P
 // elements per workgroup of the momentum / square-sum pass: small tensors give few workgroups, large ones many partial sums
 __host__ __device__ constexpr int k0_elems(long n) { return n < (1L << 21) ? 4096 : 16384; }
-constexpr int GT = 128, AI = 128, AJ = 256;      // tiles: Gram; apply (rows, columns)
+constexpr int GT = 128, AI = 128;      // tiles: Gram; apply (rows)
 
 struct NsMat {
   long src, ld, st;             // the caller's storage: element offset, row stride, tap stride
@@ -51,7 +51,7 @@ struct NsMat {
   long x, g, part;              // offsets in the workspace: X planes and chain planes (halves), Gram partials (floats)
   int sq0;                      // first partial sum of squares
 };
-enum { F_MOM, F_SPLIT, F_GRAM, F_JOIN, F_CHAIN, F_APPLY, F_N };       // launches (F_JOIN also: the chain's tiles of 32)
+enum { F_MOM, F_SPLIT, F_GRAM, F_JOIN, F_CHAIN, F_APPLY, F_APPLY2, F_N };       // launches (F_JOIN also: the chain's tiles of 32; apply: 256 or 128 columns)
 struct NsGroup {                // matrices of one call: a device table, or (tab = nullptr) `n` equal ones
   const NsMat* tab;
   const int* first;             // [F_N][n]: the first workgroup of each record
@@ -769,21 +769,42 @@ __device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned 
                : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
 }
 
-// A tile is 128 rows x 256 columns: 4 waves side by side, 128 x 64 each (per K step 12 KB of LDS reads for 24 MFMAs; 64 x 64 would need
-// two thirds more), K steps of 16 through three stages: 72 KB, two workgroups per CU, whose epilogues run under each other's products.
+__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[2][2][2]) {
+  asm volatile(NS_RD "%0, %12\n\t" NS_TR "%4, %13\n\t" NS_TR "%5, %14\n\t" NS_RD "%1, %12 offset:1024\n\t"
+               NS_TR "%6, %13 offset:1024\n\t" NS_TR "%7, %14 offset:1024\n\t" NS_RD "%2, %12 offset:4096\n\t" NS_RD "%3, %12 offset:5120\n\t"
+               NS_TR "%8, %13 offset:4096\n\t" NS_TR "%9, %14 offset:4096\n\t" NS_TR "%10, %13 offset:5120\n\t" NS_TR "%11, %14 offset:5120\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]),
+                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1]),
+                 "=&v"(b[1][0][0]), "=&v"(b[1][0][1]), "=&v"(b[1][1][0]), "=&v"(b[1][1][1])
+               : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
+}
+__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[1][2][2]) {
+  asm volatile(NS_RD "%0, %8\n\t" NS_TR "%4, %9\n\t" NS_TR "%5, %10\n\t" NS_RD "%1, %8 offset:1024\n\t"
+               NS_TR "%6, %9 offset:1024\n\t" NS_TR "%7, %10 offset:1024\n\t" NS_RD "%2, %8 offset:4096\n\t" NS_RD "%3, %8 offset:5120\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]),
+                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1])
+               : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
+}
+
+// WI = 1: a tile is 128 rows x 256 columns, 4 waves side by side, 128 x 64 each (per K step 12 KB of LDS reads for 24 MFMAs; 64 x 64 need
+// a third more per MFMA); K steps of 16 through three stages: 72 KB, two workgroups per CU, whose epilogues run under each other's products.
+// WI = 2 (fewer tiles than that fills the chip with): 128 x 128, waves of 64 x 64.
 __device__ __forceinline__ void muon_update(const NsStep& s, long at, float keep, float step, float o) {
   const float p = s.p[at] * keep - step * o;
   s.p[at] = p;
   if (s.pb) s.pb[at] = (bf16_t)(ns_pack_bf16(p, 0.f) & 0xffffu);
 }
-template <int PX, int OUT>
-__global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int total, const ApplyK k) {
+template <int PX, int OUT, int WI>
+__global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr, int total, const ApplyK k) {
+  constexpr int AJ = 256 / WI, TM = 4 / WI, IPP = AJ / 32;           // IPP: transfers per plane of X
   constexpr int A_BYTES = AI * 2 * 32, B_BYTES = 16 * AJ * 2 * PX, STAGE = A_BYTES + B_BYTES, ST = 3;
   constexpr int PA = A_BYTES / 4096, PB = B_BYTES / 4096, NI = PA + PB;
   __shared__ __attribute__((aligned(1024))) char smem[ST * STAGE];
   const int bt = xcd_tile(blockIdx.x, total, 4);
   if (bt < 0) return;
-  const NsRef r = ns_find<F_APPLY>(gr, bt);
+  const NsRef r = ns_find<WI == 1 ? F_APPLY : F_APPLY2>(gr, bt);
   const NsMat& m = r.m;
   const int ti = (m.Mp + AI - 1) / AI;
   const int i0 = (r.tile % ti) * AI, j0 = (r.tile / ti) * AJ;
@@ -791,10 +812,10 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
   const _Float16* P = k.wsg + m.g + k.pbuf * 2 * pl;
   const _Float16* X = k.wsx + m.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = wave * 64;
-  f32x16 acc[4][2];
+  const int wm = WI == 1 ? 0 : (wave >> 1) * 64, wn = WI == 1 ? wave * 64 : (wave & 1) * 64;
+  f32x16 acc[TM][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -810,7 +831,7 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
   const _Float16* bs[PB];
 #pragma unroll
   for (int q = 0; q < PB; ++q) {
-    const int x = q * 4 + wave, plane = x >> 3, blk = min((j0 >> 4) + (x & 7) * 2 + (lane >> 5), m.Np / 16 - 1);
+    const int x = q * 4 + wave, plane = x / IPP, blk = min((j0 >> 4) + x % IPP * 2 + (lane >> 5), m.Np / 16 - 1);
     const int kr = ((lane >> 1) & 15) ^ ((lane >> 5) << 2);
     bs[q] = X + plane * xpl + ((long)blk * (m.Mp + 8) + kr) * 16 + (lane & 1) * 8;
   }
@@ -823,7 +844,7 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
   };
   const unsigned lds0 = (unsigned)(size_t)smem;
   const int r4 = (lane >> 2) & 3, cq = lane & 3, mb = (lane >> 4) & 1, kh = lane >> 5;
-  const unsigned pa = lds0 + (lane & 31) * 32 + ((kh ^ swz(lane & 31)) << 4);
+  const unsigned pa = lds0 + (wm + (lane & 31)) * 32 + ((kh ^ swz(lane & 31)) << 4);
   const unsigned pb0 = lds0 + A_BYTES + ((wn >> 4) + mb) * 512 + (8 * kh + r4 + 4 * mb) * 32 + cq * 8, pb1 = pb0 ^ 128;
   const int n = m.Mp / 16;
   issue(0);
@@ -835,7 +856,7 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
     wg_barrier();
     if (it + 2 < n) issue(nxt);
     const unsigned so = (unsigned)(cur * STAGE);
-    half8 a[2][4];
+    half8 a[2][TM];
     half4 bq[PX][2][2];
     fetch_apply(pa + so, pb0 + so, pb1 + so, a, bq);
     half8 b[PX][2];
@@ -844,7 +865,7 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
 #pragma unroll
       for (int j = 0; j < 2; ++j) b[p][j] = __builtin_shufflevector(bq[p][j][0], bq[p][j][1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         // the transposed product: a lane holds one row of the result and runs of four of its columns
@@ -860,8 +881,8 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
   if (OUT != 0 && m.tall) {
     // the stored row is the long side: 32 neighbouring lanes hold 32 neighbours of a stored row
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int gi = i0 + i * 32 + (lane & 31);
+    for (int i = 0; i < TM; ++i) {
+      const int gi = i0 + wm + i * 32 + (lane & 31);
       if (gi >= m.M) continue;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
@@ -877,20 +898,24 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
     }
     return;
   }
-  // 32 rows at a time through LDS (rows of 264 floats: both the writes and the reads meet every bank once): a wave then handles whole rows, four
-  // neighbours per lane
+  // 32 rows per row of waves at a time through LDS (rows of AJ + 8 floats: both the writes and the reads meet every bank once): a wave then
+  // handles whole rows, four neighbours per lane
+  constexpr int BS = AJ + 8, RP = 32 * WI, LR = AJ / 4;               // LR: lanes of a row
   float* buf = reinterpret_cast<float*>(smem);
-  const int c = lane * 4, gj = j0 + c;
+  const int c = lane % LR * 4, gj = j0 + c;
   const long cbase = OUT == 3 && gj < m.N ? ns_at(m, 0, gj) : 0;
+  // the row in the pass, and in the matrix, of a lane's t-th run
+  auto prow = [&](int t) { return wave * (RP / 4) + t * (64 / LR) + lane / LR; };
+  auto mrow = [&](int i, int r) { return i0 + (r >> 5) * 64 + i * 32 + (r & 31); };
   const bool four = gj + 4 <= m.N && (OUT != 3 || (m.cols & 3) == 0);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < TM; ++i) {
     float4 p[8];
     if constexpr (OUT == 3) {
       if (four) {
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-          const int gi = i0 + i * 32 + wave * 8 + t;
+          const int gi = mrow(i, prow(t));
           if (gi < m.M) {
             const NsU4 u = *reinterpret_cast<const NsU4*>(k.s.p + cbase + (long)gi * m.ld);
             p[t] = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
@@ -903,21 +928,22 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<float4*>(buf + (lane & 31) * 264 + wn + j * 32 + 8 * q + 4 * (lane >> 5)) =
+        *reinterpret_cast<float4*>(buf + ((WI == 1 ? 0 : (wave >> 1) * 32) + (lane & 31)) * BS + wn + j * 32 + 8 * q + 4 * (lane >> 5)) =
             make_float4(acc[i][j][4 * q] * f, acc[i][j][4 * q + 1] * f, acc[i][j][4 * q + 2] * f, acc[i][j][4 * q + 3] * f);
     __syncthreads();
     if constexpr (OUT == 0) {
-      // planes: 16 blocks of 32 rows, 1 KB each
+      // planes: blocks of 32 rows, 1 KB each
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int blk = t * 4 + wave, row = lane >> 1, col = blk * 16 + (lane & 1) * 8;
-        if (i0 + i * 32 + row >= m.Mp || j0 + col >= m.Np) continue;
-        const float4 u = *reinterpret_cast<const float4*>(buf + row * 264 + col), w = *reinterpret_cast<const float4*>(buf + row * 264 + col + 4);
+        const int k16 = t * 4 + wave, blk = k16 % (AJ / 16), row = k16 / (AJ / 16) * 32 + (lane >> 1), col = blk * 16 + (lane & 1) * 8;
+        const int gi = mrow(i, row);
+        if (gi >= m.Mp || j0 + col >= m.Np) continue;
+        const float4 u = *reinterpret_cast<const float4*>(buf + row * BS + col), w = *reinterpret_cast<const float4*>(buf + row * BS + col + 4);
         const float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
         half8 h, l;
 #pragma unroll
         for (int e = 0; e < 8; ++e) { _Float16 th, tl; split16(x[e], th, tl); h[e] = th; l[e] = tl; }
-        _Float16* o = k.wso + m.x + cat(m.Mp, i0 + i * 32 + row, j0 + col);
+        _Float16* o = k.wso + m.x + cat(m.Mp, gi, j0 + col);
         *reinterpret_cast<half8*>(o) = h;
         *reinterpret_cast<half8*>(o + xpl) = l;
       }
@@ -925,8 +951,8 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(const NsGroup gr, int 
     }
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      const int gi = i0 + i * 32 + wave * 8 + t;
-      const float4 v = *reinterpret_cast<const float4*>(buf + (wave * 8 + t) * 264 + c);
+      const int gi = mrow(i, prow(t));
+      const float4 v = *reinterpret_cast<const float4*>(buf + prow(t) * BS + c);
       const float x[4] = {v.x, v.y, v.z, v.w};
       if (gi < m.M && four) {
         if constexpr (OUT == 3) {
@@ -1305,7 +1331,8 @@ static NsCounts ns_counts(NsMat& m, long ks, bool flat) {
   const long n64 = m.Mp / 64, n32 = m.Mp / 32;
   c.n[F_CHAIN] = n64 * (n64 + 1) / 2;
   c.n[F_JOIN] = n32 * (n32 + 1) / 2;
-  c.n[F_APPLY] = (long)cdiv(m.Mp, AI) * cdiv(m.Np, AJ);
+  c.n[F_APPLY] = (long)cdiv(m.Mp, AI) * cdiv(m.Np, 256);
+  c.n[F_APPLY2] = (long)cdiv(m.Mp, AI) * cdiv(m.Np, 128);
   c.x = 2L * m.Np * (m.Mp + 8);
   c.g = 10L * m.Mp * (m.Mp + 8);
   c.part = c.n[F_GRAM] * GT * GT;
@@ -1389,6 +1416,7 @@ static const char* ns_plan_table(NsPlan& pl, const pg_muon_entry_t* e, int n) {
   return nullptr;
 }
 
+constexpr long APPLY_FEW = 512;
 struct NsSource { int kind; const void* x; };      // kind: ns_elem's SRC
 
 // everything behind the sums of squares.  out_kind: ns_apply_kernel's OUT of the last product
@@ -1455,18 +1483,25 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     a.mul = (float)ldexp(1.0, -psc) * (last ? 1.f : sx);
     a.out = out; a.ldo = ldo; a.s = step;
     const int o = last ? out_kind : 0;
-    const dim3 gd((unsigned)up(pl.n[F_APPLY], 8));
-    const int na = (int)pl.n[F_APPLY];
+    const bool wide = pl.n[F_APPLY] > APPLY_FEW;
+    const int na = (int)pl.n[wide ? F_APPLY : F_APPLY2];
+    const dim3 gd((unsigned)up(na, 8));
+#define NS_APPLY(PX, O)                                                                              \
+  do {                                                                                               \
+    if (wide) PG_KLAUNCH((ns_apply_kernel<PX, O, 1>), gd, blk, 0, st, gr, na, a);                    \
+    else PG_KLAUNCH((ns_apply_kernel<PX, O, 2>), gd, blk, 0, st, gr, na, a);                         \
+  } while (0)
     if (one) {
-      if (o == 0) PG_KLAUNCH((ns_apply_kernel<1, 0>), gd, blk, 0, st, gr, na, a);
-      else if (o == 1) PG_KLAUNCH((ns_apply_kernel<1, 1>), gd, blk, 0, st, gr, na, a);
-      else PG_KLAUNCH((ns_apply_kernel<1, 2>), gd, blk, 0, st, gr, na, a);
+      if (o == 0) NS_APPLY(1, 0);
+      else if (o == 1) NS_APPLY(1, 1);
+      else NS_APPLY(1, 2);
     } else {
-      if (o == 0) PG_KLAUNCH((ns_apply_kernel<2, 0>), gd, blk, 0, st, gr, na, a);
-      else if (o == 1) PG_KLAUNCH((ns_apply_kernel<2, 1>), gd, blk, 0, st, gr, na, a);
-      else if (o == 2) PG_KLAUNCH((ns_apply_kernel<2, 2>), gd, blk, 0, st, gr, na, a);
-      else PG_KLAUNCH((ns_apply_kernel<2, 3>), gd, blk, 0, st, gr, na, a);
+      if (o == 0) NS_APPLY(2, 0);
+      else if (o == 1) NS_APPLY(2, 1);
+      else if (o == 2) NS_APPLY(2, 2);
+      else NS_APPLY(2, 3);
     }
+#undef NS_APPLY
     _Float16* t = xin; xin = xout; xout = t;
     first = false;
   }
