@@ -300,6 +300,31 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
   const long n = (long)m.taps * m.rows * m.cols;
   const int np = m.np;
   const int first = gr.tab ? m.sq0 : r.id * gr.per[F_MOM];
+  // the tile's elements are on their way while the sums are joined
+  // wide: 64 rows x 128 columns, 8 plane elements per thread and trip, 1 KB runs per wave
+  const int tr = m.Mp / 64, tj = m.Np / 64;
+  const int wi = (r.tile % tr) * 64 + ((threadIdx.x >> 1) & 63), wj = (r.tile / tr) * 128 + (threadIdx.x & 1) * 8 + (threadIdx.x >> 7) * 16;
+  // tall: 64 x 64 through LDS, plane row i = stored flat column, plane column j = stored row
+  const int i0 = (r.tile / tj) * 64, j0 = (r.tile % tj) * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  float v[4][8];
+  if (!m.tall) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int j = wj + q * 32;
+      if (wi < m.M && j < m.N) {
+        ns_load8<SRC>(m, x, s, wi, j, v[q]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[q][e] = 0.f;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const int j = j0 + q * 4 + ty, i = i0 + tx;
+      v[q >> 3][q & 7] = (j < m.N && i < m.M) ? ns_elem<SRC>(x, s, ns_at(m, j, i)) : 0.f;
+    }
+  }
   double a = 0.0;
   for (int i = threadIdx.x; i < np; i += 256) a += sq[first + i];
   a = block_sum_d256(a, red);
@@ -311,35 +336,19 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
   _Float16* hi = ws + m.x;
   _Float16* lo = hi + xplane(m);
   if (!m.tall) {
-    // 64 rows x 128 columns: 8 plane elements per thread and trip, 1 KB runs per wave
-    const int tr = m.Mp / 64;
-    const int i = (r.tile % tr) * 64 + ((threadIdx.x >> 1) & 63), jt = (r.tile / tr) * 128 + (threadIdx.x & 1) * 8 + (threadIdx.x >> 7) * 16;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int j = jt + q * 32;
+      const int j = wj + q * 32;
       if (j >= m.Np) break;
-      float v[8];
-      if (i < m.M && j < m.N) {
-        ns_load8<SRC>(m, x, s, i, j, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      }
       half8 h, l;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { _Float16 th, tl; split16(v[e] * f, th, tl); h[e] = th; l[e] = tl; }
-      *reinterpret_cast<half8*>(hi + cat(m.Mp, i, j)) = h;
-      if constexpr (!ONE) *reinterpret_cast<half8*>(lo + cat(m.Mp, i, j)) = l;
+      for (int e = 0; e < 8; ++e) { _Float16 th, tl; split16(v[q][e] * f, th, tl); h[e] = th; l[e] = tl; }
+      *reinterpret_cast<half8*>(hi + cat(m.Mp, wi, j)) = h;
+      if constexpr (!ONE) *reinterpret_cast<half8*>(lo + cat(m.Mp, wi, j)) = l;
     }
   } else {
-    // 64 x 64 tile through LDS: plane row i = stored flat column, plane column j = stored row
-    const int tj = m.Np / 64;
-    const int i0 = (r.tile / tj) * 64, j0 = (r.tile % tj) * 64;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    for (int q = ty; q < 64; q += 4) {
-      const int j = j0 + q, i = i0 + tx;
-      tile[q][tx] = (j < m.N && i < m.M) ? ns_elem<SRC>(x, s, ns_at(m, j, i)) : 0.f;
-    }
+#pragma unroll
+    for (int q = 0; q < 16; ++q) tile[q * 4 + ty][tx] = v[q >> 3][q & 7];
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -1416,7 +1425,7 @@ static const char* ns_plan_table(NsPlan& pl, const pg_muon_entry_t* e, int n) {
   return nullptr;
 }
 
-constexpr long APPLY_FEW = 512;
+constexpr long APPLY_FEW = 256;
 struct NsSource { int kind; const void* x; };      // kind: ns_elem's SRC
 
 // everything behind the sums of squares.  out_kind: ns_apply_kernel's OUT of the last product
