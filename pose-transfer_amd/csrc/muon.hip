@@ -1316,11 +1316,12 @@ static bool ns_shape(NsMat& m) {
   const long rows = m.rows, cols = (long)m.taps * m.cols;
   if (rows * cols > 0x7fffffffL) return false;
   m.tall = rows > cols;
+  const long Mp = up(m.tall ? cols : rows, 64), Np = up(m.tall ? rows : cols, 64);
+  if (Mp * Np > 0x7fffffffL) return false;           // also: Np fits an int
   m.M = (int)(m.tall ? cols : rows);
   m.N = (int)(m.tall ? rows : cols);
-  m.Mp = (int)up(m.M, 64);
-  m.Np = (int)up(m.N, 64);
-  if ((long)m.Mp * m.Np > 0x7fffffffL) return false;
+  m.Mp = (int)Mp;
+  m.Np = (int)Np;
   return true;
 }
 struct NsCounts { long n[F_N], x, g, part; };
@@ -1371,7 +1372,7 @@ constexpr long GRAM_SLOTS = 512;
 static const char* ns_plan_batch(NsPlan& pl, long batch, long rows, long cols, long sx, long ldx, long so) {
   NsMat m{};
   m.taps = 1; m.rows = (int)rows; m.cols = (int)cols; m.ld = ldx; m.st = 0;
-  if (!ns_shape(m)) return "a matrix has more than 2^31 - 1 elements";
+  if (!ns_shape(m)) return "a matrix has more than 2^31 - 1 elements (sides rounded up to 64)";
   const long nt = cdiv(m.Mp, GT);
   const NsCounts c = ns_counts(m, GRAM_SLOTS / (nt * (nt + 1) / 2 * batch), false);
   pl.top = m.Mp;
@@ -1399,7 +1400,7 @@ static const char* ns_plan_table(NsPlan& pl, const pg_muon_entry_t* e, int n) {
     m.ld = m.cols; m.st = (long)m.rows * m.cols;
     if ((long)m.taps * m.rows > 0x7fffffffL || (long)m.taps * m.rows * m.cols > 0x7fffffffL) return "a tensor has more than 2^31 - 1 elements";
     if (m.kind == 0) {
-      if (!ns_shape(m)) return "a matrix has more than 2^31 - 1 elements";
+      if (!ns_shape(m)) return "a matrix has more than 2^31 - 1 elements (sides rounded up to 64)";
       work += ns_gram_work(m);
       if (m.Mp > pl.top) pl.top = m.Mp;
     }

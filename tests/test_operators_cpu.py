@@ -74,6 +74,16 @@ def test_orthogonalise_empty_and_workspace():
     assert 0 < a < b < 6 * a
 
 
+@pytest.mark.parametrize("rows,cols", [(1, (1 << 31) - 1), ((1 << 31) - 1, 1), (1, (1 << 31) - 40), (2, 1 << 30), (1, 1 << 26)])
+def test_orthogonalise_refuses_long_thin_matrices(rows, cols):
+    """a side near 2^31 rounds up past 32 bits: refused, never wrapped to a small padded size"""
+    assert L.load().pg_orthogonalise_workspace(1, rows, cols) == -1
+    assert orth(batch=1, rows=rows, cols=cols, ldx=cols, ldo=cols) != 0
+    t = table([(0, 1, rows, cols, 0, 1.0)])
+    assert L.load().pg_muon_workspace(t.ctypes.data, 1) == -1
+    assert muon(entries=[(0, 1, rows, cols, 0, 1.0)], total=1 << 40) != 0
+
+
 def table(rows):
     return np.array([tuple(r) + (0,) for r in rows], dtype=O.MUON_ENTRY)
 
