@@ -381,7 +381,7 @@ typedef struct {
   float scale;                 /* kind 0: factor of the orthogonal update, e.g. 0.2 sqrt(max(rows, taps * cols)) for an rms of 0.2 */
   int32_t _pad;
 } pg_muon_entry_t;
-/* The optimiser step of every tensor of an arena (entries in ascending, disjoint order, a HOST array read during the call):
+/* The optimiser step of every tensor of an arena (at most 65536 entries in ascending, disjoint order, a HOST array read during the call):
  *   kind 0: m = momentum m + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum m : m;
  *           p = p (1 - lr weight_decay) - lr scale orthogonalise(u)
  *   kind 1: Adam with (beta1, beta2, adam_eps), the step number `step` (+ *ctr if ctr is given: replay-safe, as pg_adam_ctr)

@@ -26,6 +26,7 @@
 // All matrices of a call share every launch (a device table of tile ranges).
 #include "common.h"
 #include <math.h>
+#include <new>
 #include <vector>
 
 namespace pg {
@@ -1389,8 +1390,15 @@ static const char* ns_plan_batch(NsPlan& pl, long batch, long rows, long cols, l
   return nullptr;
 }
 
+constexpr int MAX_ENTRIES = 1 << 16;
 static const char* ns_plan_table(NsPlan& pl, const pg_muon_entry_t* e, int n) {
-  pl.mats.resize((size_t)n);
+  if (n > MAX_ENTRIES) return "more than 65536 tensors";
+  try {                                              // no exception leaves a C entry
+    pl.mats.resize((size_t)n);
+    pl.first.resize((size_t)n * F_N);
+  } catch (const std::bad_alloc&) {
+    return "out of host memory";
+  }
   long work = 0;
   for (int i = 0; i < n; ++i) {
     NsMat& m = pl.mats[(size_t)i];
@@ -1405,7 +1413,6 @@ static const char* ns_plan_table(NsPlan& pl, const pg_muon_entry_t* e, int n) {
       if (m.Mp > pl.top) pl.top = m.Mp;
     }
   }
-  pl.first.resize((size_t)n * F_N);
   long x = 0, g = 0, part = 0;
   for (int i = 0; i < n; ++i) {
     NsMat& m = pl.mats[(size_t)i];
@@ -1599,7 +1606,7 @@ extern "C" int pg_muon_step(const pg_muon_t* d, void* stream) {
   PG_REQUIRE(bad == nullptr, "pg_muon_step: %s", bad);
   for (int i = 0; i < d->n; ++i) {
     const pg_muon_entry_t& e = d->entries[i];
-    PG_REQUIRE(e.off + (int64_t)e.taps * e.rows * e.cols <= d->total, "pg_muon_step: entry %d ends behind the arena", i);
+    PG_REQUIRE(e.off <= d->total - (int64_t)e.taps * e.rows * e.cols, "pg_muon_step: entry %d ends behind the arena", i);
     PG_REQUIRE(e.kind == 0 || d->v, "pg_muon_step: an Adam entry needs v");
     if (i > 0) {
       const pg_muon_entry_t& q = d->entries[i - 1];

@@ -116,6 +116,16 @@ def test_muon_step_refuses(bad):
     assert L.load().pg_last_error().decode().startswith("pg_muon_step")
 
 
+def test_muon_step_refuses_sizes_behind_the_address_space():
+    """a count or an offset that no arena can have ends in an error, not in an exception of the allocator or a wrapped sum"""
+    t = table(GOOD)
+    assert L.load().pg_muon_workspace(t.ctypes.data, (1 << 16) + 1) == -1
+    assert muon(n=(1 << 31) - 1) != 0
+    assert "65536" in L.load().pg_last_error().decode()
+    assert muon(entries=[((1 << 63) - 1, 1, 8, 24, 0, 1.0)], total=(1 << 63) - 1) != 0
+    assert "ends behind the arena" in L.load().pg_last_error().decode()
+
+
 def test_muon_tables():
     lib = L.load()
     assert lib.pg_muon_workspace(None, 0) == 0
