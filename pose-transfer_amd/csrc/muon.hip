@@ -1370,23 +1370,34 @@ static void ns_place(NsPlan& pl, int nmat, long nx, long ng, long npart) {
 // workgroups of a Gram launch that run at once: two per CU
 constexpr long GRAM_SLOTS = 512;
 
-static const char* ns_plan_batch(NsPlan& pl, long batch, long rows, long cols, long sx, long ldx, long so) {
+// a launch has less than 2^32 lanes: at most this many workgroups of 256 (the chain's launches have two per tile)
+constexpr long MAX_GROUPS = 1L << 22;
+// A batch goes in pieces whose workspace stays below 2 GB (padded planes of many thin matrices take far more than the matrices): a
+// piece of that size runs for milliseconds, its twenty launches cost 0.1 ms.
+constexpr long PIECE_BYTES = 2L << 30;
+
+// the plan of `piece` of the batch's matrices
+static const char* ns_plan_batch(NsPlan& pl, long batch, long rows, long cols, long sx, long ldx, long so, long& piece) {
   NsMat m{};
   m.taps = 1; m.rows = (int)rows; m.cols = (int)cols; m.ld = ldx; m.st = 0;
   if (!ns_shape(m)) return "a matrix has more than 2^31 - 1 elements (sides rounded up to 64)";
   const long nt = cdiv(m.Mp, GT);
   const NsCounts c = ns_counts(m, GRAM_SLOTS / (nt * (nt + 1) / 2 * batch), false);
+  long most = 1;
+  for (int f = 0; f < F_N; ++f) most = c.n[f] > most ? c.n[f] : most;
+  if (most > MAX_GROUPS) return "a matrix is too large";
+  const long fit = PIECE_BYTES / (c.x * 4 + c.g * 2 + c.part * 4);
+  piece = MAX_GROUPS / most < fit ? MAX_GROUPS / most : fit < 1 ? 1 : fit;
+  if (piece > batch) piece = batch;
   pl.top = m.Mp;
   pl.gr.tab = nullptr;
-  pl.gr.n = (int)batch;
   pl.gr.u = m;
   pl.gr.src_step = sx; pl.gr.out_step = so; pl.gr.x_step = c.x; pl.gr.g_step = c.g; pl.gr.part_step = c.part;
   for (int f = 0; f < F_N; ++f) {
     pl.gr.per[f] = (int)c.n[f];
-    pl.n[f] = c.n[f] * batch;
-    if (c.n[f] > 0x3fffffffL || pl.n[f] > 0x3fffffffL) return "too many matrices for one call";
+    pl.n[f] = c.n[f] * piece;
   }
-  ns_place(pl, (int)batch, c.x * batch, c.g * batch, c.part * batch);
+  ns_place(pl, (int)piece, c.x * piece, c.g * piece, c.part * piece);
   return nullptr;
 }
 
@@ -1425,7 +1436,7 @@ static const char* ns_plan_table(NsPlan& pl, const pg_muon_entry_t* e, int n) {
     for (int f = 0; f < F_N; ++f) {
       pl.first[(size_t)(f * n + i)] = (int)pl.n[f];
       pl.n[f] += c.n[f];
-      if (pl.n[f] > 0x3fffffffL) return "too many tensors for one call";
+      if (pl.n[f] > MAX_GROUPS) return "too many tensors for one call";
     }
   }
   ns_place(pl, n, x, g, part);
@@ -1544,7 +1555,8 @@ extern "C" int64_t pg_orthogonalise_workspace(int64_t batch, int64_t rows, int64
   if (batch > 0x3fffffff || rows > 0x7fffffff || cols > 0x7fffffff) return -1;
   if (ns_is_small(rows, cols)) return 0;
   NsPlan pl{};
-  return ns_plan_batch(pl, batch, rows, cols, 0, cols, 0) ? -1 : pl.bytes;
+  long piece;
+  return ns_plan_batch(pl, batch, rows, cols, 0, cols, 0, piece) ? -1 : pl.bytes;
 }
 
 extern "C" int pg_orthogonalise(const void* x, int32_t x_is_bf16, int64_t batch, int64_t rows, int64_t cols, int64_t x_batch, int64_t ldx,
@@ -1564,26 +1576,35 @@ extern "C" int pg_orthogonalise(const void* x, int32_t x_is_bf16, int64_t batch,
     m.taps = 1; m.rows = (int)rows; m.cols = (int)cols; m.ld = (long)ldx;
     ns_shape(m);
     hipStream_t st = (hipStream_t)stream;
-    const unsigned nb = (unsigned)batch;
-    if (x_is_bf16 && out_is_bf16) ns_small<1, 2>(m, x, (long)x_batch, out, (long)out_batch, (long)ldo, steps, eps, nb, st);
-    else if (x_is_bf16) ns_small<1, 1>(m, x, (long)x_batch, out, (long)out_batch, (long)ldo, steps, eps, nb, st);
-    else if (out_is_bf16) ns_small<0, 2>(m, x, (long)x_batch, out, (long)out_batch, (long)ldo, steps, eps, nb, st);
-    else ns_small<0, 1>(m, x, (long)x_batch, out, (long)out_batch, (long)ldo, steps, eps, nb, st);
+    for (int64_t b = 0; b < batch; b += MAX_GROUPS) {        // a workgroup of 512 per matrix
+      const unsigned nb = (unsigned)(batch - b < MAX_GROUPS ? batch - b : MAX_GROUPS);
+      const char* xb = reinterpret_cast<const char*>(x) + b * x_batch * (x_is_bf16 ? 2 : 4);
+      char* ob = reinterpret_cast<char*>(out) + b * out_batch * (out_is_bf16 ? 2 : 4);
+      if (x_is_bf16 && out_is_bf16) ns_small<1, 2>(m, xb, (long)x_batch, ob, (long)out_batch, (long)ldo, steps, eps, nb, st);
+      else if (x_is_bf16) ns_small<1, 1>(m, xb, (long)x_batch, ob, (long)out_batch, (long)ldo, steps, eps, nb, st);
+      else if (out_is_bf16) ns_small<0, 2>(m, xb, (long)x_batch, ob, (long)out_batch, (long)ldo, steps, eps, nb, st);
+      else ns_small<0, 1>(m, xb, (long)x_batch, ob, (long)out_batch, (long)ldo, steps, eps, nb, st);
+    }
     PG_LAUNCH_OK("pg_orthogonalise");
     return 0;
   }
   NsPlan pl{};
-  const char* bad = ns_plan_batch(pl, batch, rows, cols, x_batch, ldx, out_batch);
+  long piece = 0;
+  const char* bad = ns_plan_batch(pl, batch, rows, cols, x_batch, ldx, out_batch, piece);
   PG_REQUIRE(bad == nullptr, "pg_orthogonalise: %s", bad);
   PG_REQUIRE(workspace && workspace_bytes >= pl.bytes, "pg_orthogonalise: workspace of %lld bytes required", (long long)pl.bytes);
   char* w = reinterpret_cast<char*>(workspace);
   hipStream_t st = (hipStream_t)stream;
   double* sq = reinterpret_cast<double*>(w + pl.off_sq);
-  if (x_is_bf16) PG_KLAUNCH((ns_sumsq_kernel<1>), dim3((unsigned)pl.n[F_MOM]), dim3(256), 0, st, pl.gr, x, sq);
-  else PG_KLAUNCH((ns_sumsq_kernel<0>), dim3((unsigned)pl.n[F_MOM]), dim3(256), 0, st, pl.gr, x, sq);
-  const NsSource in = {x_is_bf16 ? 1 : 0, x};
   const NsStep none{};
-  ns_run(pl, w, in, none, steps, eps, out_is_bf16 ? 2 : 1, out, (long)ldo, st);
+  for (int64_t b = 0; b < batch; b += piece) {
+    pl.gr.n = (int)(batch - b < piece ? batch - b : piece);
+    for (int f = 0; f < F_N; ++f) pl.n[f] = (long)pl.gr.per[f] * pl.gr.n;
+    const NsSource in = {x_is_bf16 ? 1 : 0, reinterpret_cast<const char*>(x) + b * x_batch * (x_is_bf16 ? 2 : 4)};
+    if (x_is_bf16) PG_KLAUNCH((ns_sumsq_kernel<1>), dim3((unsigned)pl.n[F_MOM]), dim3(256), 0, st, pl.gr, in.x, sq);
+    else PG_KLAUNCH((ns_sumsq_kernel<0>), dim3((unsigned)pl.n[F_MOM]), dim3(256), 0, st, pl.gr, in.x, sq);
+    ns_run(pl, w, in, none, steps, eps, out_is_bf16 ? 2 : 1, reinterpret_cast<char*>(out) + b * out_batch * (out_is_bf16 ? 2 : 4), (long)ldo, st);
+  }
   PG_LAUNCH_OK("pg_orthogonalise");
   return 0;
 }

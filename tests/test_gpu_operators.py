@@ -216,6 +216,28 @@ def test_orthogonalise_singular_values_and_spectra():
             assert 0.6 < float(s.min()) and float(s.max()) < 1.25
 
 
+def test_orthogonalise_large_batches():
+    """a batch that does not fit one launch (lanes of the one-launch form) or one workspace goes in pieces: every matrix gets what it
+    gets by itself, a piece's last one and the next one's first among them"""
+    from pose_transfer_amd.runtime import lib as L
+    O = ops()
+    n = (1 << 23) + 5
+    x = rnd(46, n, 2, 2)
+    out = O.orthogonalise(x)
+    for sl in (slice(0, 3), slice((1 << 22) - 2, (1 << 22) + 2), slice((1 << 23) - 2, n)):
+        assert torch.equal(out[sl], O.orthogonalise(x[sl])), sl
+    n = 12000
+    assert L.load().pg_orthogonalise_workspace(n, 1, 385) <= 1 << 31 < n * (2 * 2 * 448 * 72 * 2)
+    x = rnd(47, n, 1, 385, dtype=torch.bfloat16)
+    out = O.orthogonalise(x, out_dtype=torch.float32).double()
+    ref = x.double()
+    ref = ref / (ref.norm(dim=2, keepdim=True) + 1e-7)
+    for _ in range(5):                                        # one row: A = |x|^2
+        a = (ref * ref).sum(2, keepdim=True)
+        ref = (NS[0] + NS[1] * a + NS[2] * a * a) * ref
+    assert float(((out - ref).norm(dim=2) / ref.norm(dim=2)).max()) <= 1.5 * NS[0] ** 5 * 2.0 ** -20
+
+
 def test_orthogonalise_scales_strides_and_special_values():
     O = ops()
     x = rnd(22, 4, 70, 210)
