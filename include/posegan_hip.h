@@ -314,7 +314,8 @@ int pg_warp_mask_max_bwd(const float* gout, const uint8_t* argmax, const float* 
  * x [rows][C] with row stride ldx, res (NULL: none) ldr, y (NULL: not written) ldy; h (NULL: not written), q packed [rows][C].
  * q (NULL: none): e4m3 bytes of y / scale, scale = max|y| / 448 of a group of `group` channels (32, 64, 128, 256; 0: of the row; the last
  * group may be short), 1 where the group is all zero; scales [rows][ceil(C / group)].  rstd (NULL: none) [rows] = s, for the backward
- * pass.  h may be x or res, y may be x, res or h (row strides equal) for C <= 2048; a NaN stays in its row.                       */
+ * pass.  h may be x or res, y may be x, res or h (row strides equal) for C <= 2048; a NaN stays in its row.
+ * C <= 2^30, rows <= 2^40.                                                                                                   */
 int pg_rms_norm_fwd(const void* x, const void* res, const float* gamma, int64_t rows, int32_t C, int64_t ldx, int64_t ldr, float eps,
                     int32_t io_flags, void* h, void* y, int64_t ldy, void* q, float* scales, int32_t group, float* rstd, void* stream);
 /* backward: dx (= the residual's gradient) = s (w - h s mean_c(w h s)) + dh with w = dy gamma; dgamma[c] (+)= sum_rows dy h s.  dy has row

@@ -522,6 +522,14 @@ static long rms_bwd_blocks(long rows, int lpr, int nch) {
   return b > 1024 ? 1024 : b;
 }
 static int rms_long_slices(long rows) { return rows < 64 ? (int)rows : 64; }
+// the kernels count a row's elements in 32 bits, up to a turn of the lanes behind its end
+constexpr int MAX_C = 1 << 30;
+// a launch has less than 2^32 lanes: more rows go in several
+constexpr long MAX_BLOCKS = 1L << 23;
+template <typename P>
+static P* rms_at(P* p, long elems, size_t size) {
+  return p ? reinterpret_cast<P*>(const_cast<char*>(reinterpret_cast<const char*>(p)) + elems * (long)size) : nullptr;
+}
 
 }  // namespace pg
 
@@ -530,7 +538,8 @@ using namespace pg;
 extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamma, int64_t rows, int32_t C, int64_t ldx, int64_t ldr,
                                float eps, int32_t io_flags, void* h, void* y, int64_t ldy, void* q, float* scales, int32_t group,
                                float* rstd, void* stream) {
-  PG_REQUIRE(x && gamma && rows >= 0 && C > 0 && ldx >= C && eps >= 0.f, "pg_rms_norm_fwd: x, gamma, rows >= 0, C > 0 and ldx >= C required");
+  PG_REQUIRE(x && gamma && rows >= 0 && C > 0 && C <= MAX_C && ldx >= C && eps >= 0.f,
+             "pg_rms_norm_fwd: x, gamma, rows >= 0, 0 < C <= 2^30 and ldx >= C required");
   PG_REQUIRE(io_flags == 0 || io_flags == 3, "pg_rms_norm_fwd: io_flags 0 (fp32) or 3 (bf16)");
   PG_REQUIRE(y || q || h, "pg_rms_norm_fwd: nothing to write (y, q and h are all NULL)");
   PG_REQUIRE(!res || ldr >= C, "pg_rms_norm_fwd: ldr >= C required");
@@ -546,17 +555,17 @@ extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamm
   const int grp = q && group < C ? group : 0;          // a group that is the whole row
   const RmsShape sh = rms_shape((long)rows, C, V, grp, false);
   const int lpr = sh.lpr, nch = sh.nch;
-  const long blocks = nch ? (rows + 256 / lpr - 1) / (256 / lpr) : rows;
-  PG_REQUIRE(blocks < (1L << 31), "pg_rms_norm_fwd: too many rows");
+  const long per = nch ? 256 / lpr : 1;                // rows of a workgroup
+  const size_t es = io_flags ? 2 : 4;
+  PG_REQUIRE(rows <= (1L << 40), "pg_rms_norm_fwd: too many rows");
   PG_REQUIRE(nch || ((h == nullptr || (h != x && h != res)) && (y == nullptr || (y != x && y != res && y != h))),
              "pg_rms_norm_fwd: rows of more than 2048 channels are read twice: outputs must not be inputs");
   PG_REQUIRE((h == nullptr || ((h != x || ldx == C) && (h != res || ldr == C))) &&
              (y == nullptr || ((y != x || ldy == ldx) && (y != res || ldy == ldr) && (y != h || ldy == C))),
              "pg_rms_norm_fwd: an output in place of an input needs the same row stride");
-  RmsFwdK k = {x, res, gamma, (long)rows, C, (long)ldx, (long)ldr, (long)ldy, eps, h, y, (uint8_t*)q, scales, grp,
-               grp ? (C + grp - 1) / grp : 1, rstd};
+  const int ngroups = grp ? (C + grp - 1) / grp : 1;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)blocks), wg(256);
+  const dim3 wg(256);
 #define PG_RF1(T, L, N, EX)                                                                                        \
   do {                                                                                                             \
     if (q) PG_KLAUNCH((rms_fwd_kernel<T, L, N, true, EX>), grid, wg, 0, st, k);                                    \
@@ -599,8 +608,15 @@ extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamm
         break;                                                                                                     \
     }                                                                                                              \
   } while (0)
-  if (io_flags == 0) PG_RF(float);
-  else PG_RF(bf16_t);
+  for (long r0 = 0; r0 < rows; r0 += MAX_BLOCKS * per) {
+    const long n = rows - r0 < MAX_BLOCKS * per ? rows - r0 : MAX_BLOCKS * per;
+    const dim3 grid((unsigned)((n + per - 1) / per));
+    const RmsFwdK k = {rms_at(x, r0 * ldx, es), rms_at(res, r0 * ldr, es), gamma, n, C, (long)ldx, (long)ldr, (long)ldy, eps,
+                       rms_at(h, r0 * C, es), rms_at(y, r0 * ldy, es), rms_at((uint8_t*)q, r0 * C, 1), rms_at(scales, r0 * ngroups, 4), grp, ngroups,
+                       rms_at(rstd, r0, 4)};
+    if (io_flags == 0) PG_RF(float);
+    else PG_RF(bf16_t);
+  }
 #undef PG_RF
 #undef PG_RF1
   PG_LAUNCH_OK("pg_rms_norm_fwd");
@@ -618,8 +634,8 @@ extern "C" int64_t pg_rms_norm_bwd_workspace(int64_t rows, int32_t C, int32_t io
 extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, const void* h, const float* rstd, const float* gamma,
                                int64_t rows, int32_t C, int32_t io_flags, void* dx, float* dgamma, int32_t accumulate,
                                void* workspace, int64_t workspace_bytes, void* stream) {
-  PG_REQUIRE(dy && h && rstd && gamma && dx && dgamma && rows >= 0 && C > 0 && lddy >= C,
-             "pg_rms_norm_bwd: dy, h, rstd, gamma, dx, dgamma, rows >= 0, C > 0 and lddy >= C required");
+  PG_REQUIRE(dy && h && rstd && gamma && dx && dgamma && rows >= 0 && C > 0 && C <= MAX_C && lddy >= C,
+             "pg_rms_norm_bwd: dy, h, rstd, gamma, dx, dgamma, rows >= 0, 0 < C <= 2^30 and lddy >= C required");
   PG_REQUIRE(io_flags == 0 || io_flags == 3, "pg_rms_norm_bwd: io_flags 0 (fp32) or 3 (bf16)");
   const size_t em = io_flags ? 1 : 3;
   PG_REQUIRE((((size_t)dy | (size_t)dh | (size_t)h | (size_t)dx) & em) == 0 &&
@@ -636,7 +652,7 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
   const RmsShape sh = rms_shape((long)rows, C, io_flags ? 8 : 4, 0, true);
   const int lpr = sh.lpr, nch = sh.nch;
   const long nb = nch ? rms_bwd_blocks(rows, lpr, nch) : rms_long_slices(rows);
-  PG_REQUIRE(nch || rows < (1L << 31), "pg_rms_norm_bwd: too many rows");
+  PG_REQUIRE(rows <= (1L << 40), "pg_rms_norm_bwd: too many rows");
   PG_REQUIRE(nch || (dx != dy && dx != dh && dx != h), "pg_rms_norm_bwd: rows of more than 2048 channels are read twice: dx must not be an input");
   PG_REQUIRE(dx != dy || lddy == C, "pg_rms_norm_bwd: dx in place of dy needs lddy == C");
   RmsBwdK k = {dy, dh, h, rstd, gamma, (long)rows, C, (long)lddy, dx, (float*)workspace, dgamma, accumulate};
@@ -679,7 +695,12 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
       case 64 * 32 + 14: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 7 : 4), false); break;                                   \
       case 64 * 32 + 16: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 8 : 4), false); break;                                   \
       default:                                                                                                     \
-        PG_KLAUNCH((rms_bwd_long_kernel<T>), dim3((unsigned)rows), dim3(256), 0, st, k);                           \
+        for (long r0 = 0; r0 < rows; r0 += MAX_BLOCKS) {                                                           \
+          const long n = rows - r0 < MAX_BLOCKS ? rows - r0 : MAX_BLOCKS;                                          \
+          const RmsBwdK kr = {rms_at(dy, r0 * lddy, sizeof(T)), rms_at(dh, r0 * C, sizeof(T)), rms_at(h, r0 * C, sizeof(T)), \
+                              rms_at(rstd, r0, 4), gamma, n, C, (long)lddy, rms_at(dx, r0 * C, sizeof(T)), nullptr, nullptr, 0}; \
+          PG_KLAUNCH((rms_bwd_long_kernel<T>), dim3((unsigned)n), dim3(256), 0, st, kr);                           \
+        }                                                                                                          \
         PG_KLAUNCH((rms_dgamma_long_kernel<T>), dim3((C + 255) / 256, (unsigned)nb), dim3(256), 0, st, k);         \
         break;                                                                                                     \
     }                                                                                                              \

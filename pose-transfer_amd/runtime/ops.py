@@ -66,10 +66,16 @@ def _vector(t, name, like, n):
         raise ValueError("%s: a contiguous fp32 vector of %d on %s expected" % (name, n, like.device))
 
 
+def _channels(n):
+    if n > 1 << 30:                  # the C argument has 32 bits, which ctypes would wrap
+        raise ValueError("rms_norm: at most 2^30 channels")
+
+
 def _norm_args(x, gamma, residual):
     if not (torch.is_tensor(x) and x.is_cuda and x.dtype in _IO and x.dim() == 2 and x.shape[1] > 0):
         raise ValueError("rms_norm: x must be an fp32 or bf16 [rows, channels] tensor on the GPU")
     shape = x.shape
+    _channels(shape[1])
     _vector(gamma, "gamma", x, shape[1])
     return shape[0], shape[1], _rows(x, "x", x, shape), 0 if residual is None else _rows(residual, "residual", x, shape)
 
@@ -111,6 +117,7 @@ def rms_norm_bwd(dy, h, rstd, gamma, dh=None):
         raise ValueError("rms_norm_bwd: h must be an fp32 or bf16 [rows, channels] tensor on the GPU")
     shape = h.shape
     rows, ch = shape
+    _channels(ch)
     if _rows(h, "h", h, shape) != ch or (dh is not None and _rows(dh, "dh", h, shape) != ch):
         raise ValueError("rms_norm_bwd: h and dh must be packed")
     lddy = _rows(dy, "dy", h, shape)
@@ -136,6 +143,7 @@ def orthogonalise(x, steps=5, eps=1e-7, out_dtype=None):
     _need(x.dim() in (2, 3), "orthogonalise: [rows, cols] or [batch, rows, cols] expected")
     out_dtype = x.dtype if out_dtype is None else out_dtype
     _need(out_dtype in _IO, "orthogonalise: out_dtype must be float32 or bfloat16")
+    _need(1 <= steps <= 32, "orthogonalise: steps 1..32")
     x3 = x if x.dim() == 3 else x.unsqueeze(0)
     b, r, c = x3.shape
     if c > 1 and x3.stride(2) != 1 or r > 1 and x3.stride(1) < c or b > 1 and x3.stride(0) < 0:
@@ -174,6 +182,7 @@ def muon_step(p, g, m, v, table, lr, momentum=0.95, nesterov=True, weight_decay=
             continue
         _need(torch.is_tensor(t) and t.dtype in dts and t.device == p.device and t.shape == p.shape and t.is_contiguous(),
               "muon_step: g, m, v and p_bf16 must be contiguous arenas like p (g fp32 or bf16, m and v fp32, p_bf16 bf16)")
+    _need(1 <= ns_steps <= 32, "muon_step: ns_steps 1..32")
     _need(ctr is None or (torch.is_tensor(ctr) and ctr.dtype == torch.int64 and ctr.device == p.device and ctr.numel() >= 1),
           "muon_step: ctr must be an int64 tensor on p's device")
     if len(table) == 0:

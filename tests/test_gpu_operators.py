@@ -145,6 +145,37 @@ def test_rms_norm_special_values():
     assert torch.equal(q[ok].view(torch.uint8), q0.view(torch.uint8)) and torch.equal(scale[ok], scale0)
 
 
+def test_rms_norm_more_rows_than_one_launch_holds():
+    """2^28 rows of one channel fill a launch of eight lanes each: the rows behind them too"""
+    O = ops()
+    n = (1 << 28) + 77
+    x = torch.arange(n, device="cuda", dtype=torch.int32).remainder_(7).to(torch.bfloat16).add_(1).view(n, 1)
+    gamma = torch.full((1,), 0.5, device="cuda")
+    y, _, rstd = O.rms_norm(x, gamma)
+    # h rstd gamma = 0.5 / sqrt(1 + eps / h^2): 0.5 in bf16
+    assert bool((y == 0.5).all())
+    assert float((rstd * x[:, 0].float() - 1).abs().max()) < 1e-6
+    del y
+    q, scale, _, _ = O.rms_norm_q8(x, gamma)
+    assert bool((q.view(torch.uint8) == q.view(torch.uint8)[0, 0]).all())
+    assert float((scale * q[0, 0].float() - 0.5).abs().max()) < 1e-6          # 1e-6 / 2 (eps) and three roundings of 2^-25
+    del x, q, scale, rstd
+    n, c = (1 << 23) + 3, 2049                             # a workgroup per row: 34 GB a tensor
+    h = torch.ones(n, c, dtype=torch.bfloat16, device="cuda")
+    rstd = torch.ones(n, device="cuda")
+    g = torch.ones(c, device="cuda")
+    h[-1] = 2.0
+    dx, dgamma = O.rms_norm_bwd(h, h, rstd, g)              # w = xh: dx = h - h mean(h^2)
+    assert bool((dx[:-1] == 0).all()) and bool((dx[-1] == -6).all())
+    del dx
+    assert float((dgamma - (n + 3)).abs().max()) <= 2.0 ** -24 * (n + 3)
+    h[-1] = 3.0
+    y, _, r = O.rms_norm(h, g, eps=0.0)
+    assert bool((y == 1).all()) and float((r[-1] - 1 / 3).abs()) < 1e-7
+    del y, h
+    torch.cuda.empty_cache()
+
+
 def test_rms_norm_empty_and_other_stream():
     O = ops()
     e = torch.empty(0, 64, device="cuda")

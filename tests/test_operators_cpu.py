@@ -144,6 +144,18 @@ def test_wrappers_refuse_on_the_host():
             f()
 
 
+def test_sizes_that_32_bits_do_not_hold():
+    """ctypes wraps an argument that its type does not hold, and a row's end plus a turn of the lanes must fit an int"""
+    for n in ((1 << 30) + 1, (1 << 32) + 8):
+        with pytest.raises(ValueError):
+            O._channels(n)
+    O._channels(1 << 30)
+    n = (1 << 31) - 1
+    assert rms(rows=1, C=n, ldx=n, ldy=n) != 0 and "2^30" in L.load().pg_last_error().decode()
+    assert rms_bwd(rows=1, C=n, lddy=n, ws=P, wsb=1 << 40) != 0 and "2^30" in L.load().pg_last_error().decode()
+    assert rms(rows=(1 << 40) + 1) != 0 and rms_bwd(rows=(1 << 40) + 1, ws=P, wsb=1 << 40) != 0
+
+
 def test_muon_table_of_the_networks():
     """every element of an arena is in exactly one record; the matrices are the inner blocks' filters"""
     from pose_transfer_amd.runtime import engine as E
