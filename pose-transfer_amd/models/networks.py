@@ -12,6 +12,7 @@ import os
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from ..runtime import engine as E
 from ..runtime import lib as L
@@ -272,9 +273,16 @@ class Discriminator(_ArenaModule):
 
 class _RMSNormFn(torch.autograd.Function):
     @staticmethod
+    def _rows(t):
+        """t as rows of its last dimension for the kernels: a copy where the channels do not lie together or the rows overlap (the
+        expanded gradient of a sum, a broadcast residual)"""
+        t = t.reshape(-1, t.shape[-1])
+        return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+    @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        c = x.shape[-1]
-        y, h, rstd = OPS.rms_norm(x.reshape(-1, c), weight, None if residual is None else residual.reshape(-1, c), eps=eps)
+        rows = _RMSNormFn._rows
+        y, h, rstd = OPS.rms_norm(rows(x), weight, None if residual is None else rows(residual), eps=eps)
         h = h.contiguous()
         ctx.save_for_backward(h, rstd, weight)
         ctx.has_res = residual is not None
@@ -282,21 +290,23 @@ class _RMSNormFn(torch.autograd.Function):
         return (y.view(x.shape), h.view(x.shape)) if ctx.has_res else y.view(x.shape)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gy, gh=None):
         h, rstd, weight = ctx.saved_tensors
         if gy is None:
             return gh, None, gh, None
-        shape = gy.shape
         dh = None if gh is None else gh.reshape(h.shape).contiguous()
-        dx, dw = OPS.rms_norm_bwd(gy.reshape(h.shape), h, rstd, weight, dh=dh)
-        dx = dx.view(shape)
+        dx, dw = OPS.rms_norm_bwd(_RMSNormFn._rows(gy), h, rstd, weight, dh=dh)
+        dx = dx.view(gy.shape)
         return dx, dw, dx if ctx.has_res else None, None
 
 
 class RMSNorm(nn.Module):
     """Root-mean-square norm along the last dimension (the channels of pixel-major activations [N][H][W][C]) with a gain per
     channel, next to the per-sample norm of the reference's blocks (networks.py:159,166-169).  forward(x) -> y;
-    forward(x, residual) -> (y, x + residual): a pre-norm residual block hands the sum on.  fp32 or bf16."""
+    forward(x, residual) -> (y, x + residual): a pre-norm residual block hands the sum on.  fp32 or bf16; differentiable once.
+    In a captured graph forward and backward belong together: autograd cannot capture the backward of leaves that an earlier eager
+    graph still holds."""
 
     def __init__(self, channels, eps=1e-6, device="cuda"):
         super().__init__()
@@ -304,4 +314,6 @@ class RMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(channels, dtype=torch.float32, device=device))
 
     def forward(self, x, residual=None):
+        if residual is not None and residual.shape != x.shape:
+            raise ValueError("RMSNorm: residual %s and x %s differ in shape" % (tuple(residual.shape), tuple(x.shape)))
         return _RMSNormFn.apply(x, self.weight, residual, self.eps)

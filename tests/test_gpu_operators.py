@@ -444,6 +444,43 @@ def test_rms_norm_module(dtype):
     assert torch.equal(only_h, torch.ones_like(x))
 
 
+def test_rms_norm_module_layouts_and_refusals():
+    """expanded gradients, channels-first inputs and broadcast residuals, as autograd and other layers hand them over"""
+    from pose_transfer_amd.models.networks import RMSNorm
+    mod = RMSNorm(24)
+    x = rnd(75, 6, 24).requires_grad_()
+    mod(x).sum().backward()                                   # the gradient is one expanded element
+    want, gw = torch.autograd.grad(mod(x), (x, mod.weight), torch.ones(6, 24, device="cuda"))
+    assert torch.equal(x.grad, want) and torch.equal(mod.weight.grad, gw)
+    xt = rnd(76, 24, 6).requires_grad_()                      # channels first: a transposed view
+    wy = rnd(77, 24, 6)
+    (mod(xt.t()) * wy.t()).sum().backward()
+    xc = xt.detach().t().contiguous().requires_grad_()
+    (mod(xc) * wy.t().contiguous()).sum().backward()
+    assert torch.equal(xt.grad.t(), xc.grad)
+    r = rnd(78, 1, 24).requires_grad_()                       # one residual row for all
+    y, h = mod(x.detach(), r.expand(6, 24))
+    (y * h).sum().backward()
+    rc = r.detach().repeat(6, 1).requires_grad_()
+    y, h = mod(x.detach(), rc)
+    (y * h).sum().backward()
+    assert torch.equal(r.grad, rc.grad.sum(0, keepdim=True))
+    s = rnd(79, 6, 24).requires_grad_()                       # both inputs the same tensor: twice the gradient
+    y, h = mod(s, s)
+    (y.sum() + (2 * h).sum()).backward()
+    s2, s3 = s.detach().clone().requires_grad_(), s.detach().clone().requires_grad_()
+    y, h = mod(s2, s3)
+    (y.sum() + (2 * h).sum()).backward()
+    assert torch.equal(s.grad, s2.grad + s3.grad) and s2.grad.data_ptr() != s3.grad.data_ptr()
+    with pytest.raises(ValueError):
+        mod(x, torch.zeros(12, 12, device="cuda"))
+    with pytest.raises(ValueError):
+        mod(rnd(80, 2, 3, 24), rnd(81, 3, 2, 24))
+    (g,) = torch.autograd.grad(mod(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def trainer(optimizer, precision=0, n=2, size=64):
     from types import SimpleNamespace
     from pose_transfer_amd.models.pose_gan import DeformablePose_GAN
