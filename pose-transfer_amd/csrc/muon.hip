@@ -1483,26 +1483,29 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
       else PG_KLAUNCH((ns_chain_small_kernel<128>), gm, dim3(1024), 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
       psc = ns > 1 ? SP : SG;
     } else {
-    PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.n[F_JOIN]), blk, 0, st, gr, (const float*)part, cf, 1.f / sx, g);
-    auto chain = [&](const ChainJob& a, const ChainJob* b) {
-      const int total = b ? 2 * nc : nc;
-      const dim3 gd((unsigned)up(total, 8));
-      const ChainJob b1 = b ? *b : a;
-      if (many) PG_KLAUNCH(ns_chain_kernel, gd, blk, 0, st, gr, a, b1, total, nc, g);
-      else if (pl.top <= 256) PG_KLAUNCH((ns_chain32_kernel<256>), gd, blk, 0, st, gr, a, b1, total, nc, g);
-      else PG_KLAUNCH((ns_chain32_kernel<512>), gd, blk, 0, st, gr, a, b1, total, nc, g);
-    };
-    for (int k = 0; k < ns; ++k) {
-      const int q = k == 0 ? 3 : 1;
-      const ChainJob quad = {0, 0, q, NS_C * q1, 1};
-      const ChainJob qg = {q, 0, 2, q1, 0}, qp = {q, p, 7 - p, (float)ldexp(1.0, SP - SG - psc), 0}, qqg = {q, 2, 0, q1, 0};
-      const bool more = k + 1 < ns;
-      chain(quad, nullptr);
-      if (more) chain(qg, k > 0 ? &qp : nullptr);
-      else if (k > 0) chain(qp, nullptr);
-      if (more) chain(qqg, nullptr);
-      if (k > 0) { p = 7 - p; psc = SP; }
-    }
+      PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.n[F_JOIN]), blk, 0, st, gr, (const float*)part, cf, 1.f / sx, g);
+      auto chain = [&](const ChainJob& a, const ChainJob* b) {
+        const int total = b ? 2 * nc : nc;
+        const dim3 gd((unsigned)up(total, 8));
+        const ChainJob b1 = b ? *b : a;
+        if (many) PG_KLAUNCH(ns_chain_kernel, gd, blk, 0, st, gr, a, b1, total, nc, g);
+        // all tiles run at once: 1, 2 or 5 workgroups to a CU by their LDS, fewer columns at a time (two jobs of 184 tiles: 9.4 us in
+        // two turns of 512 columns, 7.4 us in one with 256; of 336 tiles: 9.3 us with 256, 5.8 us with 128)
+        else if (total > 512) PG_KLAUNCH((ns_chain32_kernel<128>), gd, blk, 0, st, gr, a, b1, total, nc, g);
+        else if (pl.top <= 256 || total > 256) PG_KLAUNCH((ns_chain32_kernel<256>), gd, blk, 0, st, gr, a, b1, total, nc, g);
+        else PG_KLAUNCH((ns_chain32_kernel<512>), gd, blk, 0, st, gr, a, b1, total, nc, g);
+      };
+      for (int k = 0; k < ns; ++k) {
+        const int q = k == 0 ? 3 : 1;
+        const ChainJob quad = {0, 0, q, NS_C * q1, 1};
+        const ChainJob qg = {q, 0, 2, q1, 0}, qp = {q, p, 7 - p, (float)ldexp(1.0, SP - SG - psc), 0}, qqg = {q, 2, 0, q1, 0};
+        const bool more = k + 1 < ns;
+        chain(quad, nullptr);
+        if (more) chain(qg, k > 0 ? &qp : nullptr);
+        else if (k > 0) chain(qp, nullptr);
+        if (more) chain(qqg, nullptr);
+        if (k > 0) { p = 7 - p; psc = SP; }
+      }
     }
     ApplyK a;
     memset(&a, 0, sizeof(a));
