@@ -1035,14 +1035,13 @@ struct SmallChain {
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-    const unsigned pa = (unsigned)(size_t)a + fa, pb = (unsigned)(size_t)b + fb;
 #pragma unroll
     for (int ks = 0; ks < MP / 16; ++ks) {
-      half8 x[2][1], y[2][1];
-      fetch_nt<PS>(pa + ks * (MP * 32), pb + ks * (MP * 32), x, y);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0][0], y[0][0], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[0][0], y[1][0], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[1][0], y[0][0], acc, 0, 0, 0);
+      const half8 x0 = *reinterpret_cast<const half8*>(a + fa + ks * (MP * 32)), x1 = *reinterpret_cast<const half8*>(a + fa + ks * (MP * 32) + PS);
+      const half8 y0 = *reinterpret_cast<const half8*>(b + fb + ks * (MP * 32)), y1 = *reinterpret_cast<const half8*>(b + fb + ks * (MP * 32) + PS);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x0, y0, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x0, y1, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x1, y0, acc, 0, 0, 0);
     }
     return acc;
   }
