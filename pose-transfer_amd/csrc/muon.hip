@@ -15,7 +15,7 @@
 // Arithmetic.  The matrix cores have no fast fp32 form (1 / 16 of the fp16 rate).  Every operand is held as TWO fp16 values, hi + lo =
 // 22 bits, scaled by a power of two; a product is three MFMAs, hi hi + hi lo + lo hi, with fp32 accumulation: what an fp32 product
 // gives (measured 4.8e-6 against 4.7e-6 through five steps; a bf16 pair with its 16 bits: 4e-5, single bf16 operands: 2e-2).  X0's
-// scale makes its rms 1 within a factor 2^0.5: its largest element is then at most sqrt(rows cols) <= 2^15.5, the loss of a tiny one's last bits
+// scale makes its rms 1/2 .. 1: its largest element is then at most sqrt(rows cols) <= 2^15.5, the loss of a tiny one's last bits
 // is 2^-25 of the rms.  |G|, |Q G| <= 1.5, |Q| <= 3.45, |P| <= 3.45^3 = 41 bound the others' scales.  A bf16 input is one fp16 value exactly (8 bits): one plane.
 //
 // Layout.  A matrix is stored by the caller as [taps][rows][cols] with row and tap strides (a packed convolution weight is one matrix
@@ -49,6 +49,7 @@ struct NsMat {
   int ks, kc;                   // Gram: splits of the long side and their length (a multiple of 32)
   int np;                       // partial sums of squares
   float scale;
+  double inv;                   // 1 / number of elements
   long x, g, part;              // offsets in the workspace: X planes and chain planes (halves), Gram partials (floats)
   int sq0;                      // first partial sum of squares
 };
@@ -280,13 +281,16 @@ __device__ __forceinline__ long xplane(const NsMat& m) { return (long)m.Np * (m.
 __device__ __forceinline__ long cplane(const NsMat& m) { return (long)m.Mp * (m.Mp + 8); }
 
 // ---------------------------------------------------------------------------------------------- split into fp16 planes
-// planes hold 2^-k U with an rms in 2^-0.75 .. 2^0.25: the largest element, at most sqrt(n) rms <= 2^15.5 2^0.25, fits fp16.
-// c = 2^k / (|U| + eps): from the planes' units to X0's
-__device__ __forceinline__ void ns_scale(double sumsq, long n, float eps, int& k, float& c) {
-  const double norm = sqrt(sumsq), rms = sqrt(sumsq / (double)n);
-  k = 0;
-  if (rms > 0.0 && rms < 1e300) k = max(-126, min(126, (int)rint(log2(rms) + 0.25)));
-  c = norm == 0.0 ? 0.f : (float)(ldexp(1.0, k) / (norm + (double)eps));
+// planes hold 2^-k U with an rms in 2^-1 .. 1: the largest element, at most sqrt(n) rms <= 2^15.5, fits fp16.  k from the exponent of the
+// mean square alone: every thread of every workgroup needs it (with log2 and a square root in fp64 it took 2 us)
+__device__ __forceinline__ int ns_exponent(double sumsq, double inv) {
+  const int e = (int)((__double_as_longlong(sumsq * inv) >> 52) & 0x7ff) - 1023;      // 2^e <= mean square < 2^(e + 1)
+  return max(-126, min(126, (e + 2) >> 1));
+}
+__device__ __forceinline__ float ns_pow2(int k) { return __uint_as_float((unsigned)(k + 127) << 23); }      // |k| <= 126
+// 2^k / (|U| + eps): from the planes' units to X0's
+__device__ __forceinline__ float ns_factor(double sumsq, int k, float eps) {
+  return sumsq == 0.0 ? 0.f : (float)((double)ns_pow2(k) / (sqrt(sumsq) + (double)eps));
 }
 // every workgroup joins its matrix's partial sums of squares itself (a few hundred doubles); the first one publishes
 // c = 2^k / (|U| + eps), the factor from the planes' units to X0's
@@ -298,7 +302,6 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
   constexpr bool ONE = SRC == 1;
   const NsRef r = ns_find<F_SPLIT>(gr, blockIdx.x);
   const NsMat& m = r.m;
-  const long n = (long)m.taps * m.rows * m.cols;
   const int np = m.np;
   const int first = gr.tab ? m.sq0 : r.id * gr.per[F_MOM];
   // the tile's elements are on their way while the sums are joined
@@ -329,11 +332,9 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
   double a = 0.0;
   for (int i = threadIdx.x; i < np; i += 256) a += sq[first + i];
   a = block_sum_d256(a, red);
-  int k;
-  float cf;
-  ns_scale(a, n, eps, k, cf);
-  const float f = (float)ldexp(1.0, -k);
-  if (r.tile == 0 && threadIdx.x == 0) cfac[r.id] = cf;
+  const int k = ns_exponent(a, m.inv);
+  const float f = ns_pow2(-k);
+  if (r.tile == 0 && threadIdx.x == 0) cfac[r.id] = ns_factor(a, k, eps);
   _Float16* hi = ws + m.x;
   _Float16* lo = hi + xplane(m);
   if (!m.tall) {
@@ -1143,6 +1144,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
   typedef SmallChain<64> Sc;
   __shared__ __attribute__((aligned(1024))) char smem[2 * XP + 2 * Sc::BUF];
   __shared__ double red[8];
+  __shared__ float cfac;
   char* const X = smem;
   char* const b1 = smem + 2 * XP;
   char* const b2 = b1 + Sc::BUF;
@@ -1173,10 +1175,9 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
   a = 0.0;
 #pragma unroll
   for (int w = 0; w < 8; ++w) a += red[w];
-  int k;
-  float cf;
-  ns_scale(a, (long)m.rows * m.cols, eps, k, cf);
-  const float f = (float)ldexp(1.0, -k);
+  const int k = ns_exponent(a, m.inv);
+  const float f = ns_pow2(-k);
+  if (tid == 511) cfac = ns_factor(a, k, eps);
 #pragma unroll
   for (int t = 0; t < RUNS; ++t) {
     const int c = t * 512 + tid;
@@ -1204,7 +1205,8 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
   const Sc sc(wave & 3);
   const int r4 = (lane >> 2) & 3, cq = lane & 3, mb = (lane >> 4) & 1, kh = lane >> 5;
   const int nblk = m.Np / 16;
-  float c1 = cf;
+  __syncthreads();
+  float c1 = cfac;
   while (steps > 0) {
     const int ns = steps < 3 ? steps : 3;
     steps -= ns;
@@ -1322,6 +1324,7 @@ static bool ns_shape(NsMat& m) {
   m.N = (int)(m.tall ? rows : cols);
   m.Mp = (int)Mp;
   m.Np = (int)Np;
+  m.inv = 1.0 / (double)(rows * cols);
   return true;
 }
 struct NsCounts { long n[F_N], x, g, part; };
