@@ -1136,6 +1136,12 @@ __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32)) void ns_chain_small_ker
   }
 }
 
+// the transposing read (fetch_apply) where no transfer is in flight: the compiler places its wait
+__device__ __forceinline__ half4 lds_tr(const char* p) {
+  typedef __fp16 tr4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr4*)p));
+}
+
 // Everything in one launch for matrices of at most 64 x NX: X stays in LDS from the first load to the result.  8 waves: the Gram product
 // divides the columns among two groups of four, the chain takes four waves, P X goes by strips of 32 columns, in place.
 template <int NX, int SRC, int OUT>
@@ -1214,13 +1220,14 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
     f32x16 g;
 #pragma unroll
     for (int e = 0; e < 16; ++e) g[e] = 0.f;
+#pragma unroll 2
     for (int b = wave >> 2; b < nblk; b += 2) {
-      half8 p[2][1], q[2][1];
-      const unsigned at = (unsigned)(size_t)X + b * 2048;
-      fetch_nt<XP>(at + sc.fa, at + sc.fb, p, q);
-      g = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0][0], q[0][0], g, 0, 0, 0);
-      g = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[0][0], q[1][0], g, 0, 0, 0);
-      g = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[1][0], q[0][0], g, 0, 0, 0);
+      const char* at = X + b * 2048;
+      const half8 p0 = *reinterpret_cast<const half8*>(at + sc.fa), p1 = *reinterpret_cast<const half8*>(at + sc.fa + XP);
+      const half8 q0 = *reinterpret_cast<const half8*>(at + sc.fb), q1 = *reinterpret_cast<const half8*>(at + sc.fb + XP);
+      g = __builtin_amdgcn_mfma_f32_32x32x16_f16(p0, q0, g, 0, 0, 0);
+      g = __builtin_amdgcn_mfma_f32_32x32x16_f16(p0, q1, g, 0, 0, 0);
+      g = __builtin_amdgcn_mfma_f32_32x32x16_f16(p1, q0, g, 0, 0, 0);
     }
     float4* buf = reinterpret_cast<float4*>(b1);
     if (!on) {
@@ -1252,16 +1259,13 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         half8 p[2][2];
-        half4 t[2][2];
         const int r = lane & 31;
-        const unsigned pa = (unsigned)(size_t)b1 + ks * 2048 + r * 32 + ((kh ^ swz(r)) << 4);
-        const unsigned pb = (unsigned)(size_t)X + (s * 2 + mb) * 2048 + (ks * 16 + 8 * kh + r4) * 32 + (((cq >> 1) ^ kh) << 4) + (cq & 1) * 8;
-        asm volatile(NS_RD "%0, %8\n\t" NS_RD "%1, %8 offset:1024\n\t" NS_RD "%2, %8 offset:%10\n\t" NS_RD "%3, %8 offset:%11\n\t"
-                     NS_TR "%4, %9\n\t" NS_TR "%5, %9 offset:128\n\t" NS_TR "%6, %9 offset:%12\n\t" NS_TR "%7, %9 offset:%13\n\t" "s_waitcnt lgkmcnt(0)"
-                     : "=&v"(p[0][0]), "=&v"(p[0][1]), "=&v"(p[1][0]), "=&v"(p[1][1]), "=&v"(t[0][0]), "=&v"(t[0][1]), "=&v"(t[1][0]), "=&v"(t[1][1])
-                     : "v"(pa), "v"(pb), "n"(Sc::PS), "n"(Sc::PS + 1024), "n"(XP), "n"(XP + 128) : "memory");
-        const half8 y0 = __builtin_shufflevector(t[0][0], t[0][1], 0, 1, 2, 3, 4, 5, 6, 7);
-        const half8 y1 = __builtin_shufflevector(t[1][0], t[1][1], 0, 1, 2, 3, 4, 5, 6, 7);
+        const char* pa = b1 + ks * 2048 + r * 32 + ((kh ^ swz(r)) << 4);
+        const char* pb = X + (s * 2 + mb) * 2048 + (ks * 16 + 8 * kh + r4) * 32 + (((cq >> 1) ^ kh) << 4) + (cq & 1) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i >> 1][i & 1] = *reinterpret_cast<const half8*>(pa + (i >> 1) * Sc::PS + (i & 1) * 1024);
+        const half8 y0 = __builtin_shufflevector(lds_tr(pb), lds_tr(pb + 128), 0, 1, 2, 3, 4, 5, 6, 7);
+        const half8 y1 = __builtin_shufflevector(lds_tr(pb + XP), lds_tr(pb + XP + 128), 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y0, p[0][i], acc[i], 0, 0, 0);
@@ -1286,6 +1290,19 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
             *reinterpret_cast<half4*>(at) = h;
             *reinterpret_cast<half4*>(at + XP) = l;
           } else if (row < m.M) {
+            if (!m.tall && col + 4 <= m.N) {
+              const long at = (long)blockIdx.x * out_step + (long)row * ldo + col;
+              if constexpr (OUT == 1) {
+                NsU4 u;
+                u.x = __float_as_uint(o[0]); u.y = __float_as_uint(o[1]); u.z = __float_as_uint(o[2]); u.w = __float_as_uint(o[3]);
+                *reinterpret_cast<NsU4*>(reinterpret_cast<float*>(outp) + at) = u;
+              } else {
+                NsU2 u;
+                u.x = ns_pack_bf16(o[0], o[1]); u.y = ns_pack_bf16(o[2], o[3]);
+                *reinterpret_cast<NsU2*>(reinterpret_cast<bf16_t*>(outp) + at) = u;
+              }
+              continue;
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               if (col + e >= m.N) break;
