@@ -1005,7 +1005,7 @@ __global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr,
 
 // ---------------------------------------------------------------------------------------------- small matrices
 // The chain of a matrix with a short side of at most MP (64, 128) in ONE workgroup: (MP / 32)^2 waves, each with one 32 x 32 block of every
-// matrix in its registers; two LDS buffers hold the operands of the product under way (fp16 pairs, [plane][block][MP rows][16]).
+// matrix in its registers; LDS buffers hold the operands of the products under way (fp16 pairs, [plane][block][MP rows][16]).
 // A launch of the tiled form costs 5 us whatever its size, a product here 0.6 (64) to 1.2 us (128).
 template <int MP>
 struct SmallChain {
@@ -1046,47 +1046,86 @@ struct SmallChain {
     }
     return acc;
   }
-  // g: this wave's block of G (scale 2^SG).  Returns its block of P, scale 2^(steps > 1 ? SP : SG).  `on`: this wave has a block; every
-  // wave of the workgroup calls it
-  __device__ __forceinline__ f32x16 run(bool on, f32x16 g, int steps, char* b1, char* b2) const {
+  // q = a I + b G + c G^2, G's block in g and all of it in `buf`
+  __device__ __forceinline__ f32x16 quad(const f32x16& g, const char* buf) const {
+    f32x16 q = mul(buf, buf);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      q[e] = q[e] * (NS_C / (float)(1 << SG)) + NS_B * g[e];
+      if (wi == wj && 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31)) q[e] += NS_A * (float)(1 << SG);
+    }
+    return q;
+  }
+  static __device__ __forceinline__ float pscale(int k) { return 1.f / (float)(1 << (k == 1 ? 2 * SG - SP : SG)); }
+
+  // g: this wave's block of G (scale 2^SG).  Returns its block of P, scale 2^(steps > 1 ? SP : SG).  Every wave of the workgroup calls it;
+  // a product begins when both operands are in LDS and its result goes where nobody reads any more.
+  // Two buffers: one group of waves.
+  __device__ __forceinline__ f32x16 run2(f32x16 g, int steps, char* b1, char* b2) const {
     const float q1 = 1.f / (float)(1 << SG);
     f32x16 P, y;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) P[e] = 0.f;
     __syncthreads();
-    if (on) put(b1, g);
+    put(b1, g);
     __syncthreads();
     for (int k = 0; k < steps; ++k) {
       const bool more = k + 1 < steps;
-      f32x16 q;
-      if (on) {
-        q = mul(b1, b1);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          q[e] = q[e] * (NS_C * q1) + NS_B * g[e];
-          if (wi == wj && 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31)) q[e] += NS_A * (float)(1 << SG);
-        }
-        put(b2, q);
-      }
+      const f32x16 q = quad(g, b1);
+      put(b2, q);
       __syncthreads();
-      if (on && more) y = mul(b2, b1) * q1;
+      if (more) y = mul(b2, b1) * q1;
       if (k == 0) {
         P = q;
       } else {
         __syncthreads();
-        if (on) put(b1, P);
+        put(b1, P);
         __syncthreads();
-        if (on) P = mul(b2, b1) * (k == 1 ? 1.f / (float)(1 << (2 * SG - SP)) : q1);
+        P = mul(b2, b1) * pscale(k);
       }
       if (more) {
         __syncthreads();
-        if (on) put(b1, y);
+        put(b1, y);
         __syncthreads();
-        if (on) g = mul(b2, b1) * q1;
+        g = mul(b2, b1) * q1;
         __syncthreads();
-        if (on) put(b1, g);
+        put(b1, g);
         __syncthreads();
       }
+    }
+    return P;
+  }
+  // Four buffers and two groups of waves (grp): the first one follows G, the second one P; three barriers a step.  P is group
+  // (steps > 1)'s; g is group 0's.
+  __device__ __forceinline__ f32x16 run4(int grp, f32x16 g, int steps, char* b) const {
+    const float q1 = 1.f / (float)(1 << SG);
+    char *const bg = b, *const bq = b + BUF, *const by = b + 2 * BUF, *const bp = b + 3 * BUF;
+    f32x16 P;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) P[e] = 0.f;
+    __syncthreads();
+    if (grp == 0) put(bg, g);
+    __syncthreads();
+    for (int k = 0; k < steps; ++k) {
+      if (grp == 0) {
+        const f32x16 q = quad(g, bg);
+        put(bq, q);
+        if (k == 0) { P = q; put(bp, q); }
+      }
+      __syncthreads();
+      const bool more = k + 1 < steps;
+      if (grp == 0) {
+        if (more) put(by, mul(bq, bg) * q1);
+      } else if (k > 0) {
+        P = mul(bq, bp) * pscale(k);
+      }
+      if (!more) break;
+      __syncthreads();
+      if (grp == 0) {
+        g = mul(bq, by) * q1;
+        put(bg, g);
+      } else if (k > 0) {
+        put(bp, P);
+      }
+      __syncthreads();
     }
     return P;
   }
@@ -1094,15 +1133,16 @@ struct SmallChain {
 
 // the join of the Gram slices and the whole chain of one stage: one workgroup per matrix, P to buffer 3
 template <int MP>
-__global__ __launch_bounds__(64 * (MP / 32) * (MP / 32)) void ns_chain_small_kernel(const NsGroup gr, const float* part, const float* cfac, float cconst,
+__global__ __launch_bounds__(MP * 8) void ns_chain_small_kernel(const NsGroup gr, const float* part, const float* cfac, float cconst,
                                                                                   int steps, _Float16* ws) {
   typedef SmallChain<MP> Sc;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * Sc::BUF];
+  __shared__ __attribute__((aligned(1024))) char smem[(MP == 64 ? 4 : 2) * Sc::BUF];
   const int id = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = wave / (Sc::W * Sc::W);            // 64: two groups of waves; 128: one
   NsMat m = gr.tab ? gr.tab[id] : gr.u;
   if (m.kind == 1) return;
   if (!gr.tab) { m.g += (long)id * gr.g_step; m.part += (long)id * gr.part_step; }
-  const Sc sc(wave);
+  const Sc sc(wave % (Sc::W * Sc::W));
   const int frag = ((sc.wi >> 1) * 2 + (sc.wj >> 1)) * 4 + (sc.wi & 1) * 2 + (sc.wj & 1);
   const float4* src = reinterpret_cast<const float4*>(part + m.part) + frag * 256 + lane;
   const float c1 = cfac ? cfac[id] : cconst;
@@ -1110,7 +1150,7 @@ __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32)) void ns_chain_small_ker
   f32x16 g;
 #pragma unroll
   for (int e = 0; e < 16; ++e) g[e] = 0.f;
-  if (sc.wi * 32 < m.Mp && sc.wj * 32 < m.Mp) {
+  if (grp == 0 && sc.wi * 32 < m.Mp && sc.wj * 32 < m.Mp) {
 #pragma unroll 4
     for (int s = 0; s < m.ks; ++s)
 #pragma unroll
@@ -1120,9 +1160,11 @@ __global__ __launch_bounds__(64 * (MP / 32) * (MP / 32)) void ns_chain_small_ker
       }
     g = g * c2;
   }
-  const f32x16 P = sc.run(true, g, steps, smem, smem + Sc::BUF);
+  f32x16 P;
+  if constexpr (MP == 64) P = sc.run4(grp, g, steps, smem);
+  else P = sc.run2(g, steps, smem, smem + Sc::BUF);
   const int row = sc.wj * 32 + (lane & 31);
-  if (sc.wi * 32 >= m.Mp || sc.wj * 32 >= m.Mp) return;
+  if (sc.wi * 32 >= m.Mp || sc.wj * 32 >= m.Mp || (MP == 64 && grp != (steps > 1))) return;
   const long pl = cplane(m);
   _Float16* out = ws + m.g + 6 * pl;
 #pragma unroll
@@ -1148,12 +1190,11 @@ template <int NX, int SRC, int OUT>
 __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void* x, long src_step, void* outp, long out_step, long ldo, int steps, float eps) {
   constexpr int XP = NX * 64 * 2;                     // bytes of a plane: [NX / 16][64 rows][16]
   typedef SmallChain<64> Sc;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * XP + 2 * Sc::BUF];
-  __shared__ double red[8];
-  __shared__ float cfac;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * XP + 4 * Sc::BUF];         // 64 x 384: all of the CU's 160 KB
   char* const X = smem;
   char* const b1 = smem + 2 * XP;
-  char* const b2 = b1 + Sc::BUF;
+  double* const red = reinterpret_cast<double*>(b1);                // before the first product
+  float& cfac = *reinterpret_cast<float*>(b1 + 64);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   NsMat mm = m;
   mm.src += (long)blockIdx.x * src_step;
@@ -1244,9 +1285,9 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
         g[4 * q + 2] = (g[4 * q + 2] + u.z) * c2; g[4 * q + 3] = (g[4 * q + 3] + u.w) * c2;
       }
     }
-    const f32x16 P = sc.run(on, g, ns, b1, b2);
+    const f32x16 P = sc.run4(wave >> 2, g, ns, b1);
     __syncthreads();
-    if (on) sc.put(b1, P);
+    if ((wave >> 2) == (ns > 1)) sc.put(b1, P);
     __syncthreads();
     const bool last = steps == 0;
     const float mul = c1 * (ns > 1 ? 1.f / (float)(1 << SP) : 1.f / (float)(1 << SG)) * (last ? 1.f : 32768.f);
@@ -1498,7 +1539,7 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     const int nc = (int)pl.n[many ? F_CHAIN : F_JOIN];
     if (pl.top <= 128) {
       const dim3 gm((unsigned)gr.n);
-      if (pl.top == 64) PG_KLAUNCH((ns_chain_small_kernel<64>), gm, blk, 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
+      if (pl.top == 64) PG_KLAUNCH((ns_chain_small_kernel<64>), gm, dim3(512), 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
       else PG_KLAUNCH((ns_chain_small_kernel<128>), gm, dim3(1024), 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
       psc = ns > 1 ? SP : SG;
     } else {
