@@ -780,38 +780,37 @@ __device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned 
                : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
 }
 
-__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[2][2][2]) {
-  asm volatile(NS_RD "%0, %12\n\t" NS_TR "%4, %13\n\t" NS_TR "%5, %14\n\t" NS_RD "%1, %12 offset:1024\n\t"
-               NS_TR "%6, %13 offset:1024\n\t" NS_TR "%7, %14 offset:1024\n\t" NS_RD "%2, %12 offset:4096\n\t" NS_RD "%3, %12 offset:5120\n\t"
-               NS_TR "%8, %13 offset:4096\n\t" NS_TR "%9, %14 offset:4096\n\t" NS_TR "%10, %13 offset:5120\n\t" NS_TR "%11, %14 offset:5120\n\t"
+__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[2][1][2]) {
+  asm volatile(NS_RD "%0, %8\n\t" NS_TR "%4, %9\n\t" NS_TR "%5, %10\n\t" NS_RD "%1, %8 offset:1024\n\t"
+               NS_RD "%2, %8 offset:4096\n\t" NS_RD "%3, %8 offset:5120\n\t" NS_TR "%6, %9 offset:4096\n\t" NS_TR "%7, %10 offset:4096\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]),
-                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1]),
-                 "=&v"(b[1][0][0]), "=&v"(b[1][0][1]), "=&v"(b[1][1][0]), "=&v"(b[1][1][1])
+                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[1][0][0]), "=&v"(b[1][0][1])
                : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
 }
-__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[1][2][2]) {
-  asm volatile(NS_RD "%0, %8\n\t" NS_TR "%4, %9\n\t" NS_TR "%5, %10\n\t" NS_RD "%1, %8 offset:1024\n\t"
-               NS_TR "%6, %9 offset:1024\n\t" NS_TR "%7, %10 offset:1024\n\t" NS_RD "%2, %8 offset:4096\n\t" NS_RD "%3, %8 offset:5120\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]),
-                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1])
+__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[1][1][2]) {
+  asm volatile(NS_RD "%0, %6\n\t" NS_TR "%4, %7\n\t" NS_TR "%5, %8\n\t" NS_RD "%1, %6 offset:1024\n\t"
+               NS_RD "%2, %6 offset:4096\n\t" NS_RD "%3, %6 offset:5120\n\t" "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(b[0][0][0]), "=&v"(b[0][0][1])
                : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
 }
 
 // WI = 1: a tile is 128 rows x 256 columns, 4 waves side by side, 128 x 64 each (per K step 12 KB of LDS reads for 24 MFMAs; 64 x 64 need
 // a third more per MFMA); K steps of 16 through three stages: 72 KB, two workgroups per CU, whose epilogues run under each other's products.
-// WI = 2 (fewer tiles than that fills the chip with): 128 x 128, waves of 64 x 64.
+// WI = 2 (fewer tiles than that fills the chip with): 128 x 128, 8 waves of 64 x 32: with one workgroup on a CU, two waves to a SIMD, one
+// reads while the other multiplies.
 __device__ __forceinline__ void muon_update(const NsStep& s, long at, float keep, float step, float o) {
   const float p = s.p[at] * keep - step * o;
   s.p[at] = p;
   if (s.pb) s.pb[at] = (bf16_t)(ns_pack_bf16(p, 0.f) & 0xffffu);
 }
 template <int PX, int OUT, int WI>
-__global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr, int total, const ApplyK k) {
-  constexpr int AJ = 256 / WI, TM = 4 / WI, IPP = AJ / 32;           // IPP: transfers per plane of X
+__global__ __launch_bounds__(256 * WI, 2) void ns_apply_kernel(const NsGroup gr, int total, const ApplyK k) {
+  constexpr int AJ = 256 / WI, TM = 4 / WI, TN = 2 / WI, NW = 4 * WI, IPP = AJ / 32;      // IPP: transfers per plane of X
   constexpr int A_BYTES = AI * 2 * 32, B_BYTES = 16 * AJ * 2 * PX, STAGE = A_BYTES + B_BYTES, ST = 3;
-  constexpr int PA = A_BYTES / 4096, PB = B_BYTES / 4096, NI = PA + PB;
+  // transfers per wave; 128 columns of one plane keep only the first four waves busy
+  constexpr int PA = A_BYTES / 1024 / NW, PB = (B_BYTES / 1024 + NW - 1) / NW, NI = PA + PB;
+  constexpr bool HALF = B_BYTES / 1024 < NW;
   __shared__ __attribute__((aligned(1024))) char smem[ST * STAGE];
   const int bt = xcd_tile(blockIdx.x, total, 4);
   if (bt < 0) return;
@@ -823,12 +822,12 @@ __global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr,
   const _Float16* P = k.wsg + m.g + k.pbuf * 2 * pl;
   const _Float16* X = k.wsx + m.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = WI == 1 ? 0 : (wave >> 1) * 64, wn = WI == 1 ? wave * 64 : (wave & 1) * 64;
-  f32x16 acc[TM][2];
+  const int wm = WI == 1 ? 0 : (wave >> 2) * 64, wn = WI == 1 ? wave * 64 : (wave & 3) * 32;
+  f32x16 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   // P: 32 rows of a block per transfer; X: 16 rows of two blocks.  Rows and blocks behind the matrix read its last ones: products that
@@ -836,22 +835,25 @@ __global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr,
   const _Float16* as[PA];
 #pragma unroll
   for (int q = 0; q < PA; ++q) {
-    const int row = (q * 4 + wave) * 32 + (lane >> 1), plane = row / AI, lr = min(i0 + row - plane * AI, m.Mp - 1);
+    const int row = (q * NW + wave) * 32 + (lane >> 1), plane = row / AI, lr = min(i0 + row - plane * AI, m.Mp - 1);
     as[q] = P + plane * pl + (long)lr * 16 + ((lane & 1) ^ swz(row)) * 8;
   }
   const _Float16* bs[PB];
 #pragma unroll
   for (int q = 0; q < PB; ++q) {
-    const int x = q * 4 + wave, plane = x / IPP, blk = min((j0 >> 4) + x % IPP * 2 + (lane >> 5), m.Np / 16 - 1);
+    const int x = q * NW + wave, plane = x / IPP, blk = min((j0 >> 4) + x % IPP * 2 + (lane >> 5), m.Np / 16 - 1);
     const int kr = ((lane >> 1) & 15) ^ ((lane >> 5) << 2);
     bs[q] = X + plane * xpl + ((long)blk * (m.Mp + 8) + kr) * 16 + (lane & 1) * 8;
   }
   const long astep = 16L * (m.Mp + 8);
   auto issue = [&](int st) {
 #pragma unroll
-    for (int q = 0; q < PA; ++q) { dma16(as[q], smem + st * STAGE + (q * 4 + wave) * 1024); as[q] += astep; }
+    for (int q = 0; q < PA; ++q) { dma16(as[q], smem + st * STAGE + (q * NW + wave) * 1024); as[q] += astep; }
 #pragma unroll
-    for (int q = 0; q < PB; ++q) { dma16(bs[q], smem + st * STAGE + A_BYTES + (q * 4 + wave) * 1024); bs[q] += 256; }
+    for (int q = 0; q < PB; ++q) {
+      if (HALF && wave >= 4) break;
+      dma16(bs[q], smem + st * STAGE + A_BYTES + (q * NW + wave) * 1024); bs[q] += 256;
+    }
   };
   const unsigned lds0 = (unsigned)(size_t)smem;
   const int r4 = (lane >> 2) & 3, cq = lane & 3, mb = (lane >> 4) & 1, kh = lane >> 5;
@@ -862,23 +864,24 @@ __global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr,
   issue(1);
   int cur = 0, nxt = 2;
   for (int it = 0; it < n; ++it) {
-    if (it + 1 < n) wait_dma<NI>();
-    else wait_dma<0>();
+    if (it + 1 >= n) wait_dma<0>();
+    else if (HALF && wave >= 4) wait_dma<PA>();
+    else wait_dma<NI>();
     wg_barrier();
     if (it + 2 < n) issue(nxt);
     const unsigned so = (unsigned)(cur * STAGE);
     half8 a[2][TM];
-    half4 bq[PX][2][2];
+    half4 bq[PX][TN][2];
     fetch_apply(pa + so, pb0 + so, pb1 + so, a, bq);
-    half8 b[PX][2];
+    half8 b[PX][TN];
 #pragma unroll
     for (int p = 0; p < PX; ++p)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) b[p][j] = __builtin_shufflevector(bq[p][j][0], bq[p][j][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      for (int j = 0; j < TN; ++j) b[p][j] = __builtin_shufflevector(bq[p][j][0], bq[p][j][1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < TN; ++j) {
         // the transposed product: a lane holds one row of the result and runs of four of its columns
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[0][j], a[0][i], acc[i][j], 0, 0, 0);
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[0][j], a[1][i], acc[i][j], 0, 0, 0);
@@ -896,7 +899,7 @@ __global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr,
       const int gi = i0 + wm + i * 32 + (lane & 31);
       if (gi >= m.M) continue;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int gj = j0 + wn + j * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
@@ -911,21 +914,21 @@ __global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr,
   }
   // 32 rows per row of waves at a time through LDS (rows of AJ + 8 floats: both the writes and the reads meet every bank once): a wave then
   // handles whole rows, four neighbours per lane
-  constexpr int BS = AJ + 8, RP = 32 * WI, LR = AJ / 4;               // LR: lanes of a row
+  constexpr int BS = AJ + 8, RP = 32 * WI, LR = AJ / 4, NT = RP * LR / NW / 64;      // LR: lanes of a row; NT: runs of a lane
   float* buf = reinterpret_cast<float*>(smem);
   const int c = lane % LR * 4, gj = j0 + c;
   const long cbase = OUT == 3 && gj < m.N ? ns_at(m, 0, gj) : 0;
   // the row in the pass, and in the matrix, of a lane's t-th run
-  auto prow = [&](int t) { return wave * (RP / 4) + t * (64 / LR) + lane / LR; };
+  auto prow = [&](int t) { return wave * (RP / NW) + t * (64 / LR) + lane / LR; };
   auto mrow = [&](int i, int r) { return i0 + (r >> 5) * 64 + i * 32 + (r & 31); };
   const bool four = gj + 4 <= m.N && (OUT != 3 || (m.cols & 3) == 0);
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    float4 p[8];
+    float4 p[NT];
     if constexpr (OUT == 3) {
       if (four) {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
+        for (int t = 0; t < NT; ++t) {
           const int gi = mrow(i, prow(t));
           if (gi < m.M) {
             const NsU4 u = *reinterpret_cast<const NsU4*>(k.s.p + cbase + (long)gi * m.ld);
@@ -936,17 +939,17 @@ __global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr,
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<float4*>(buf + ((WI == 1 ? 0 : (wave >> 1) * 32) + (lane & 31)) * BS + wn + j * 32 + 8 * q + 4 * (lane >> 5)) =
+        *reinterpret_cast<float4*>(buf + ((WI == 1 ? 0 : (wave >> 2) * 32) + (lane & 31)) * BS + wn + j * 32 + 8 * q + 4 * (lane >> 5)) =
             make_float4(acc[i][j][4 * q] * f, acc[i][j][4 * q + 1] * f, acc[i][j][4 * q + 2] * f, acc[i][j][4 * q + 3] * f);
     __syncthreads();
     if constexpr (OUT == 0) {
       // planes: blocks of 32 rows, 1 KB each
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int k16 = t * 4 + wave, blk = k16 % (AJ / 16), row = k16 / (AJ / 16) * 32 + (lane >> 1), col = blk * 16 + (lane & 1) * 8;
+      for (int t = 0; t < RP / 32 * (AJ / 16) / NW; ++t) {
+        const int k16 = t * NW + wave, blk = k16 % (AJ / 16), row = k16 / (AJ / 16) * 32 + (lane >> 1), col = blk * 16 + (lane & 1) * 8;
         const int gi = mrow(i, row);
         if (gi >= m.Mp || j0 + col >= m.Np) continue;
         const float4 u = *reinterpret_cast<const float4*>(buf + row * BS + col), w = *reinterpret_cast<const float4*>(buf + row * BS + col + 4);
@@ -961,7 +964,7 @@ __global__ __launch_bounds__(256, WI + 1) void ns_apply_kernel(const NsGroup gr,
       continue;
     }
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
+    for (int t = 0; t < NT; ++t) {
       const int gi = mrow(i, prow(t));
       const float4 v = *reinterpret_cast<const float4*>(buf + prow(t) * BS + c);
       const float x[4] = {v.x, v.y, v.z, v.w};
@@ -1580,7 +1583,7 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
 #define NS_APPLY(PX, O)                                                                              \
   do {                                                                                               \
     if (wide) PG_KLAUNCH((ns_apply_kernel<PX, O, 1>), gd, blk, 0, st, gr, na, a);                    \
-    else PG_KLAUNCH((ns_apply_kernel<PX, O, 2>), gd, blk, 0, st, gr, na, a);                         \
+    else PG_KLAUNCH((ns_apply_kernel<PX, O, 2>), gd, dim3(512), 0, st, gr, na, a);                   \
   } while (0)
     if (one) {
       if (o == 0) NS_APPLY(1, 0);
