@@ -151,8 +151,8 @@ __global__ __launch_bounds__(256) void out_conv_dgrad_kernel(const OutDgradK p) 
     for (int u = 0; u < U; ++u) {
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
       if constexpr (DG) {
-        // packed fp32 FMAs (v_pk_fma_f32: two channels per instruction, the broadcast gradient value in both halves): the
-        // loop is VALU-bound (27 readlanes + 108 FMAs per pixel and wave), 54 packed instead of 108 scalar FMAs
+        // two channels per vector operation, the broadcast gradient value in both halves: the loop is VALU-bound (27 readlanes
+        // + 108 FMAs per pixel and wave); built without packed fp32 instructions, so 108 scalar FMAs
         typedef float f32x2 __attribute__((ext_vector_type(2)));
         f32x2 a01 = {0.f, 0.f}, a23 = {0.f, 0.f};
 #pragma unroll

@@ -520,7 +520,7 @@ __global__ __launch_bounds__(256) void warp_fwd5_kernel(const void* feat, const 
                                                         int T, int C, int h, int w, int H0, int W0, int align, void* out,
                                                         uint8_t* amax, int relu_out) {
   constexpr int V = 8;
-  typedef float f2 __attribute__((ext_vector_type(2)));        // v_pk_fma_f32: two channels per instruction
+  typedef float f2 __attribute__((ext_vector_type(2)));        // two channels per vector operation
   __shared__ Theta th[MAXT];
   extern __shared__ __attribute__((aligned(16))) char wsm[];
   float* xs_t = reinterpret_cast<float*>(wsm);                 // [w] normalised column coordinate, [h] row coordinate: the two
