@@ -40,7 +40,7 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int SG = 12, SP = 10;                 // log2 of the scales of G, Q, Q G and of P
 // elements per workgroup of the momentum / square-sum pass: small tensors give few workgroups, large ones many partial sums
 __host__ __device__ constexpr int k0_elems(long n) { return n < (1L << 21) ? 4096 : 16384; }
-constexpr int GT = 128, AI = 128;      // tiles: Gram; apply (rows)
+constexpr int GT = 128, AI = 128, AJ = 128;      // tiles: Gram; apply (rows, columns)
 
 struct NsMat {
   long src, ld, st;             // the caller's storage: element offset, row stride, tap stride
@@ -53,7 +53,7 @@ struct NsMat {
   long x, g, part;              // offsets in the workspace: X planes and chain planes (halves), Gram partials (floats)
   int sq0;                      // first partial sum of squares
 };
-enum { F_MOM, F_SPLIT, F_GRAM, F_JOIN, F_CHAIN, F_APPLY, F_APPLY2, F_N };       // launches (F_JOIN also: the chain's tiles of 32; apply: 256 or 128 columns)
+enum { F_MOM, F_SPLIT, F_GRAM, F_JOIN, F_CHAIN, F_APPLY, F_N };       // launches (F_JOIN also: the chain's tiles of 32)
 struct NsGroup {                // matrices of one call: a device table, or (tab = nullptr) `n` equal ones
   const NsMat* tab;
   const int* first;             // [F_N][n]: the first workgroup of each record
@@ -134,7 +134,8 @@ struct NsStep {
 __device__ __forceinline__ float ns_grad(const NsStep& s, long i) { return (s.gb ? bf2f(s.gb[i]) : s.g[i]) * s.gscale; }
 __device__ __forceinline__ float ns_update(const NsStep& s, float g, float m1) { return s.nesterov ? (1.f - s.mu) * g + s.mu * m1 : m1; }
 
-// one workgroup = k0_elems consecutive elements of a tensor; 28 bytes / element for Adam's, 12 for a matrix's
+// one workgroup = k0_elems consecutive elements of a tensor; 28 bytes / element for Adam's, 12 for a matrix's: HBM-bound (77 M elements of
+// 20 matrices: 177 us, 5.2 TB/s; 2.8 M: 12 us)
 __global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, const NsStep s, double* sq) {
   __shared__ double red[4];
   const NsRef r = ns_find<F_MOM>(gr, blockIdx.x);
@@ -293,7 +294,8 @@ __device__ __forceinline__ float ns_factor(double sumsq, int k, float eps) {
   return sumsq == 0.0 ? 0.f : (float)((double)ns_pow2(k) / (sqrt(sumsq) + (double)eps));
 }
 // every workgroup joins its matrix's partial sums of squares itself (a few hundred doubles); the first one publishes
-// c = 2^k / (|U| + eps), the factor from the planes' units to X0's
+// c = 2^k / (|U| + eps), the factor from the planes' units to X0's.  12 bytes / element from fp32 pairs (m', g), HBM-bound: 211 us for 77 M
+// elements (4.4 TB/s); 14 us for 512 x 24576 bf16 (6 bytes)
 template <int SRC>
 __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const void* x, const NsStep s, const double* sq, float eps,
                                                        float* cfac, _Float16* ws) {
@@ -503,7 +505,10 @@ __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
   bj = t - i * (i + 1) / 2;
 }
 
-// G = X X^T over one slice of the long side: fp32 partial tiles, in the order of the accumulators (one float4 = four rows of a column)
+// G = X X^T over one slice of the long side: fp32 partial tiles, in the order of the accumulators (one float4 = four rows of a column).
+// 128 x 128 tiles of the lower triangle, two workgroups per CU; the long side in as many slices as run at once.  The generator's 20 matrices (up to
+// 512 x 24576) take 201 - 212 us, 512 x 24576 alone 29 us (two planes) and 16 us (bf16: one): MFMA-bound with operands from L2.  Where few slices run (16 x
+// 770 x 189: 144 workgroups, 11 - 13 us) it is launch, first transfer and the partial tiles' way out; more stages or slices gave nothing.
 template <int PL>
 __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int total, const _Float16* ws, float* part) {
   typedef NtCore<GT, PL, 2> Core;
@@ -532,7 +537,8 @@ __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int t
             make_float4(c.acc[i][j][4 * q], c.acc[i][j][4 * q + 1], c.acc[i][j][4 * q + 2], c.acc[i][j][4 * q + 3]);
 }
 
-// join of the slices, in order; both triangles of G from the lower one.  One workgroup = one 32 x 32 block, a float4 per thread
+// join of the slices, in order; both triangles of G from the lower one.  One workgroup = one 32 x 32 block, a float4 per thread: 4 - 6 us, mostly
+// launch (12 us for the generator's 20 matrices)
 __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, const float* part, const float* cfac, float cconst, _Float16* ws) {
   const NsRef r = ns_find<F_JOIN>(gr, blockIdx.x);
   const NsMat& m = r.m;
@@ -576,7 +582,8 @@ __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, con
 // C = A B of commuting symmetric matrices: the lower triangle of 64 x 64 tiles, mirrored.  `quad`: C = a I + b A + c A A
 struct ChainJob { int a, b, c; float mul; int quad; };
 
-// Tiles of 64 x 64 (many matrices): four stages of 16 KB, two workgroups per CU.  The result leaves through LDS: written four
+// Tiles of 64 x 64 (many matrices): four stages of 16 KB, two workgroups per CU; 17 - 19 us for 472
+// tiles of 64 .. 512 columns (32 x 32 tiles: 22 - 23 us; a launch of two jobs 31 and 38 us).  The result leaves through LDS: written four
 // neighbours at a time as the mirrored tile, which is copied out as it is and, by transposing reads, turned.
 __global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
   typedef NtCore<64, 2, 4> Core;
@@ -643,7 +650,8 @@ __global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, Chai
 
 // Tiles of 32 x 32 (few matrices: at most two per CU).  Such a product is latency alone: launch, one round of transfers, a few dependent
 // MFMAs.  A workgroup brings the whole of its rows (KC columns at a time, 128 KB for 512) in one go; each of its 4 waves moves and
-// multiplies every fourth block, with no barrier before the sums are joined.
+// multiplies every fourth block, with no barrier before the sums are joined.  4.5 - 6 us for one 512 x 512 product
+// (136 tiles; 64 x 64 tiles: 8.2 - 10 us).
 template <int KC>
 __global__ __launch_bounds__(256) void ns_chain32_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
   constexpr int NB = KC / 64;                        // blocks per wave and round
@@ -754,59 +762,37 @@ struct ApplyK {
   void* out; long ldo;
   NsStep s;
 };
-// one K step of the apply product: 4 fragments of 32 rows of P; X (K step = 16 of its rows, [column / 16][16 rows][16]) through the
+// one K step of the apply product: 2 fragments of 32 rows of P, one of 32 columns of X; X (K step = 16 of its rows, [column / 16][16 rows][16]) through the
 // transposing read: in a group of 16 lanes lane 4 r + c gives the address of four columns of row r and gets one column of four
 // rows; two of them make a fragment.  Odd blocks hold their rows in the order 4..7 0..3 12..15 8..11, so that the two blocks a
 // 32-lane half reads lie in different banks: the second read's address is the first one's ^ 128.
 #define NS_TR "ds_read_b64_tr_b16 "
-__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][4], half4 (&b)[2][2][2]) {
-  asm volatile(NS_RD "%0, %16\n\t" NS_TR "%8, %17\n\t" NS_TR "%9, %18\n\t" NS_RD "%1, %16 offset:1024\n\t"
-               NS_TR "%10, %17 offset:1024\n\t" NS_TR "%11, %18 offset:1024\n\t" NS_RD "%2, %16 offset:2048\n\t" NS_RD "%3, %16 offset:3072\n\t"
-               NS_RD "%4, %16 offset:4096\n\t" NS_RD "%5, %16 offset:5120\n\t" NS_RD "%6, %16 offset:6144\n\t" NS_RD "%7, %16 offset:7168\n\t"
-               NS_TR "%12, %17 offset:8192\n\t" NS_TR "%13, %18 offset:8192\n\t" NS_TR "%14, %17 offset:9216\n\t" NS_TR "%15, %18 offset:9216\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[0][2]), "=&v"(a[0][3]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(a[1][2]), "=&v"(a[1][3]),
-                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1]),
-                 "=&v"(b[1][0][0]), "=&v"(b[1][0][1]), "=&v"(b[1][1][0]), "=&v"(b[1][1][1])
-               : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
-}
-__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][4], half4 (&b)[1][2][2]) {
-  asm volatile(NS_RD "%0, %12\n\t" NS_TR "%8, %13\n\t" NS_TR "%9, %14\n\t" NS_RD "%1, %12 offset:1024\n\t"
-               NS_TR "%10, %13 offset:1024\n\t" NS_TR "%11, %14 offset:1024\n\t" NS_RD "%2, %12 offset:2048\n\t" NS_RD "%3, %12 offset:3072\n\t"
-               NS_RD "%4, %12 offset:4096\n\t" NS_RD "%5, %12 offset:5120\n\t" NS_RD "%6, %12 offset:6144\n\t" NS_RD "%7, %12 offset:7168\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[0][2]), "=&v"(a[0][3]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(a[1][2]), "=&v"(a[1][3]),
-                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1])
-               : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
-}
-
-__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[2][1][2]) {
+__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[2][2]) {
   asm volatile(NS_RD "%0, %8\n\t" NS_TR "%4, %9\n\t" NS_TR "%5, %10\n\t" NS_RD "%1, %8 offset:1024\n\t"
                NS_RD "%2, %8 offset:4096\n\t" NS_RD "%3, %8 offset:5120\n\t" NS_TR "%6, %9 offset:4096\n\t" NS_TR "%7, %10 offset:4096\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]),
-                 "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[1][0][0]), "=&v"(b[1][0][1])
+                 "=&v"(b[0][0]), "=&v"(b[0][1]), "=&v"(b[1][0]), "=&v"(b[1][1])
                : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
 }
-__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[1][1][2]) {
+__device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned pb1, half8 (&a)[2][2], half4 (&b)[1][2]) {
   asm volatile(NS_RD "%0, %6\n\t" NS_TR "%4, %7\n\t" NS_TR "%5, %8\n\t" NS_RD "%1, %6 offset:1024\n\t"
                NS_RD "%2, %6 offset:4096\n\t" NS_RD "%3, %6 offset:5120\n\t" "s_waitcnt lgkmcnt(0)"
-               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(b[0][0][0]), "=&v"(b[0][0][1])
+               : "=&v"(a[0][0]), "=&v"(a[0][1]), "=&v"(a[1][0]), "=&v"(a[1][1]), "=&v"(b[0][0]), "=&v"(b[0][1])
                : "v"(pa), "v"(pb0), "v"(pb1) : "memory");
 }
 
-// WI = 1: a tile is 128 rows x 256 columns, 4 waves side by side, 128 x 64 each (per K step 12 KB of LDS reads for 24 MFMAs; 64 x 64 need
-// a third more per MFMA); K steps of 16 through three stages: 72 KB, two workgroups per CU, whose epilogues run under each other's products.
-// WI = 2 (fewer tiles than that fills the chip with): 128 x 128, 8 waves of 64 x 32: with one workgroup on a CU, two waves to a SIMD, one
-// reads while the other multiplies.
+// A tile is 128 rows x 128 columns, 8 waves (2 x 4) of 64 x 32; K steps of 16 through three stages: 48 KB, three workgroups per CU, so that reads,
+// products and epilogues of different waves run under each other.  MFMA- and power-bound: 312 and 320 us for the generator's two
+// products (128 x 256 tiles, 4 waves of 128 x 64: 302 and 331 us), 512 x 24576 36 us (bf16 X) and 44 us (37 and 47 us), the discriminator's 17 and 18 us (29 and 35 us: 88 tiles).
 __device__ __forceinline__ void muon_update(const NsStep& s, long at, float keep, float step, float o) {
   const float p = s.p[at] * keep - step * o;
   s.p[at] = p;
   if (s.pb) s.pb[at] = (bf16_t)(ns_pack_bf16(p, 0.f) & 0xffffu);
 }
-template <int PX, int OUT, int WI>
-__global__ __launch_bounds__(256 * WI, 2) void ns_apply_kernel(const NsGroup gr, int total, const ApplyK k) {
-  constexpr int AJ = 256 / WI, TM = 4 / WI, TN = 2 / WI, NW = 4 * WI, IPP = AJ / 32;      // IPP: transfers per plane of X
+template <int PX, int OUT>
+__global__ __launch_bounds__(512, 2) void ns_apply_kernel(const NsGroup gr, int total, const ApplyK k) {
+  constexpr int TM = 2, NW = 8, IPP = AJ / 32;      // IPP: transfers per plane of X
   constexpr int A_BYTES = AI * 2 * 32, B_BYTES = 16 * AJ * 2 * PX, STAGE = A_BYTES + B_BYTES, ST = 3;
   // transfers per wave; 128 columns of one plane keep only the first four waves busy
   constexpr int PA = A_BYTES / 1024 / NW, PB = (B_BYTES / 1024 + NW - 1) / NW, NI = PA + PB;
@@ -814,7 +800,7 @@ __global__ __launch_bounds__(256 * WI, 2) void ns_apply_kernel(const NsGroup gr,
   __shared__ __attribute__((aligned(1024))) char smem[ST * STAGE];
   const int bt = xcd_tile(blockIdx.x, total, 4);
   if (bt < 0) return;
-  const NsRef r = ns_find<WI == 1 ? F_APPLY : F_APPLY2>(gr, bt);
+  const NsRef r = ns_find<F_APPLY>(gr, bt);
   const NsMat& m = r.m;
   const int ti = (m.Mp + AI - 1) / AI;
   const int i0 = (r.tile % ti) * AI, j0 = (r.tile / ti) * AJ;
@@ -822,14 +808,12 @@ __global__ __launch_bounds__(256 * WI, 2) void ns_apply_kernel(const NsGroup gr,
   const _Float16* P = k.wsg + m.g + k.pbuf * 2 * pl;
   const _Float16* X = k.wsx + m.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = WI == 1 ? 0 : (wave >> 2) * 64, wn = WI == 1 ? wave * 64 : (wave & 3) * 32;
-  f32x16 acc[TM][TN];
+  const int wm = (wave >> 2) * 64, wn = (wave & 3) * 32;
+  f32x16 acc[TM];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
   // P: 32 rows of a block per transfer; X: 16 rows of two blocks.  Rows and blocks behind the matrix read its last ones: products that
   // nobody stores.
   const _Float16* as[PA];
@@ -871,22 +855,18 @@ __global__ __launch_bounds__(256 * WI, 2) void ns_apply_kernel(const NsGroup gr,
     if (it + 2 < n) issue(nxt);
     const unsigned so = (unsigned)(cur * STAGE);
     half8 a[2][TM];
-    half4 bq[PX][TN][2];
+    half4 bq[PX][2];
     fetch_apply(pa + so, pb0 + so, pb1 + so, a, bq);
-    half8 b[PX][TN];
+    half8 b[PX];
 #pragma unroll
-    for (int p = 0; p < PX; ++p)
+    for (int p = 0; p < PX; ++p) b[p] = __builtin_shufflevector(bq[p][0], bq[p][1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) b[p][j] = __builtin_shufflevector(bq[p][j][0], bq[p][j][1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        // the transposed product: a lane holds one row of the result and runs of four of its columns
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[0][j], a[0][i], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[0][j], a[1][i], acc[i][j], 0, 0, 0);
-        if constexpr (PX == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[1][j], a[0][i], acc[i][j], 0, 0, 0);
-      }
+    for (int i = 0; i < TM; ++i) {
+      // the transposed product: a lane holds one row of the result and runs of four of its columns
+      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[0], a[0][i], acc[i], 0, 0, 0);
+      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[0], a[1][i], acc[i], 0, 0, 0);
+      if constexpr (PX == 2) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[1], a[0][i], acc[i], 0, 0, 0);
+    }
     cur = cur == ST - 1 ? 0 : cur + 1;
     nxt = nxt == ST - 1 ? 0 : nxt + 1;
   }
@@ -899,22 +879,20 @@ __global__ __launch_bounds__(256 * WI, 2) void ns_apply_kernel(const NsGroup gr,
       const int gi = i0 + wm + i * 32 + (lane & 31);
       if (gi >= m.M) continue;
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int gj = j0 + wn + j * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-          if (gj >= m.N) continue;
-          const float v = acc[i][j][e] * f;
-          if constexpr (OUT == 1) reinterpret_cast<float*>(k.out)[r.out + (long)gj * k.ldo + gi] = v;
-          else if constexpr (OUT == 2) reinterpret_cast<bf16_t*>(k.out)[r.out + (long)gj * k.ldo + gi] = (bf16_t)(ns_pack_bf16(v, 0.f) & 0xffffu);
-          else muon_update(k.s, ns_at(m, gj, gi), keep, step, v);
-        }
+      for (int e = 0; e < 16; ++e) {
+        const int gj = j0 + wn + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        if (gj >= m.N) continue;
+        const float v = acc[i][e] * f;
+        if constexpr (OUT == 1) reinterpret_cast<float*>(k.out)[r.out + (long)gj * k.ldo + gi] = v;
+        else if constexpr (OUT == 2) reinterpret_cast<bf16_t*>(k.out)[r.out + (long)gj * k.ldo + gi] = (bf16_t)(ns_pack_bf16(v, 0.f) & 0xffffu);
+        else muon_update(k.s, ns_at(m, gj, gi), keep, step, v);
+      }
     }
     return;
   }
   // 32 rows per row of waves at a time through LDS (rows of AJ + 8 floats: both the writes and the reads meet every bank once): a wave then
   // handles whole rows, four neighbours per lane
-  constexpr int BS = AJ + 8, RP = 32 * WI, LR = AJ / 4, NT = RP * LR / NW / 64;      // LR: lanes of a row; NT: runs of a lane
+  constexpr int BS = AJ + 8, RP = 64, LR = AJ / 4, NT = RP * LR / NW / 64;      // LR: lanes of a row; NT: runs of a lane
   float* buf = reinterpret_cast<float*>(smem);
   const int c = lane % LR * 4, gj = j0 + c;
   const long cbase = OUT == 3 && gj < m.N ? ns_at(m, 0, gj) : 0;
@@ -939,11 +917,9 @@ __global__ __launch_bounds__(256 * WI, 2) void ns_apply_kernel(const NsGroup gr,
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<float4*>(buf + ((WI == 1 ? 0 : (wave >> 2) * 32) + (lane & 31)) * BS + wn + j * 32 + 8 * q + 4 * (lane >> 5)) =
-            make_float4(acc[i][j][4 * q] * f, acc[i][j][4 * q + 1] * f, acc[i][j][4 * q + 2] * f, acc[i][j][4 * q + 3] * f);
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<float4*>(buf + ((wave >> 2) * 32 + (lane & 31)) * BS + wn + 8 * q + 4 * (lane >> 5)) =
+          make_float4(acc[i][4 * q] * f, acc[i][4 * q + 1] * f, acc[i][4 * q + 2] * f, acc[i][4 * q + 3] * f);
     __syncthreads();
     if constexpr (OUT == 0) {
       // planes: blocks of 32 rows, 1 KB each
@@ -1405,8 +1381,7 @@ static NsCounts ns_counts(NsMat& m, long ks, bool flat) {
   const long n64 = m.Mp / 64, n32 = m.Mp / 32;
   c.n[F_CHAIN] = n64 * (n64 + 1) / 2;
   c.n[F_JOIN] = n32 * (n32 + 1) / 2;
-  c.n[F_APPLY] = (long)cdiv(m.Mp, AI) * cdiv(m.Np, 256);
-  c.n[F_APPLY2] = (long)cdiv(m.Mp, AI) * cdiv(m.Np, 128);
+  c.n[F_APPLY] = (long)cdiv(m.Mp, AI) * cdiv(m.Np, AJ);
   c.x = 2L * m.Np * (m.Mp + 8);
   c.g = 10L * m.Mp * (m.Mp + 8);
   c.part = c.n[F_GRAM] * GT * GT;
@@ -1507,7 +1482,6 @@ static const char* ns_plan_table(NsPlan& pl, const pg_muon_entry_t* e, int n) {
   return nullptr;
 }
 
-constexpr long APPLY_FEW = 256;
 struct NsSource { int kind; const void* x; };      // kind: ns_elem's SRC
 
 // everything behind the sums of squares.  out_kind: ns_apply_kernel's OUT of the last product
@@ -1577,14 +1551,9 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     a.mul = (float)ldexp(1.0, -psc) * (last ? 1.f : sx);
     a.out = out; a.ldo = ldo; a.s = step;
     const int o = last ? out_kind : 0;
-    const bool wide = pl.n[F_APPLY] > APPLY_FEW;
-    const int na = (int)pl.n[wide ? F_APPLY : F_APPLY2];
+    const int na = (int)pl.n[F_APPLY];
     const dim3 gd((unsigned)up(na, 8));
-#define NS_APPLY(PX, O)                                                                              \
-  do {                                                                                               \
-    if (wide) PG_KLAUNCH((ns_apply_kernel<PX, O, 1>), gd, blk, 0, st, gr, na, a);                    \
-    else PG_KLAUNCH((ns_apply_kernel<PX, O, 2>), gd, dim3(512), 0, st, gr, na, a);                   \
-  } while (0)
+#define NS_APPLY(PX, O) PG_KLAUNCH((ns_apply_kernel<PX, O>), gd, dim3(512), 0, st, gr, na, a)
     if (one) {
       if (o == 0) NS_APPLY(1, 0);
       else if (o == 1) NS_APPLY(1, 1);
