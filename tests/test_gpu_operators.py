@@ -417,6 +417,29 @@ def test_operators_in_a_captured_graph():
         assert bool(torch.isfinite(junk).all())
 
 
+def test_two_streams_at_once():
+    """calls on two streams side by side, each with workspaces of its own: what each gets alone"""
+    O = ops()
+    a, b = rnd(90, 3, 200, 900), rnd(91, 2, 130, 2000, dtype=torch.bfloat16)
+    dy, h = rnd(92, 5000, 129), rnd(93, 5000, 129)
+    g, rstd = rnd(94, 129), torch.ones(5000, device="cuda")
+    want_a, want_b, want_n = O.orthogonalise(a), O.orthogonalise(b), O.rms_norm_bwd(dy, h, rstd, g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(8):
+        with torch.cuda.stream(streams[0]):
+            got.append((O.orthogonalise(a), want_a))
+            got.append((O.rms_norm_bwd(dy, h, rstd, g)[1], want_n[1]))
+        with torch.cuda.stream(streams[1]):
+            got.append((O.rms_norm_bwd(dy, h, rstd, g)[0], want_n[0]))
+            got.append((O.orthogonalise(b), want_b))
+    torch.cuda.synchronize()
+    for x, y in got:
+        assert torch.equal(x, y)
+
+
 # ------------------------------------------------------------------------------------------------ module and trainer
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rms_norm_module(dtype):
