@@ -699,7 +699,7 @@ __global__ __launch_bounds__(256) void ns_chain32_kernel(const NsGroup gr, Chain
       dma16(pa, base + u * 4096);
       dma16(pa + pl, base + u * 4096 + 1024);
       dma16(pb, base + u * 4096 + 2048);
-      dma16(pb + pl, base + u * 4096 + 3072);
+      dma16(pb + pl, base + u * 4096 + 3 * 1024);
       pa += step; pb += step;
     }
     __builtin_amdgcn_sched_barrier(0);
