@@ -14,9 +14,13 @@
 //
 // Arithmetic.  The matrix cores have no fast fp32 form (1 / 16 of the fp16 rate).  Every operand is held as TWO fp16 values, hi + lo =
 // 22 bits, scaled by a power of two; a product is three MFMAs, hi hi + hi lo + lo hi, with fp32 accumulation: what an fp32 product
-// gives (measured 4.8e-6 against 4.7e-6 through five steps; a bf16 pair with its 16 bits: 4e-5, single bf16 operands: 2e-2).  X0's
-// scale makes its rms 1/2 .. 1: its largest element is then at most sqrt(rows cols) <= 2^15.5, the loss of a tiny one's last bits
-// is 2^-25 of the rms.  |G|, |Q G| <= 1.5, |Q| <= 3.45, |P| <= 3.45^3 = 41 bound the others' scales.  A bf16 input is one fp16 value exactly (8 bits): one plane.
+// gives (measured 4.8e-6 against 4.7e-6 through five steps; a bf16 pair with its 16 bits: 4e-5, single bf16 operands: 2e-2).
+// fp16 has few exponents: below 2^-3 of a plane's unit the pair loses bits, its error is then 2^-25 absolute.  So every plane's largest value
+// lies near fp16's end: X0's largest element at 2^14 .. 2^15; |G|, |Q G| <= 1.5, |Q| <= 3.45 and |P| <= 3.45^3 = 41 bound the others.
+// Elements keep 22 bits down to 2^-18 of the largest and 2^-40 of it behind that.  A row that is a fraction r of the others comes out
+// with an error of about max(1e-6, 5e-11 / r) of itself (128 x 1152: 7e-7 at r = 1e-4, 6e-6 at 1e-5, 5e-5 at 1e-6; the limit is
+// 2^-40 in G); fp32 products keep 1e-6.  With the mean square at 1 instead of the largest element at 2^14: 1.7e-4, 1.8e-3, 1.7e-2.
+// A bf16 input (8 bits) is one fp16 value exactly down to 2^-32 of the largest, behind that to 2^-40 of it: one plane.
 //
 // Layout.  A matrix is stored by the caller as [taps][rows][cols] with row and tap strides (a packed convolution weight is one matrix
 // [rows, taps * cols]).  The planes here are M x N, M <= N the short side, both padded with zeros to multiples of 64: no product checks
@@ -37,9 +41,11 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
-constexpr int SG = 12, SP = 10;                 // log2 of the scales of G, Q, Q G and of P
+constexpr int SG = 15, SQ = 14, SP = 10;        // log2 of the scales of G and Q G, of Q, of P
 // elements per workgroup of the momentum / square-sum pass: small tensors give few workgroups, large ones many partial sums
 __host__ __device__ constexpr int k0_elems(long n) { return n < (1L << 21) ? 4096 : 16384; }
+// Q = a I + b G + c G G in the planes' units
+constexpr float QUAD_A = NS_A * (float)(1 << SQ), QUAD_B = NS_B / (float)(1 << (SG - SQ)), QUAD_C = NS_C / (float)(1 << (2 * SG - SQ));
 constexpr int GT = 128, AI = 128, AJ = 128;      // tiles: Gram; apply (rows, columns)
 
 struct NsMat {
@@ -49,7 +55,6 @@ struct NsMat {
   int ks, kc;                   // Gram: splits of the long side and their length (a multiple of 32)
   int np;                       // partial sums of squares
   float scale;
-  double inv;                   // 1 / number of elements
   long x, g, part;              // offsets in the workspace: X planes and chain planes (halves), Gram partials (floats)
   int sq0;                      // first partial sum of squares
 };
@@ -103,12 +108,20 @@ __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
 }
-__device__ __forceinline__ double block_sum_d256(double v, double* red) {
-  v = wave_sum_d(v);
+// sum of squares and largest magnitude of some elements of a matrix (a NaN shows in the sum)
+struct NsNorm { double sum; float top; int _pad; };
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ NsNorm block_norm256(double sum, float top, NsNorm* red) {
+  sum = wave_sum_d(sum);
+  top = wave_max(top);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6].sum = sum; red[threadIdx.x >> 6].top = top; }
   __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
+  return {red[0].sum + red[1].sum + red[2].sum + red[3].sum, fmaxf(fmaxf(red[0].top, red[1].top), fmaxf(red[2].top, red[3].top)), 0};
 }
 
 // ---------------------------------------------------------------------------------------------- table upload
@@ -136,8 +149,9 @@ __device__ __forceinline__ float ns_update(const NsStep& s, float g, float m1) {
 
 // one workgroup = k0_elems consecutive elements of a tensor; 28 bytes / element for Adam's, 12 for a matrix's: HBM-bound (77 M elements of
 // 20 matrices: 177 us, 5.2 TB/s; 2.8 M: 12 us)
-__global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, const NsStep s, double* sq) {
-  __shared__ double red[4];
+__global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, const NsStep s, NsNorm* sq) {
+  __shared__ NsNorm red[4];
+  __shared__ double bc[2];
   const NsRef r = ns_find<F_MOM>(gr, blockIdx.x);
   const long n = (long)r.m.taps * r.m.rows * r.m.cols;
   const long e0 = (long)r.tile * k0_elems(n), e1 = min(n, e0 + k0_elems(n));
@@ -145,11 +159,11 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, co
   if (r.m.kind == 1) {
     if (threadIdx.x < 2) {                             // 1 - beta^t, in fp64, by one lane each
       const double t = (double)(s.step0 + (s.ctr ? (long)s.ctr[0] : 0L));
-      red[threadIdx.x] = 1.0 - pow(threadIdx.x ? s.b2d : s.b1d, t);
+      bc[threadIdx.x] = 1.0 - pow(threadIdx.x ? s.b2d : s.b1d, t);
     }
     __syncthreads();
-    const float step_size = (float)((double)s.lr / red[0]);
-    const float bc2 = (float)sqrt(red[1]);
+    const float step_size = (float)((double)s.lr / bc[0]);
+    const float bc2 = (float)sqrt(bc[1]);
 #pragma unroll 4
     for (long i = e0 + threadIdx.x; i < e1; i += 256) {
       const float g = ns_grad(s, base + i);
@@ -162,6 +176,7 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, co
     return;
   }
   double acc = 0.0;
+  float top = 0.f;
   const bool vec = ((base | n) & 3) == 0;
   if (vec) {
 #pragma unroll 4
@@ -181,8 +196,9 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, co
       for (int e = 0; e < 4; ++e) {
         const float gg = g[e] * s.gscale;
         m[e] = s.mu * m[e] + (1.f - s.mu) * gg;
-        const double u = (double)ns_update(s, gg, m[e]);
-        acc = fma(u, u, acc);
+        const float u = ns_update(s, gg, m[e]);
+        acc = fma((double)u, (double)u, acc);
+        top = fmaxf(top, fabsf(u));
       }
       *reinterpret_cast<float4*>(s.m + base + i) = make_float4(m[0], m[1], m[2], m[3]);
     }
@@ -191,12 +207,13 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, co
       const float gg = ns_grad(s, base + i);
       const float m = s.mu * s.m[base + i] + (1.f - s.mu) * gg;
       s.m[base + i] = m;
-      const double u = (double)ns_update(s, gg, m);
-      acc = fma(u, u, acc);
+      const float u = ns_update(s, gg, m);
+      acc = fma((double)u, (double)u, acc);
+      top = fmaxf(top, fabsf(u));
     }
   }
-  acc = block_sum_d256(acc, red);
-  if (threadIdx.x == 0) sq[blockIdx.x] = acc;
+  const NsNorm n4 = block_norm256(acc, top, red);
+  if (threadIdx.x == 0) sq[blockIdx.x] = n4;
 }
 
 // the stored element (row, flat column = tap * cols + col) of a matrix that is orthogonalised
@@ -257,23 +274,24 @@ __device__ __forceinline__ void ns_load8(const NsMat& m, const void* x, const Ns
 // one workgroup = 512 runs of eight stored neighbours
 constexpr int SQ_RUNS = 512;
 template <int SRC>
-__global__ __launch_bounds__(256) void ns_sumsq_kernel(const NsGroup gr, const void* x, double* sq) {
-  __shared__ double red[4];
+__global__ __launch_bounds__(256) void ns_sumsq_kernel(const NsGroup gr, const void* x, NsNorm* sq) {
+  __shared__ NsNorm red[4];
   const NsRef r = ns_find<F_MOM>(gr, blockIdx.x);
   const unsigned rpr = (unsigned)(r.m.cols + 7) / 8u;
   const unsigned n = (unsigned)r.m.rows * rpr;
   const unsigned e0 = (unsigned)r.tile * SQ_RUNS, e1 = min(n, e0 + SQ_RUNS);
   double acc = 0.0;
+  float top = 0.f;
   const NsStep s{};
   for (unsigned i = e0 + threadIdx.x; i < e1; i += 256) {
     const unsigned row = i / rpr;
     float v[8];
     ns_load8<SRC>(r.m, x, s, (int)row, (int)(i - row * rpr) * 8, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc = fma((double)v[e], (double)v[e], acc);
+    for (int e = 0; e < 8; ++e) { acc = fma((double)v[e], (double)v[e], acc); top = fmaxf(top, fabsf(v[e])); }
   }
-  acc = block_sum_d256(acc, red);
-  if (threadIdx.x == 0) sq[blockIdx.x] = acc;
+  const NsNorm n4 = block_norm256(acc, top, red);
+  if (threadIdx.x == 0) sq[blockIdx.x] = n4;
 }
 
 // element (i, j) of a plane in blocks of 16 columns; planes of X and of an m x m matrix
@@ -282,11 +300,9 @@ __device__ __forceinline__ long xplane(const NsMat& m) { return (long)m.Np * (m.
 __device__ __forceinline__ long cplane(const NsMat& m) { return (long)m.Mp * (m.Mp + 8); }
 
 // ---------------------------------------------------------------------------------------------- split into fp16 planes
-// planes hold 2^-k U with an rms in 2^-1 .. 1: the largest element, at most sqrt(n) rms <= 2^15.5, fits fp16.  k from the exponent of the
-// mean square alone: every thread of every workgroup needs it (with log2 and a square root in fp64 it took 2 us)
-__device__ __forceinline__ int ns_exponent(double sumsq, double inv) {
-  const int e = (int)((__double_as_longlong(sumsq * inv) >> 52) & 0x7ff) - 1023;      // 2^e <= mean square < 2^(e + 1)
-  return max(-126, min(126, (e + 2) >> 1));
+// planes hold 2^-k U with a largest element of 2^14 .. 2^15 (as far as k goes: an infinity makes the planes infinite)
+__device__ __forceinline__ int ns_exponent(float top) {
+  return max(-126, min(126, (int)((__float_as_uint(top) >> 23) & 0xff) - 127 - 14));
 }
 __device__ __forceinline__ float ns_pow2(int k) { return __uint_as_float((unsigned)(k + 127) << 23); }      // |k| <= 126
 // 2^k / (|U| + eps): from the planes' units to X0's
@@ -297,9 +313,9 @@ __device__ __forceinline__ float ns_factor(double sumsq, int k, float eps) {
 // c = 2^k / (|U| + eps), the factor from the planes' units to X0's.  12 bytes / element from fp32 pairs (m', g), HBM-bound: 211 us for 77 M
 // elements (4.4 TB/s); 14 us for 512 x 24576 bf16 (6 bytes)
 template <int SRC>
-__global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const void* x, const NsStep s, const double* sq, float eps,
+__global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const void* x, const NsStep s, const NsNorm* sq, float eps,
                                                        float* cfac, _Float16* ws) {
-  __shared__ double red[4];
+  __shared__ NsNorm red[4];
   __shared__ float tile[64][65];
   constexpr bool ONE = SRC == 1;
   const NsRef r = ns_find<F_SPLIT>(gr, blockIdx.x);
@@ -332,11 +348,12 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
     }
   }
   double a = 0.0;
-  for (int i = threadIdx.x; i < np; i += 256) a += sq[first + i];
-  a = block_sum_d256(a, red);
-  const int k = ns_exponent(a, m.inv);
+  float top = 0.f;
+  for (int i = threadIdx.x; i < np; i += 256) { a += sq[first + i].sum; top = fmaxf(top, sq[first + i].top); }
+  const NsNorm nm = block_norm256(a, top, red);
+  const int k = ns_exponent(nm.top);
   const float f = ns_pow2(-k);
-  if (r.tile == 0 && threadIdx.x == 0) cfac[r.id] = ns_factor(a, k, eps);
+  if (r.tile == 0 && threadIdx.x == 0) cfac[r.id] = ns_factor(nm.sum, k, eps);
   _Float16* hi = ws + m.x;
   _Float16* lo = hi + xplane(m);
   if (!m.tall) {
@@ -619,8 +636,8 @@ __global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, Chai
       const half4 h = *reinterpret_cast<const half4*>(A + at), l = *reinterpret_cast<const half4*>(A + pl + at);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[e] += NS_B * ((float)h[e] + (float)l[e]);
-        if (diag && i + e == j) v[e] += NS_A * (float)(1 << SG);
+        v[e] += QUAD_B * ((float)h[e] + (float)l[e]);
+        if (diag && i + e == j) v[e] += QUAD_A;
       }
     }
     half4 hh, ll;
@@ -742,7 +759,7 @@ __global__ __launch_bounds__(256) void ns_chain32_kernel(const NsGroup gr, Chain
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     v[e] *= jb.mul;
-    if (jb.quad) v[e] += NS_B * ((float)gh[e] + (float)gl[e]) + (gi + e == gj ? NS_A * (float)(1 << SG) : 0.f);
+    if (jb.quad) v[e] += QUAD_B * ((float)gh[e] + (float)gl[e]) + (gi + e == gj ? QUAD_A : 0.f);
     _Float16 h, l;
     split16(v[e], h, l);
     hh[e] = h; ll[e] = l;
@@ -1030,18 +1047,18 @@ struct SmallChain {
     f32x16 q = mul(buf, buf);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      q[e] = q[e] * (NS_C / (float)(1 << SG)) + NS_B * g[e];
-      if (wi == wj && 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31)) q[e] += NS_A * (float)(1 << SG);
+      q[e] = q[e] * QUAD_C + QUAD_B * g[e];
+      if (wi == wj && 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31)) q[e] += QUAD_A;
     }
     return q;
   }
-  static __device__ __forceinline__ float pscale(int k) { return 1.f / (float)(1 << (k == 1 ? 2 * SG - SP : SG)); }
+  static __device__ __forceinline__ float pscale(int k) { return 1.f / (float)(1 << (k == 1 ? 2 * SQ - SP : SQ)); }
 
-  // g: this wave's block of G (scale 2^SG).  Returns its block of P, scale 2^(steps > 1 ? SP : SG).  Every wave of the workgroup calls it;
+  // g: this wave's block of G (scale 2^SG).  Returns its block of P, scale 2^(steps > 1 ? SP : SQ).  Every wave of the workgroup calls it;
   // a product begins when both operands are in LDS and its result goes where nobody reads any more.
   // Two buffers: one group of waves.
   __device__ __forceinline__ f32x16 run2(f32x16 g, int steps, char* b1, char* b2) const {
-    const float q1 = 1.f / (float)(1 << SG);
+    const float q1 = 1.f / (float)(1 << SQ);
     f32x16 P, y;
     __syncthreads();
     put(b1, g);
@@ -1075,7 +1092,7 @@ struct SmallChain {
   // Four buffers and two groups of waves (grp): the first one follows G, the second one P; three barriers a step.  P is group
   // (steps > 1)'s; g is group 0's.
   __device__ __forceinline__ f32x16 run4(int grp, f32x16 g, int steps, char* b) const {
-    const float q1 = 1.f / (float)(1 << SG);
+    const float q1 = 1.f / (float)(1 << SQ);
     char *const bg = b, *const bq = b + BUF, *const by = b + 2 * BUF, *const bp = b + 3 * BUF;
     f32x16 P;
 #pragma unroll
@@ -1172,8 +1189,8 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
   __shared__ __attribute__((aligned(1024))) char smem[2 * XP + 4 * Sc::BUF];         // 64 x 384: all of the CU's 160 KB
   char* const X = smem;
   char* const b1 = smem + 2 * XP;
-  double* const red = reinterpret_cast<double*>(b1);                // before the first product
-  float& cfac = *reinterpret_cast<float*>(b1 + 64);
+  NsNorm* const red = reinterpret_cast<NsNorm*>(b1);                // before the first product: of each wave
+  float& cfac = *reinterpret_cast<float*>(b1 + 8 * sizeof(NsNorm));
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   NsMat mm = m;
   mm.src += (long)blockIdx.x * src_step;
@@ -1183,6 +1200,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
   const int rpr = (m.cols + 7) / 8, nrun = m.rows * rpr;
   float v[RUNS][8];
   double a = 0.0;
+  float top = 0.f;
 #pragma unroll
   for (int t = 0; t < RUNS; ++t) {
     const int c = t * 512 + tid;
@@ -1190,18 +1208,19 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
       const int row = c / rpr;
       ns_load8<SRC>(mm, x, none, row, (c - row * rpr) * 8, v[t]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a = fma((double)v[t][e], (double)v[t][e], a);
+      for (int e = 0; e < 8; ++e) { a = fma((double)v[t][e], (double)v[t][e], a); top = fmaxf(top, fabsf(v[t][e])); }
     }
   }
 #pragma unroll
   for (int t = 0; t < 2 * XP / 16 / 512; ++t) *reinterpret_cast<uint4*>(X + (t * 512 + tid) * 16) = make_uint4(0u, 0u, 0u, 0u);
   a = wave_sum_d(a);
-  if (lane == 0) red[wave] = a;
+  top = wave_max(top);
+  if (lane == 0) { red[wave].sum = a; red[wave].top = top; }
   __syncthreads();
   a = 0.0;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) a += red[w];
-  const int k = ns_exponent(a, m.inv);
+  for (int w = 0; w < 8; ++w) { a += red[w].sum; top = fmaxf(top, red[w].top); }
+  const int k = ns_exponent(top);
   const float f = ns_pow2(-k);
   if (tid == 511) cfac = ns_factor(a, k, eps);
 #pragma unroll
@@ -1269,7 +1288,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
     if ((wave >> 2) == (ns > 1)) sc.put(b1, P);
     __syncthreads();
     const bool last = steps == 0;
-    const float mul = c1 * (ns > 1 ? 1.f / (float)(1 << SP) : 1.f / (float)(1 << SG)) * (last ? 1.f : 32768.f);
+    const float mul = c1 * (ns > 1 ? 1.f / (float)(1 << SP) : 1.f / (float)(1 << SQ)) * (last ? 1.f : 32768.f);
     for (int s = wave; s < m.Np / 32; s += 8) {       // a strip of 32 columns: all of its rows are this wave's
       f32x16 acc[2];
 #pragma unroll
@@ -1361,7 +1380,6 @@ static bool ns_shape(NsMat& m) {
   m.N = (int)(m.tall ? rows : cols);
   m.Mp = (int)Mp;
   m.Np = (int)Np;
-  m.inv = 1.0 / (double)(rows * cols);
   return true;
 }
 struct NsCounts { long n[F_N], x, g, part; };
@@ -1398,7 +1416,7 @@ static void ns_place(NsPlan& pl, int nmat, long nx, long ng, long npart) {
   take(pl.off_tab, (long)pl.mats.size() * (long)sizeof(NsMat));
   take(pl.off_first, (long)pl.first.size() * 4);
   take(pl.off_c, (long)nmat * 4);
-  take(pl.off_sq, pl.n[F_MOM] * 8);
+  take(pl.off_sq, pl.n[F_MOM] * (long)sizeof(NsNorm));
   pl.x_halves = up(nx, 128);
   take(pl.off_x, pl.x_halves * 2 * 2);               // two sets of planes: X and its successor
   take(pl.off_g, ng * 2);
@@ -1489,7 +1507,7 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
                    long ldo, hipStream_t st) {
   const NsGroup& gr = pl.gr;
   float* cfac = reinterpret_cast<float*>(w + pl.off_c);
-  const double* sq = reinterpret_cast<const double*>(w + pl.off_sq);
+  const NsNorm* sq = reinterpret_cast<const NsNorm*>(w + pl.off_sq);
   _Float16* xin = reinterpret_cast<_Float16*>(w + pl.off_x);
   _Float16* xout = xin + pl.x_halves;
   _Float16* g = reinterpret_cast<_Float16*>(w + pl.off_g);
@@ -1510,15 +1528,15 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     if (one) PG_KLAUNCH((ns_gram_kernel<1>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
     else PG_KLAUNCH((ns_gram_kernel<2>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
     // buffers: 0 G, 1 Q, 2 Q G, 3 and 4 P in turn; the first step's Q is the first P (and keeps Q's scale)
-    const float q1 = 1.f / (float)(1 << SG);
-    int p = 3, psc = SG;
+    const float q1 = 1.f / (float)(1 << SQ);
+    int p = 3, psc = SQ;
     const bool many = pl.n[F_JOIN] > 512;
     const int nc = (int)pl.n[many ? F_CHAIN : F_JOIN];
     if (pl.top <= 128) {
       const dim3 gm((unsigned)gr.n);
       if (pl.top == 64) PG_KLAUNCH((ns_chain_small_kernel<64>), gm, dim3(512), 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
       else PG_KLAUNCH((ns_chain_small_kernel<128>), gm, dim3(1024), 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
-      psc = ns > 1 ? SP : SG;
+      psc = ns > 1 ? SP : SQ;
     } else {
       PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.n[F_JOIN]), blk, 0, st, gr, (const float*)part, cf, 1.f / sx, g);
       auto chain = [&](const ChainJob& a, const ChainJob* b) {
@@ -1534,8 +1552,8 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
       };
       for (int k = 0; k < ns; ++k) {
         const int q = k == 0 ? 3 : 1;
-        const ChainJob quad = {0, 0, q, NS_C * q1, 1};
-        const ChainJob qg = {q, 0, 2, q1, 0}, qp = {q, p, 7 - p, (float)ldexp(1.0, SP - SG - psc), 0}, qqg = {q, 2, 0, q1, 0};
+        const ChainJob quad = {0, 0, q, QUAD_C, 1};
+        const ChainJob qg = {q, 0, 2, q1, 0}, qp = {q, p, 7 - p, (float)ldexp(1.0, SP - SQ - psc), 0}, qqg = {q, 2, 0, q1, 0};
         const bool more = k + 1 < ns;
         chain(quad, nullptr);
         if (more) chain(qg, k > 0 ? &qp : nullptr);
@@ -1630,7 +1648,7 @@ extern "C" int pg_orthogonalise(const void* x, int32_t x_is_bf16, int64_t batch,
   PG_REQUIRE(workspace && workspace_bytes >= pl.bytes, "pg_orthogonalise: workspace of %lld bytes required", (long long)pl.bytes);
   char* w = reinterpret_cast<char*>(workspace);
   hipStream_t st = (hipStream_t)stream;
-  double* sq = reinterpret_cast<double*>(w + pl.off_sq);
+  NsNorm* sq = reinterpret_cast<NsNorm*>(w + pl.off_sq);
   const NsStep none{};
   for (int64_t b = 0; b < batch; b += piece) {
     pl.gr.n = (int)(batch - b < piece ? batch - b : piece);
@@ -1692,7 +1710,7 @@ extern "C" int pg_muon_step(const pg_muon_t* d, void* stream) {
   s.mu = d->momentum; s.gscale = d->grad_scale; s.lr = d->lr; s.wd = d->weight_decay; s.nesterov = d->nesterov;
   s.b1 = (float)d->beta1; s.b2 = (float)d->beta2; s.eps = d->adam_eps; s.b1d = d->beta1; s.b2d = d->beta2;
   s.step0 = (long)d->step; s.ctr = reinterpret_cast<const unsigned long long*>(d->ctr);
-  PG_KLAUNCH(muon_momentum_kernel, dim3((unsigned)pl.n[F_MOM]), dim3(256), 0, st, pl.gr, s, reinterpret_cast<double*>(w + pl.off_sq));
+  PG_KLAUNCH(muon_momentum_kernel, dim3((unsigned)pl.n[F_MOM]), dim3(256), 0, st, pl.gr, s, reinterpret_cast<NsNorm*>(w + pl.off_sq));
   if (pl.n[F_GRAM] > 0) {
     const NsSource in = {2, nullptr};
     ns_run(pl, w, in, s, d->steps, d->eps, 3, nullptr, 0, st);
