@@ -305,16 +305,25 @@ __device__ __forceinline__ int ns_exponent(float top) {
   return max(-126, min(126, (int)((__float_as_uint(top) >> 23) & 0xff) - 127 - 14));
 }
 __device__ __forceinline__ float ns_pow2(int k) { return __uint_as_float((unsigned)(k + 127) << 23); }      // |k| <= 126
-// 2^k / (|U| + eps): from the planes' units to X0's
-__device__ __forceinline__ float ns_factor(double sumsq, int k, float eps) {
-  return sumsq == 0.0 ? 0.f : (float)((double)ns_pow2(k) / (sqrt(sumsq) + (double)eps));
+// A matrix's units: c = 2^k / (|U| + eps), from the first planes' to X0's, and gap with |X0|_F <= 2^-gap: 0 but where eps outweighs |U|.
+// Later planes hold 2^(15 + gap(stage)) X: |X| <= 1.21 (the quintic's largest value on [0, 1.21]) fits fp16, and so does an X that began
+// at 2^-gap and grew by up to 3.4445^3 < 2^6 a stage; at 2^15 alone it would sink below fp16's smallest values.
+struct NsUnit { float c; int gap; };
+__device__ __forceinline__ NsUnit ns_unit_of(double sumsq, int k, float eps) {
+  const double n = sqrt(sumsq), x0 = n / (n + (double)eps);
+  const int e = (int)((__double_as_longlong(x0) >> 52) & 0x7ff) - 1023;              // x0 < 2^(e + 1); NaN: 1024
+  return {sumsq == 0.0 ? 0.f : (float)((double)ns_pow2(k) / (n + (double)eps)), max(0, min(96, -(e + 1)))};
 }
+__device__ __forceinline__ int ns_gap(const NsUnit& u, int stage) { return max(0, u.gap - 6 * stage); }
+// from the planes' units at the beginning of a stage to values
+__device__ __forceinline__ float ns_value(const NsUnit& u, int stage) { return stage == 0 ? u.c : ns_pow2(-15 - ns_gap(u, stage)); }
+
 // every workgroup joins its matrix's partial sums of squares itself (a few hundred doubles); the first one publishes
-// c = 2^k / (|U| + eps), the factor from the planes' units to X0's.  12 bytes / element from fp32 pairs (m', g), HBM-bound: 211 us for 77 M
+// the matrix's units.  12 bytes / element from fp32 pairs (m', g), HBM-bound: 211 us for 77 M
 // elements (4.4 TB/s); 14 us for 512 x 24576 bf16 (6 bytes)
 template <int SRC>
 __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const void* x, const NsStep s, const NsNorm* sq, float eps,
-                                                       float* cfac, _Float16* ws) {
+                                                       NsUnit* unit, _Float16* ws) {
   __shared__ NsNorm red[4];
   __shared__ float tile[64][65];
   constexpr bool ONE = SRC == 1;
@@ -353,7 +362,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
   const NsNorm nm = block_norm256(a, top, red);
   const int k = ns_exponent(nm.top);
   const float f = ns_pow2(-k);
-  if (r.tile == 0 && threadIdx.x == 0) cfac[r.id] = ns_factor(nm.sum, k, eps);
+  if (r.tile == 0 && threadIdx.x == 0) unit[r.id] = ns_unit_of(nm.sum, k, eps);
   _Float16* hi = ws + m.x;
   _Float16* lo = hi + xplane(m);
   if (!m.tall) {
@@ -556,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int t
 
 // join of the slices, in order; both triangles of G from the lower one.  One workgroup = one 32 x 32 block, a float4 per thread: 4 - 6 us, mostly
 // launch (12 us for the generator's 20 matrices)
-__global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, const float* part, const float* cfac, float cconst, _Float16* ws) {
+__global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, const float* part, const NsUnit* unit, int stage, _Float16* ws) {
   const NsRef r = ns_find<F_JOIN>(gr, blockIdx.x);
   const NsMat& m = r.m;
   int bi, bj;
@@ -566,7 +575,7 @@ __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, con
   const int wave = (fi >> 1) * 2 + (fj >> 1), frag = wave * 4 + (fi & 1) * 2 + (fj & 1);
   const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
   const float4* src = reinterpret_cast<const float4*>(part + m.part + (long)(gi * (gi + 1) / 2 + gj) * (GT * GT)) + (frag * 4 + q) * 64 + lane;
-  const float c1 = cfac ? cfac[r.id] : cconst;
+  const float c1 = ns_value(unit[r.id], stage);
   const float c2 = c1 * c1 * (float)(1 << SG);
   float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
@@ -774,7 +783,7 @@ __global__ __launch_bounds__(256) void ns_chain32_kernel(const NsGroup gr, Chain
 struct ApplyK {
   const _Float16* wsx; const _Float16* wsg; _Float16* wso;
   int pbuf;
-  const float* cfac; float cconst;        // planes' units -> values
+  const NsUnit* unit; int stage;
   float mul;
   void* out; long ldo;
   NsStep s;
@@ -887,7 +896,8 @@ __global__ __launch_bounds__(512, 2) void ns_apply_kernel(const NsGroup gr, int 
     cur = cur == ST - 1 ? 0 : cur + 1;
     nxt = nxt == ST - 1 ? 0 : nxt + 1;
   }
-  const float f = (k.cfac ? k.cfac[r.id] : k.cconst) * k.mul;
+  const NsUnit un = k.unit[r.id];
+  const float f = ns_value(un, k.stage) * (OUT == 0 ? ns_pow2(15 + ns_gap(un, k.stage + 1)) : 1.f) * k.mul;
   const float keep = 1.f - k.s.lr * k.s.wd, step = k.s.lr * m.scale;
   if (OUT != 0 && m.tall) {
     // the stored row is the long side: 32 neighbouring lanes hold 32 neighbours of a stored row
@@ -1129,7 +1139,7 @@ struct SmallChain {
 
 // the join of the Gram slices and the whole chain of one stage: one workgroup per matrix, P to buffer 3
 template <int MP>
-__global__ __launch_bounds__(MP * 8) void ns_chain_small_kernel(const NsGroup gr, const float* part, const float* cfac, float cconst,
+__global__ __launch_bounds__(MP * 8) void ns_chain_small_kernel(const NsGroup gr, const float* part, const NsUnit* unit, int stage,
                                                                                   int steps, _Float16* ws) {
   typedef SmallChain<MP> Sc;
   __shared__ __attribute__((aligned(1024))) char smem[(MP == 64 ? 4 : 2) * Sc::BUF];
@@ -1141,7 +1151,7 @@ __global__ __launch_bounds__(MP * 8) void ns_chain_small_kernel(const NsGroup gr
   const Sc sc(wave % (Sc::W * Sc::W));
   const int frag = ((sc.wi >> 1) * 2 + (sc.wj >> 1)) * 4 + (sc.wi & 1) * 2 + (sc.wj & 1);
   const float4* src = reinterpret_cast<const float4*>(part + m.part) + frag * 256 + lane;
-  const float c1 = cfac ? cfac[id] : cconst;
+  const float c1 = ns_value(unit[id], stage);
   const float c2 = c1 * c1 * (float)(1 << SG);
   f32x16 g;
 #pragma unroll
@@ -1190,7 +1200,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
   char* const X = smem;
   char* const b1 = smem + 2 * XP;
   NsNorm* const red = reinterpret_cast<NsNorm*>(b1);                // before the first product: of each wave
-  float& cfac = *reinterpret_cast<float*>(b1 + 8 * sizeof(NsNorm));
+  NsUnit& unit = *reinterpret_cast<NsUnit*>(b1 + 8 * sizeof(NsNorm));
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   NsMat mm = m;
   mm.src += (long)blockIdx.x * src_step;
@@ -1222,7 +1232,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
   for (int w = 0; w < 8; ++w) { a += red[w].sum; top = fmaxf(top, red[w].top); }
   const int k = ns_exponent(top);
   const float f = ns_pow2(-k);
-  if (tid == 511) cfac = ns_factor(a, k, eps);
+  if (tid == 511) unit = ns_unit_of(a, k, eps);
 #pragma unroll
   for (int t = 0; t < RUNS; ++t) {
     const int c = t * 512 + tid;
@@ -1251,8 +1261,9 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
   const int r4 = (lane >> 2) & 3, cq = lane & 3, mb = (lane >> 4) & 1, kh = lane >> 5;
   const int nblk = m.Np / 16;
   __syncthreads();
-  float c1 = cfac;
-  while (steps > 0) {
+  const NsUnit un = unit;
+  for (int stage = 0; steps > 0; ++stage) {
+    const float c1 = ns_value(un, stage);
     const int ns = steps < 3 ? steps : 3;
     steps -= ns;
     __syncthreads();
@@ -1288,7 +1299,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
     if ((wave >> 2) == (ns > 1)) sc.put(b1, P);
     __syncthreads();
     const bool last = steps == 0;
-    const float mul = c1 * (ns > 1 ? 1.f / (float)(1 << SP) : 1.f / (float)(1 << SQ)) * (last ? 1.f : 32768.f);
+    const float mul = c1 * (last ? 1.f : ns_pow2(15 + ns_gap(un, stage + 1))) * (ns > 1 ? 1.f / (float)(1 << SP) : 1.f / (float)(1 << SQ));
     for (int s = wave; s < m.Np / 32; s += 8) {       // a strip of 32 columns: all of its rows are this wave's
       f32x16 acc[2];
 #pragma unroll
@@ -1353,7 +1364,6 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const NsMat m, const void
         }
       }
     }
-    c1 = 1.f / 32768.f;
   }
 }
 
@@ -1415,7 +1425,7 @@ static void ns_place(NsPlan& pl, int nmat, long nx, long ng, long npart) {
   pl.bytes = 0;
   take(pl.off_tab, (long)pl.mats.size() * (long)sizeof(NsMat));
   take(pl.off_first, (long)pl.first.size() * 4);
-  take(pl.off_c, (long)nmat * 4);
+  take(pl.off_c, (long)nmat * (long)sizeof(NsUnit));
   take(pl.off_sq, pl.n[F_MOM] * (long)sizeof(NsNorm));
   pl.x_halves = up(nx, 128);
   take(pl.off_x, pl.x_halves * 2 * 2);               // two sets of planes: X and its successor
@@ -1506,25 +1516,21 @@ struct NsSource { int kind; const void* x; };      // kind: ns_elem's SRC
 static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& step, int steps, float eps, int out_kind, void* out,
                    long ldo, hipStream_t st) {
   const NsGroup& gr = pl.gr;
-  float* cfac = reinterpret_cast<float*>(w + pl.off_c);
+  NsUnit* unit = reinterpret_cast<NsUnit*>(w + pl.off_c);
   const NsNorm* sq = reinterpret_cast<const NsNorm*>(w + pl.off_sq);
   _Float16* xin = reinterpret_cast<_Float16*>(w + pl.off_x);
   _Float16* xout = xin + pl.x_halves;
   _Float16* g = reinterpret_cast<_Float16*>(w + pl.off_g);
   float* part = reinterpret_cast<float*>(w + pl.off_part);
   const dim3 blk(256);
-  if (in.kind == 0) PG_KLAUNCH((ns_split_kernel<0>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, cfac, xin);
-  else if (in.kind == 1) PG_KLAUNCH((ns_split_kernel<1>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, cfac, xin);
-  else PG_KLAUNCH((ns_split_kernel<2>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, cfac, xin);
-  // planes between stages: |X| <= 1.21 (the quintic's largest value on [0, 1.21]), so 2^15 X fits fp16; its rms there is >= 0.5
-  const float sx = 32768.f;
-  bool first = true;
-  while (steps > 0) {
+  if (in.kind == 0) PG_KLAUNCH((ns_split_kernel<0>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, unit, xin);
+  else if (in.kind == 1) PG_KLAUNCH((ns_split_kernel<1>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, unit, xin);
+  else PG_KLAUNCH((ns_split_kernel<2>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, unit, xin);
+  for (int stage = 0; steps > 0; ++stage) {
     const int ns = steps < 3 ? steps : 3;
     steps -= ns;
     const bool last = steps == 0;
-    const float* cf = first ? cfac : nullptr;
-    const bool one = first && in.kind == 1;
+    const bool one = stage == 0 && in.kind == 1;
     if (one) PG_KLAUNCH((ns_gram_kernel<1>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
     else PG_KLAUNCH((ns_gram_kernel<2>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
     // buffers: 0 G, 1 Q, 2 Q G, 3 and 4 P in turn; the first step's Q is the first P (and keeps Q's scale)
@@ -1534,11 +1540,11 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     const int nc = (int)pl.n[many ? F_CHAIN : F_JOIN];
     if (pl.top <= 128) {
       const dim3 gm((unsigned)gr.n);
-      if (pl.top == 64) PG_KLAUNCH((ns_chain_small_kernel<64>), gm, dim3(512), 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
-      else PG_KLAUNCH((ns_chain_small_kernel<128>), gm, dim3(1024), 0, st, gr, (const float*)part, cf, 1.f / sx, ns, g);
+      if (pl.top == 64) PG_KLAUNCH((ns_chain_small_kernel<64>), gm, dim3(512), 0, st, gr, (const float*)part, (const NsUnit*)unit, stage, ns, g);
+      else PG_KLAUNCH((ns_chain_small_kernel<128>), gm, dim3(1024), 0, st, gr, (const float*)part, (const NsUnit*)unit, stage, ns, g);
       psc = ns > 1 ? SP : SQ;
     } else {
-      PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.n[F_JOIN]), blk, 0, st, gr, (const float*)part, cf, 1.f / sx, g);
+      PG_KLAUNCH(ns_gram_join_kernel, dim3((unsigned)pl.n[F_JOIN]), blk, 0, st, gr, (const float*)part, (const NsUnit*)unit, stage, g);
       auto chain = [&](const ChainJob& a, const ChainJob* b) {
         const int total = b ? 2 * nc : nc;
         const dim3 gd((unsigned)up(total, 8));
@@ -1565,8 +1571,8 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     ApplyK a;
     memset(&a, 0, sizeof(a));
     a.wsx = xin; a.wsg = g; a.wso = xout; a.pbuf = p;
-    a.cfac = cf; a.cconst = 1.f / sx;
-    a.mul = (float)ldexp(1.0, -psc) * (last ? 1.f : sx);
+    a.unit = unit; a.stage = stage;
+    a.mul = (float)ldexp(1.0, -psc);
     a.out = out; a.ldo = ldo; a.s = step;
     const int o = last ? out_kind : 0;
     const int na = (int)pl.n[F_APPLY];
@@ -1584,7 +1590,6 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     }
 #undef NS_APPLY
     _Float16* t = xin; xin = xout; xout = t;
-    first = false;
   }
 }
 

@@ -67,3 +67,15 @@ def test_orthogonalise_keeps_small_rows(shape, dtype):
     err = (got - ref).norm(dim=dim) / ref.norm(dim=dim)
     tol = BASE + 2.0 ** -30 * short / (41 * size.double())
     assert bool((err <= tol).all()), (err[:, at].max(0).values.tolist(), tol[at].tolist(), float(err.max()))
+
+
+@pytest.mark.parametrize("shape", ORTHO)
+@pytest.mark.parametrize("size,eps", [(1e-12, 1e-7), (1e-20, 1e-7), (1e-6, 1.0), (1e-9, 1e-10)])
+def test_orthogonalise_of_inputs_that_eps_outweighs(shape, size, eps):
+    """|x| far below eps: X0 is small, every step multiplies it by about 3.4445, and the result is as accurate as any other.
+    (1e-9, 1e-10): |x| about eps"""
+    x = rnd(2, *shape)
+    x = x * (size / x.flatten(1).norm(dim=1).max())
+    got, ref = ops().orthogonalise(x, eps=eps).double(), ortho_ref(x, eps=eps)
+    err = (got - ref).flatten(1).norm(dim=1) / ref.flatten(1).norm(dim=1)
+    assert float(err.max()) <= BASE, err.tolist()
