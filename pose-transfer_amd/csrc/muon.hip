@@ -42,8 +42,15 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int SG = 15, SQ = 14, SP = 10;        // log2 of the scales of G and Q G, of Q, of P
-// elements per workgroup of the momentum / square-sum pass: small tensors give few workgroups, large ones many partial sums
-__host__ __device__ constexpr int k0_elems(long n) { return n < (1L << 21) ? 4096 : 16384; }
+// elements per workgroup of the momentum pass, and runs of up to eight neighbours per workgroup of the square-sum pass: small tensors give
+// few workgroups; large ones at most 1024 partial sums, which every workgroup of the split reads
+constexpr long MAX_PARTIALS = 1024;
+__host__ __device__ constexpr int k0_elems(long n) {
+  return n < (1L << 21) ? 4096 : n <= 16384 * MAX_PARTIALS ? 16384 : (int)((n + MAX_PARTIALS * 4096 - 1) / (MAX_PARTIALS * 4096) * 4096);
+}
+__host__ __device__ constexpr int sq_runs(long runs) {
+  return runs <= 512 * MAX_PARTIALS ? 512 : (int)((runs + MAX_PARTIALS * 256 - 1) / (MAX_PARTIALS * 256) * 256);
+}
 // Q = a I + b G + c G G in the planes' units
 constexpr float QUAD_A = NS_A * (float)(1 << SQ), QUAD_B = NS_B / (float)(1 << (SG - SQ)), QUAD_C = NS_C / (float)(1 << (2 * SG - SQ));
 constexpr int GT = 128, AI = 128, AJ = 128;      // tiles: Gram; apply (rows, columns)
@@ -271,15 +278,14 @@ __device__ __forceinline__ void ns_load8(const NsMat& m, const void* x, const Ns
   }
 }
 
-// one workgroup = 512 runs of eight stored neighbours
-constexpr int SQ_RUNS = 512;
+// one workgroup = sq_runs runs of eight stored neighbours
 template <int SRC>
 __global__ __launch_bounds__(256) void ns_sumsq_kernel(const NsGroup gr, const void* x, NsNorm* sq) {
   __shared__ NsNorm red[4];
   const NsRef r = ns_find<F_MOM>(gr, blockIdx.x);
   const unsigned rpr = (unsigned)(r.m.cols + 7) / 8u;
   const unsigned n = (unsigned)r.m.rows * rpr;
-  const unsigned e0 = (unsigned)r.tile * SQ_RUNS, e1 = min(n, e0 + SQ_RUNS);
+  const unsigned per = (unsigned)sq_runs((long)n), e0 = (unsigned)r.tile * per, e1 = min(n, e0 + per);
   double acc = 0.0;
   float top = 0.f;
   const NsStep s{};
@@ -318,7 +324,7 @@ __device__ __forceinline__ int ns_gap(const NsUnit& u, int stage) { return max(0
 // from the planes' units at the beginning of a stage to values
 __device__ __forceinline__ float ns_value(const NsUnit& u, int stage) { return stage == 0 ? u.c : ns_pow2(-15 - ns_gap(u, stage)); }
 
-// every workgroup joins its matrix's partial sums of squares itself (a few hundred doubles); the first one publishes
+// every workgroup joins its matrix's partial sums of squares itself (at most 1024); the first one publishes
 // the matrix's units.  12 bytes / element from fp32 pairs (m', g), HBM-bound: 211 us for 77 M
 // elements (4.4 TB/s); 14 us for 512 x 24576 bf16 (6 bytes)
 template <int SRC>
@@ -1397,7 +1403,7 @@ struct NsCounts { long n[F_N], x, g, part; };
 static NsCounts ns_counts(NsMat& m, long ks, bool flat) {
   NsCounts c{};
   const long n = (long)m.taps * m.rows * m.cols;
-  c.n[F_MOM] = flat ? cdiv(n, k0_elems(n)) : cdiv((long)m.rows * cdiv(m.cols, 8), SQ_RUNS);
+  c.n[F_MOM] = flat ? cdiv(n, k0_elems(n)) : cdiv((long)m.rows * cdiv(m.cols, 8), sq_runs((long)m.rows * cdiv(m.cols, 8)));
   m.np = (int)c.n[F_MOM];
   if (m.kind == 1) return c;
   c.n[F_SPLIT] = m.tall ? (long)(m.Mp / 64) * (m.Np / 64) : (long)(m.Mp / 64) * cdiv(m.Np, 128);

@@ -79,3 +79,76 @@ def test_orthogonalise_of_inputs_that_eps_outweighs(shape, size, eps):
     got, ref = ops().orthogonalise(x, eps=eps).double(), ortho_ref(x, eps=eps)
     err = (got - ref).flatten(1).norm(dim=1) / ref.flatten(1).norm(dim=1)
     assert float(err.max()) <= BASE, err.tolist()
+
+
+@pytest.mark.parametrize("shape", [(65, 1 << 19), ((1 << 24) + 5, 1), ((1 << 20) + 1, 3), (130, (1 << 17) + 3)])
+def test_orthogonalise_long_thin_matrices(shape):
+    """more elements than 1024 workgroups of the usual share take"""
+    x = rnd(3, *shape, dtype=torch.bfloat16).float()
+    got, ref = ops().orthogonalise(x), ortho_ref(x)
+    assert float((got - ref).norm() / ref.norm()) <= BASE
+
+
+def muon_plain(p, g, m, v, table, lr, mu, nesterov, wd, b1, b2, eps, step):
+    """the step in 64 bits, coefficients as the kernels hold them: fp32, and 1 - beta as the complement of that"""
+    p, g, m, v = (t.double().clone() for t in (p, g, m, v))
+    f = lambda c: float(np.float32(c))
+    for e in table:
+        taps, rows, cols = int(e["taps"]), int(e["rows"]), int(e["cols"])
+        at = slice(int(e["off"]), int(e["off"]) + taps * rows * cols)
+        if e["kind"] == 0:
+            m[at] = f(mu) * m[at] + (1 - f(mu)) * g[at]
+            u = (1 - f(mu)) * g[at] + f(mu) * m[at] if nesterov else m[at]
+            x = u.view(taps, rows, cols).permute(1, 0, 2).reshape(rows, taps * cols)
+            o = ortho_ref(x).reshape(rows, taps, cols).permute(1, 0, 2).reshape(-1)
+            p[at] = p[at] * (1 - f(lr) * f(wd)) - f(lr) * float(e["scale"]) * o
+        else:
+            m[at] = f(b1) * m[at] + (1 - f(b1)) * g[at]
+            v[at] = f(b2) * v[at] + (1 - f(b2)) * g[at] * g[at]
+            p[at] = p[at] - lr / (1 - b1 ** step) * m[at] / (v[at].sqrt() / math.sqrt(1 - b2 ** step) + eps)
+    return p, m, v
+
+
+def table_of(parts):
+    rec, off = [], 0
+    for q in parts:
+        n = math.prod(q)
+        rec.append((off, 1, 1, n, 1, 0.0, 0) if len(q) == 1 else (off,) + tuple(q) + (0, 0.2 * math.sqrt(max(q[1], q[0] * q[2])), 0))
+        off += (n + 63) // 64 * 64
+    return np.array(rec, dtype=ops().MUON_ENTRY), off
+
+
+def muon_close(p0, p, pr, table, tol):
+    """each record's update against its own size, and the roundings of p before and after"""
+    for e in table:
+        at = slice(int(e["off"]), int(e["off"]) + int(e["taps"]) * int(e["rows"]) * int(e["cols"]))
+        a, b = p[at].double() - p0[at].double(), pr[at] - p0[at].double()
+        err = float((a - b).norm())
+        assert err <= tol * float(b.norm()) + 2 * U * float(pr[at].norm() + p0[at].double().norm()), (tuple(e), err, float(b.norm()))
+
+
+# matrices of at least four times as many columns as rows; then with tensors longer than 1024 workgroups of the usual share
+MUON = [[(1, 64, 300), (70,)], [(16, 40, 30), (5,), (9, 100, 50), (16, 130, 40), (1, 2, 9)], [(16, 512, 128), (64,)] + [(4, 300, 400)] * 9,
+        [(1, 64, 300001), (20000001,)], [(4, 1, 5000001), (3,)]]
+
+
+@pytest.mark.parametrize("parts", MUON)
+@pytest.mark.parametrize("gbf", [False, True])
+def test_muon_step_to_the_accuracy_of_its_products(parts, gbf):
+    """the update of every matrix within BASE of its own size (half a step of u, in fp32, more), with fp32 and with bf16 gradients and the
+    bf16 copy of the weights"""
+    table, total = table_of(parts)
+    p, g, m, v = rnd(10, total, scale=0.05), rnd(11, total, scale=1e-3), rnd(12, total, scale=1e-3), rnd(13, total).square() * 1e-6 + 1e-9
+    if gbf:
+        g = g.bfloat16()
+    p0, m0, v0 = p.clone(), m.clone(), v.clone()
+    pb = torch.full((total,), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops().muon_step(p, g, m, v, table, lr=2e-3, momentum=0.95, weight_decay=0.1, betas=(0.5, 0.999), eps=1e-8, step=4, p_bf16=pb)
+    pr, mr, vr = muon_plain(p0, g, m0, v0, table, 2e-3, 0.95, True, 0.1, 0.5, 0.999, 1e-8, 4)
+    muon_close(p0, p, pr, table, BASE)
+    assert bool(((m.double() - mr).abs() <= 4 * U * (m0.double().abs() + g.double().abs())).all())
+    assert bool(((v.double() - vr).abs() <= 8 * U * vr.abs()).all())
+    used = torch.zeros(total, dtype=torch.bool, device="cuda")
+    for e in table:
+        used[int(e["off"]):int(e["off"]) + int(e["taps"]) * int(e["rows"]) * int(e["cols"])] = True
+    assert torch.equal(pb[used], p[used].bfloat16()) and bool((pb[~used] == 7).all())
