@@ -400,7 +400,9 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const v
 
 // ---------------------------------------------------------------------------------------------- product cores
 // Workgroups are dealt round-robin to the 8 XCDs, each with an L2 of its own: `grp` consecutive tiles, which share operand rows, go
-// to one of them.  The grid is padded to a multiple of 8; < 0: no tile.
+// to one of them.  grp is the number of tiles of the largest matrix that read the same rows: all tiles of a Gram slice, of a chain matrix,
+// of a column strip of the apply product (against a 512-sided matrix's 10, 36 and 4 for every size: 16 x 256 x 4096 283 -> 273 us,
+// 1024 x 8192 412 -> 403 us).  The grid is padded to a multiple of 8; < 0: no tile.
 __device__ __forceinline__ int xcd_tile(int b, int total, int grp) {
   const int chunk = 8 * grp, full = total / chunk * chunk;
   if (b < full) {
@@ -542,10 +544,10 @@ __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
 // 512 x 24576) take 201 - 212 us, 512 x 24576 alone 29 us (two planes) and 16 us (bf16: one): MFMA-bound with operands from L2.  Where few slices run (16 x
 // 770 x 189: 144 workgroups, 11 - 13 us) it is launch, first transfer and the partial tiles' way out; more stages or slices gave nothing.
 template <int PL>
-__global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int total, const _Float16* ws, float* part) {
+__global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int total, int grp, const _Float16* ws, float* part) {
   typedef NtCore<GT, PL, 2> Core;
   __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
-  const int b = xcd_tile(blockIdx.x, total, 10);
+  const int b = xcd_tile(blockIdx.x, total, grp);
   if (b < 0) return;
   const NsRef r = ns_find<F_GRAM>(gr, b);
   const NsMat& m = r.m;
@@ -617,10 +619,10 @@ struct ChainJob { int a, b, c; float mul; int quad; };
 // Tiles of 64 x 64 (many matrices): four stages of 16 KB, two workgroups per CU; 17 - 19 us for 472
 // tiles of 64 .. 512 columns (32 x 32 tiles: 22 - 23 us; a launch of two jobs 31 and 38 us).  The result leaves through LDS: written four
 // neighbours at a time as the mirrored tile, which is copied out as it is and, by transposing reads, turned.
-__global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, _Float16* ws) {
+__global__ __launch_bounds__(256, 2) void ns_chain_kernel(const NsGroup gr, ChainJob j0, ChainJob j1, int total, int tiles, int grp, _Float16* ws) {
   typedef NtCore<64, 2, 4> Core;
   __shared__ __attribute__((aligned(1024))) char smem[Core::LDS_BYTES];
-  const int t = xcd_tile(blockIdx.x, total, 36);
+  const int t = xcd_tile(blockIdx.x, total, grp);
   if (t < 0) return;
   const ChainJob jb = t >= tiles ? j1 : j0;          // two jobs: the second one's tiles come behind the first one's
   const NsRef r = ns_find<F_CHAIN>(gr, t >= tiles ? t - tiles : t);
@@ -823,19 +825,20 @@ __device__ __forceinline__ void muon_update(const NsStep& s, long at, float keep
   if (s.pb) s.pb[at] = (bf16_t)(ns_pack_bf16(p, 0.f) & 0xffffu);
 }
 template <int PX, int OUT>
-__global__ __launch_bounds__(512, 2) void ns_apply_kernel(const NsGroup gr, int total, const ApplyK k) {
+__global__ __launch_bounds__(512, 2) void ns_apply_kernel(const NsGroup gr, int total, int grp, const ApplyK k) {
   constexpr int TM = 2, NW = 8, IPP = AJ / 32;      // IPP: transfers per plane of X
   constexpr int A_BYTES = AI * 2 * 32, B_BYTES = 16 * AJ * 2 * PX, STAGE = A_BYTES + B_BYTES, ST = 3;
   // transfers per wave; 128 columns of one plane keep only the first four waves busy
   constexpr int PA = A_BYTES / 1024 / NW, PB = (B_BYTES / 1024 + NW - 1) / NW, NI = PA + PB;
   constexpr bool HALF = B_BYTES / 1024 < NW;
   __shared__ __attribute__((aligned(1024))) char smem[ST * STAGE];
-  const int bt = xcd_tile(blockIdx.x, total, 4);
+  const int bt = xcd_tile(blockIdx.x, total, grp);
   if (bt < 0) return;
   const NsRef r = ns_find<F_APPLY>(gr, bt);
   const NsMat& m = r.m;
   const int ti = (m.Mp + AI - 1) / AI;
   const int i0 = (r.tile % ti) * AI, j0 = (r.tile / ti) * AJ;
+  const NsUnit un = k.unit[r.id];
   const long pl = cplane(m), xpl = xplane(m);
   const _Float16* P = k.wsg + m.g + k.pbuf * 2 * pl;
   const _Float16* X = k.wsx + m.x;
@@ -902,7 +905,6 @@ __global__ __launch_bounds__(512, 2) void ns_apply_kernel(const NsGroup gr, int 
     cur = cur == ST - 1 ? 0 : cur + 1;
     nxt = nxt == ST - 1 ? 0 : nxt + 1;
   }
-  const NsUnit un = k.unit[r.id];
   const float f = ns_value(un, k.stage) * (OUT == 0 ? ns_pow2(15 + ns_gap(un, k.stage + 1)) : 1.f) * k.mul;
   const float keep = 1.f - k.s.lr * k.s.wd, step = k.s.lr * m.scale;
   if (OUT != 0 && m.tall) {
@@ -1529,6 +1531,7 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
   _Float16* g = reinterpret_cast<_Float16*>(w + pl.off_g);
   float* part = reinterpret_cast<float*>(w + pl.off_part);
   const dim3 blk(256);
+  auto tri_tiles = [&](int t) { const int n = cdiv(pl.top, t); return n * (n + 1) / 2; };      // of the largest matrix
   if (in.kind == 0) PG_KLAUNCH((ns_split_kernel<0>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, unit, xin);
   else if (in.kind == 1) PG_KLAUNCH((ns_split_kernel<1>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, unit, xin);
   else PG_KLAUNCH((ns_split_kernel<2>), dim3((unsigned)pl.n[F_SPLIT]), blk, 0, st, gr, in.x, step, sq, eps, unit, xin);
@@ -1537,8 +1540,8 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     steps -= ns;
     const bool last = steps == 0;
     const bool one = stage == 0 && in.kind == 1;
-    if (one) PG_KLAUNCH((ns_gram_kernel<1>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
-    else PG_KLAUNCH((ns_gram_kernel<2>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], (const _Float16*)xin, part);
+    if (one) PG_KLAUNCH((ns_gram_kernel<1>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], tri_tiles(GT), (const _Float16*)xin, part);
+    else PG_KLAUNCH((ns_gram_kernel<2>), dim3((unsigned)up(pl.n[F_GRAM], 8)), blk, 0, st, gr, (int)pl.n[F_GRAM], tri_tiles(GT), (const _Float16*)xin, part);
     // buffers: 0 G, 1 Q, 2 Q G, 3 and 4 P in turn; the first step's Q is the first P (and keeps Q's scale)
     const float q1 = 1.f / (float)(1 << SQ);
     int p = 3, psc = SQ;
@@ -1555,7 +1558,7 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
         const int total = b ? 2 * nc : nc;
         const dim3 gd((unsigned)up(total, 8));
         const ChainJob b1 = b ? *b : a;
-        if (many) PG_KLAUNCH(ns_chain_kernel, gd, blk, 0, st, gr, a, b1, total, nc, g);
+        if (many) PG_KLAUNCH(ns_chain_kernel, gd, blk, 0, st, gr, a, b1, total, nc, tri_tiles(64), g);
         // all tiles run at once: 1, 2 or 5 workgroups to a CU by their LDS, fewer columns at a time (two jobs of 184 tiles: 9.4 us in
         // two turns of 512 columns, 7.4 us in one with 256; of 336 tiles: 9.3 us with 256, 5.8 us with 128)
         else if (total > 512) PG_KLAUNCH((ns_chain32_kernel<128>), gd, blk, 0, st, gr, a, b1, total, nc, g);
@@ -1583,7 +1586,7 @@ static void ns_run(const NsPlan& pl, char* w, const NsSource& in, const NsStep& 
     const int o = last ? out_kind : 0;
     const int na = (int)pl.n[F_APPLY];
     const dim3 gd((unsigned)up(na, 8));
-#define NS_APPLY(PX, O) PG_KLAUNCH((ns_apply_kernel<PX, O>), gd, dim3(512), 0, st, gr, na, a)
+#define NS_APPLY(PX, O) PG_KLAUNCH((ns_apply_kernel<PX, O>), gd, dim3(512), 0, st, gr, na, cdiv(pl.top, AI), a)
     if (one) {
       if (o == 0) NS_APPLY(1, 0);
       else if (o == 1) NS_APPLY(1, 1);
