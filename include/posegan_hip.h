@@ -387,7 +387,8 @@ typedef struct {
 /* The optimiser step of every tensor of an arena (at most 65536 entries in ascending, disjoint order, a HOST array read during the call):
  *   kind 0: m = momentum m + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum m : m;
  *           p = p (1 - lr weight_decay) - lr scale orthogonalise(u)
- *   kind 1: Adam with (beta1, beta2, adam_eps), the step number `step` (+ *ctr if ctr is given: replay-safe, as pg_adam_ctr)
+ *   kind 1: Adam with (beta1, beta2, adam_eps), betas in [0, 1), the step number `step` >= 1 (+ *ctr if ctr is given: replay-safe, as
+ *           pg_adam_ctr); pg_adam's arithmetic: betas held in fp32, 1 - beta their complement, bias corrections from the doubles
  * g: fp32 gradients, or g_bf16 (read instead if given), times grad_scale; p_bf16 (optional): bf16 copy of the updated parameters.       */
 typedef struct {
   float* p;

@@ -1696,6 +1696,9 @@ extern "C" int pg_muon_step(const pg_muon_t* d, void* stream) {
     const pg_muon_entry_t& e = d->entries[i];
     PG_REQUIRE(e.off <= d->total - (int64_t)e.taps * e.rows * e.cols, "pg_muon_step: entry %d ends behind the arena", i);
     PG_REQUIRE(e.kind == 0 || d->v, "pg_muon_step: an Adam entry needs v");
+    // 1 - beta^t divides: t >= 1 whatever a counter, which begins at 0, adds
+    PG_REQUIRE(e.kind == 0 || (d->step >= 1 && d->beta1 >= 0.0 && d->beta1 < 1.0 && d->beta2 >= 0.0 && d->beta2 < 1.0),
+               "pg_muon_step: an Adam entry needs step >= 1 and betas in [0, 1)");
     if (i > 0) {
       const pg_muon_entry_t& q = d->entries[i - 1];
       PG_REQUIRE(e.off >= q.off + (int64_t)q.taps * q.rows * q.cols, "pg_muon_step: entries %d and %d overlap or are out of order", i - 1, i);

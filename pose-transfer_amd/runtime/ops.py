@@ -171,7 +171,7 @@ def muon_workspace(table):
 def muon_step(p, g, m, v, table, lr, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5, ns_eps=1e-7, betas=(0.5, 0.999),
               eps=1e-8, step=1, grad_scale=1.0, ctr=None, p_bf16=None, workspace=None):
     """One optimiser step over a flat arena, in place on p, m (and v): the Muon update for the matrices of `table` (a numpy array
-    of MUON_ENTRY records, ascending and disjoint), Adam with (betas, eps, step) for its kind 1 records.  g: fp32 or bf16 arena.
+    of MUON_ENTRY records, ascending and disjoint), Adam with (betas, eps, step >= 1) for its kind 1 records.  g: fp32 or bf16 arena.
     `workspace`: a uint8 tensor of at least ``muon_workspace(table)`` bytes to use instead of a fresh one."""
     _need(isinstance(table, np.ndarray) and table.dtype == MUON_ENTRY and table.ndim == 1 and table.flags.c_contiguous,
           "muon_step: table must be a contiguous 1-D array of MUON_ENTRY records")

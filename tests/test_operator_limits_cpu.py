@@ -31,3 +31,26 @@ def test_partial_sums_of_squares_are_bounded(rows, cols):
     assert L.load().pg_orthogonalise_workspace(1, rows, cols) <= most
     t = np.array([(0, 1, rows, cols, 0, 1.0, 0)], dtype=O.MUON_ENTRY)
     assert L.load().pg_muon_workspace(t.ctypes.data, 1) <= most
+
+
+def table(rows):
+    return np.array([tuple(r) + (0,) for r in rows], dtype=O.MUON_ENTRY)
+
+
+GOOD = [(0, 16, 8, 20, 0, 1.0), (2624, 1, 1, 5, 1, 0.0)]
+
+
+def muon(entries=GOOD, **kw):
+    t = table(entries)
+    a = dict(p=P, g=P * 2, m=P * 3, v=P * 4, entries=t.ctypes.data, total=1 << 30, n=len(t), nesterov=1, steps=5, lr=0.1, momentum=0.9,
+             weight_decay=0.0, grad_scale=1.0, eps=1e-7, beta1=0.5, beta2=0.9, adam_eps=1e-8, step=1, workspace=P, workspace_bytes=1 << 40)
+    a.update(kw)
+    return L.load().pg_muon_step(C.byref(L.MuonDesc(**a)), None)
+
+
+@pytest.mark.parametrize("bad", [dict(step=0), dict(step=-3), dict(step=0, ctr=P), dict(beta1=1.0), dict(beta2=1.0), dict(beta2=-0.1),
+                                 dict(beta1=float("nan"))])
+def test_muon_step_refuses_corrections_that_divide_by_zero(bad):
+    """1 - beta^0 = 0: the Adam records would become infinite or NaN"""
+    assert muon(**bad) != 0
+    assert "step >= 1 and betas in [0, 1)" in L.load().pg_last_error().decode()
