@@ -3,8 +3,8 @@
 // (C,H,W); here every row (pixel) has its own scale and every channel its own gain:
 //   h = rnd_T(x + r),  s = 1 / sqrt(mean_c h^2 + eps),  y = h s gamma
 //   backward:  xh = h s,  w = dy gamma:  dx = dr = s (w - xh mean_c(w xh)) + dh,   dgamma = sum_rows dy xh
-// where dh is the gradient that reaches h past the norm (the residual stream).  Statistics and sums are fp32 (dgamma's last sum fp64);
-// the only roundings to fewer bits are the stores: T (fp32 or bf16) and e4m3.
+// where dh is the gradient that reaches h past the norm (the residual stream).  Statistics and a lane's sums are fp32, the joins of
+// dgamma's sums fp64; the only roundings to fewer bits are the stores: T (fp32 or bf16) and e4m3.
 // Both passes are HBM-bound (6 / 12 flops per element).  A row lives in the registers of a group of LPR lanes (the smallest
 // power of two that covers it in one 16-byte chunk per lane, then several chunks per lane of a whole wave): ONE read of every input,
 // statistics by lane exchanges, no LDS and no barrier.  16-byte accesses at any element alignment (gfx950 global memory takes
@@ -420,10 +420,10 @@ __global__ __launch_bounds__(WG) void rms_bwd_kernel(const RmsBwdK p) {
     for (int e = 0; e < V; ++e) red[(grp * NCH + i) * LPR * V + ln * V + e] = acc[i][e];
   __syncthreads();
   for (int c = threadIdx.x; c < p.C; c += WG) {
-    float t = 0.f;
-    for (int k = 0; k < G; ++k) t += red[k * NCH * LPR * V + c];
-    if (gridDim.x == 1) p.dgamma[c] = p.accumulate ? p.dgamma[c] + t : t;
-    else p.part[(long)blockIdx.x * p.C + c] = t;
+    double t = 0.0;
+    for (int k = 0; k < G; ++k) t += (double)red[k * NCH * LPR * V + c];
+    if (gridDim.x == 1) p.dgamma[c] = (float)(p.accumulate ? (double)p.dgamma[c] + t : t);
+    else p.part[(long)blockIdx.x * p.C + c] = (float)t;
   }
 }
 

@@ -152,3 +152,17 @@ def test_muon_step_to_the_accuracy_of_its_products(parts, gbf):
     for e in table:
         used[int(e["off"]):int(e["off"]) + int(e["taps"]) * int(e["rows"]) * int(e["cols"])] = True
     assert torch.equal(pb[used], p[used].bfloat16()) and bool((pb[~used] == 7).all())
+
+
+# ------------------------------------------------------------------------------------------------ channel norm
+@pytest.mark.parametrize("rows,ones", [(16, 16), (8192, 4)])
+def test_rms_norm_backward_joins_its_sums_in_64_bits(rows, ones):
+    """dgamma = 2^24 + ones - 1 from rows that lie in different groups of lanes: in fp32 every 1 would be rounded away.  The second
+    form joins workgroups: two roundings to fp32"""
+    h = torch.ones(rows, 200, device="cuda")
+    dy = torch.zeros(rows, 200, device="cuda")
+    dy[:ones] = 1.0
+    dy[0] = 2.0 ** 24
+    _, dgamma = ops().rms_norm_bwd(dy, h, torch.ones(rows, device="cuda"), torch.ones(200, device="cuda"))
+    want = 2.0 ** 24 + ones - 1
+    assert float((dgamma.double() - want).abs().max()) <= (1 if rows == 16 else 2) * U * want
