@@ -151,13 +151,15 @@ __device__ __forceinline__ float group_sum(float v, int lpr = LPR) {
 }
 // 8 bits: q = e4m3(448 z / max|z|), z = h gamma of a group, in fp64 and rounded to fp32 once: the row's s cancels, and a
 // value next to a border of e4m3's steps goes to the side that the definition gives (in fp32, with y and the scale rounded first,
-// one value in 500 000 changed sides).  scale = s max|z| / 448.  s joins in so that a row whose statistic is NaN is NaN.
+// one value in 500 000 changed sides).  scale = s max|z| / 448; where that is zero (a group of zeros, or s is: the row holds an infinity, or its
+// squares pass fp32) y is zero: scale 1, q zeros.  s joins in so that a row whose statistic is NaN is NaN.
 struct Q8 {
   double r;
   float scale;
   __device__ __forceinline__ Q8(double am, float s) {
-    r = am > 0.0 ? 448.0 / am : 0.0;
-    scale = am > 0.0 ? (float)((double)s * am / 448.0) : 1.f;
+    r = 448.0 / am;
+    scale = (float)((double)s * am / 448.0);
+    if (am == 0.0 || scale == 0.f) { r = 0.0; scale = 1.f; }      // (without eps s is infinite where am is zero)
     if (s != s) { r = (double)s; scale = s; }
   }
 };

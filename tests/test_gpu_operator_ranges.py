@@ -166,3 +166,63 @@ def test_rms_norm_backward_joins_its_sums_in_64_bits(rows, ones):
     _, dgamma = ops().rms_norm_bwd(dy, h, torch.ones(rows, device="cuda"), torch.ones(200, device="cuda"))
     want = 2.0 ** 24 + ones - 1
     assert float((dgamma.double() - want).abs().max()) <= (1 if rows == 16 else 2) * U * want
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group", [0, 32, 128])
+@pytest.mark.parametrize("C", [96, 300, 2500])
+def test_rms_norm_q8_of_rows_whose_scale_vanishes(dtype, group, C):
+    """y is zero where the row's statistic is infinite: scale 1 and zero bytes, as for a group of zeros; the group with the infinity
+    itself is NaN"""
+    x = rnd(20, 5, C, dtype=dtype)
+    x[1, 70] = float("inf")
+    x[2] *= 1e30                                              # the squares pass fp32
+    x[3] = 0
+    q, scale, _, rstd = ops().rms_norm_q8(x, torch.ones(C, device="cuda"), group=group)
+    assert float(rstd[1]) == 0 and float(rstd[2]) == 0
+    back = q.float()
+    for row in (2, 3):
+        assert bool((scale[row] == 1).all()) and float(back[row].abs().max()) == 0
+    if group == 0:
+        assert bool(torch.isnan(scale[1]).all()) and bool(torch.isnan(back[1, 70]))
+    else:
+        k = 70 // group
+        assert bool(torch.isnan(scale[1, k])) and bool(torch.isnan(back[1, 70]))
+        keep = torch.arange(scale.shape[1], device="cuda") != k
+        assert bool((scale[1, keep] == 1).all())
+        assert float(back[1, :k * group].abs().sum()) == 0 and float(back[1, (k + 1) * group:].abs().sum()) == 0
+    ok = [0, 4]
+    q0, s0, _, _ = ops().rms_norm_q8(x[ok].contiguous(), torch.ones(C, device="cuda"), group=group)
+    assert torch.equal(q[ok].view(torch.uint8), q0.view(torch.uint8)) and torch.equal(scale[ok], s0)
+
+
+def e4m3_bytes(v):
+    """round to nearest even in 64 bits (|v| <= 448): the value, and how far v is from a tie, relative to its size"""
+    e = torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -9))).clamp_min(-6)
+    step = torch.exp2(e - 3)
+    t = v / step
+    return torch.round(t) * step, ((t - torch.floor(t) - 0.5).abs() * step / v.abs().clamp_min(2.0 ** -9))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,C,group", [(3000, 128, 64), (500, 1030, 0), (700, 513, 32), (40, 4100, 128)])
+def test_rms_norm_q8_rounds_as_the_definition_does(dtype, rows, C, group):
+    """every byte against the 64-bit definition, but for values within 2^-50 of a tie of e4m3 (the rounding of fp64; rounding to fp32 first
+    keeps a side of a tie or lands on it, 2^-24 more)"""
+    x, r = rnd(21, rows, C, dtype=dtype), rnd(22, rows, C, dtype=dtype)
+    gamma = rnd(23, C) + 1.0
+    q, scale, h, _ = ops().rms_norm_q8(x, gamma, r, group=group)
+    z = h.double() * gamma.double()
+    g = group or C
+    n = -(-C // g)
+    zp = torch.nn.functional.pad(z, (0, n * g - C)).view(rows, n, g)
+    v = (zp * (448.0 / zp.abs().amax(2, keepdim=True))).view(rows, n * g)[:, :C]
+    want, tie = e4m3_bytes(v)
+    clear = tie > 2.0 ** -23
+    assert float((~clear).double().mean()) < 1e-5
+    assert torch.equal(q.double()[clear], want[clear])
+
+
+def test_rms_norm_q8_of_a_row_of_zeros_without_eps():
+    q, scale, _, rstd = ops().rms_norm_q8(torch.zeros(2, 96, device="cuda"), torch.ones(96, device="cuda"), eps=0.0, group=32)
+    assert bool(torch.isinf(rstd).all()) and bool((scale == 1).all()) and float(q.float().abs().max()) == 0
