@@ -429,14 +429,14 @@ __global__ __launch_bounds__(WG) void rms_bwd_kernel(const RmsBwdK p) {
   }
 }
 
-// dgamma[c] = sum of nblk partial rows: 32 columns x 32 slices per workgroup, fp64
-__global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* part, int nblk, int C, float* dgamma, int accumulate) {
+// dgamma[c] = sum of nblk partial rows, ld apart: 32 columns x 32 slices per workgroup, fp64
+__global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* part, int nblk, int ld, int C, float* dgamma, int accumulate) {
   __shared__ double red[32][33];
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), sl = threadIdx.x >> 5;
   double t = 0.0;
   if (c < C) {
 #pragma unroll 8
-    for (int k = sl; k < nblk; k += 32) t += (double)part[(long)k * C + c];
+    for (int k = sl; k < nblk; k += 32) t += (double)part[(long)k * ld + c];
   }
   red[sl][threadIdx.x & 31] = t;
   __syncthreads();
@@ -532,6 +532,13 @@ static int rms_long_slices(long rows) { return rows < 64 ? (int)rows : 64; }
 constexpr int MAX_C = 1 << 30;
 // a launch has less than 2^32 lanes: more rows go in several
 constexpr long MAX_BLOCKS = 1L << 23;
+static void rms_dgamma(const float* part, int nblk, int C, float* dgamma, int accumulate, hipStream_t st) {
+  constexpr int PIECE = 1 << 26;                       // 2^21 workgroups of 1024
+  for (int c0 = 0; c0 < C; c0 += PIECE) {
+    const int n = C - c0 < PIECE ? C - c0 : PIECE;
+    PG_KLAUNCH(rms_dgamma_kernel, dim3((n + 31) / 32), dim3(1024), 0, st, part ? part + c0 : nullptr, nblk, C, n, dgamma + c0, accumulate);
+  }
+}
 template <typename P>
 static P* rms_at(P* p, long elems, size_t size) {
   return p ? reinterpret_cast<P*>(const_cast<char*>(reinterpret_cast<const char*>(p)) + elems * (long)size) : nullptr;
@@ -651,7 +658,7 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
   PG_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "pg_rms_norm_bwd: workspace of %lld bytes required", (long long)need);
   hipStream_t st = (hipStream_t)stream;
   if (rows == 0) {                 // an empty sum
-    if (!accumulate) PG_KLAUNCH(rms_dgamma_kernel, dim3((C + 31) / 32), dim3(1024), 0, st, (const float*)nullptr, 0, C, dgamma, 0);
+    if (!accumulate) rms_dgamma(nullptr, 0, C, dgamma, 0, st);
     PG_LAUNCH_OK("pg_rms_norm_bwd");
     return 0;
   }
@@ -716,8 +723,7 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
 #undef PG_RB
 #undef PG_RB1
 #undef PG_RBN
-  if (!(nch && nb == 1))
-    PG_KLAUNCH(rms_dgamma_kernel, dim3((C + 31) / 32), dim3(1024), 0, st, (const float*)workspace, (int)nb, C, dgamma, accumulate);
+  if (!(nch && nb == 1)) rms_dgamma((const float*)workspace, (int)nb, C, dgamma, accumulate, st);
   PG_LAUNCH_OK("pg_rms_norm_bwd");
   return 0;
 }

@@ -226,3 +226,23 @@ def test_rms_norm_q8_rounds_as_the_definition_does(dtype, rows, C, group):
 def test_rms_norm_q8_of_a_row_of_zeros_without_eps():
     q, scale, _, rstd = ops().rms_norm_q8(torch.zeros(2, 96, device="cuda"), torch.ones(96, device="cuda"), eps=0.0, group=32)
     assert bool(torch.isinf(rstd).all()) and bool((scale == 1).all()) and float(q.float().abs().max()) == 0
+
+
+def test_rms_norm_of_rows_of_2_to_the_27_channels():
+    """dgamma's join takes more columns than one launch of 1024-lane workgroups holds"""
+    C = (1 << 27) + 77
+    h = torch.ones(1, C, device="cuda")
+    h[0, -1] = 3.0
+    dy = torch.full((1, C), 2.0, device="cuda")
+    one = torch.ones(1, device="cuda")
+    gamma = torch.ones(C, device="cuda")
+    dx, dgamma = ops().rms_norm_bwd(dy, h, one, gamma)
+    assert bool((dgamma[:-1] == 2).all()) and float(dgamma[-1]) == 6
+    # w - xh mean(w xh): the mean is 2 and 2^-25 more, rounded to fp32
+    assert float(dx[0, :-1].abs().max()) <= 2.0 ** -22 and abs(float(dx[0, -1]) + 4) <= 2.0 ** -21
+    del dx, h
+    e = torch.empty(0, C, device="cuda")
+    dgamma = ops().rms_norm_bwd(e, e, one[:0], gamma)[1]
+    assert float(dgamma.abs().max()) == 0
+    del dgamma, gamma, dy
+    torch.cuda.empty_cache()
