@@ -584,6 +584,12 @@ extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamm
     if (q) PG_KLAUNCH((rms_fwd_kernel<T, L, N, true, EX>), grid, wg, 0, st, k);                                    \
     else PG_KLAUNCH((rms_fwd_kernel<T, L, N, false, EX>), grid, wg, 0, st, k);                                     \
   } while (0)
+  bool none = false;       // a form that the shape's rule gives no row of this type: an error, should the rule change
+#define PG_RF14(T, L, M, EX)                                                                                       \
+  do {                                                                                                             \
+    if (RmsV<T>::N == 4) PG_RF1(T, L, (RmsV<T>::N == 4 ? M : 1), EX);                                              \
+    else none = true;                                                                                              \
+  } while (0)
 #define PG_RF(T)                                                                                                   \
   do {                                                                                                             \
     switch (lpr * 32 + nch * 2 + (sh.ex ? 1 : 0)) {                                                                \
@@ -594,10 +600,10 @@ extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamm
       case 64 * 32 + 5: PG_RF1(T, 64, 2, true); break;                                                             \
       case 64 * 32 + 7: PG_RF1(T, 64, 3, true); break;                                                             \
       case 64 * 32 + 9: PG_RF1(T, 64, 4, true); break;                                                             \
-      case 64 * 32 + 11: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 5 : 4), true); break;                                    \
-      case 64 * 32 + 13: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 6 : 4), true); break;                                    \
-      case 64 * 32 + 15: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 7 : 4), true); break;                                    \
-      case 64 * 32 + 17: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 8 : 4), true); break;                                    \
+      case 64 * 32 + 11: PG_RF14(T, 64, 5, true); break;                                                           \
+      case 64 * 32 + 13: PG_RF14(T, 64, 6, true); break;                                                           \
+      case 64 * 32 + 15: PG_RF14(T, 64, 7, true); break;                                                           \
+      case 64 * 32 + 17: PG_RF14(T, 64, 8, true); break;                                                           \
       case 8 * 32 + 2: PG_RF1(T, 8, 1, false); break;                                                              \
       case 8 * 32 + 4: PG_RF1(T, 8, 2, false); break;                                                              \
       case 8 * 32 + 6: PG_RF1(T, 8, 3, false); break;                                                              \
@@ -611,11 +617,12 @@ extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamm
       case 64 * 32 + 4: PG_RF1(T, 64, 2, false); break;                                                            \
       case 64 * 32 + 6: PG_RF1(T, 64, 3, false); break;                                                            \
       case 64 * 32 + 8: PG_RF1(T, 64, 4, false); break;                                                            \
-      case 64 * 32 + 10: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 5 : 4), false); break;                                   \
-      case 64 * 32 + 12: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 6 : 4), false); break;                                   \
-      case 64 * 32 + 14: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 7 : 4), false); break;                                   \
-      case 64 * 32 + 16: PG_RF1(T, 64, (RmsV<T>::N == 4 ? 8 : 4), false); break;                                   \
+      case 64 * 32 + 10: PG_RF14(T, 64, 5, false); break;                                                          \
+      case 64 * 32 + 12: PG_RF14(T, 64, 6, false); break;                                                          \
+      case 64 * 32 + 14: PG_RF14(T, 64, 7, false); break;                                                          \
+      case 64 * 32 + 16: PG_RF14(T, 64, 8, false); break;                                                          \
       default:                                                                                                     \
+        if (nch) { none = true; break; }                                                                           \
         if (q) PG_KLAUNCH((rms_fwd_long_kernel<T, true>), grid, wg, 0, st, k);                                     \
         else PG_KLAUNCH((rms_fwd_long_kernel<T, false>), grid, wg, 0, st, k);                                      \
         break;                                                                                                     \
@@ -629,8 +636,10 @@ extern "C" int pg_rms_norm_fwd(const void* x, const void* res, const float* gamm
                        rms_at(rstd, r0, 4)};
     if (io_flags == 0) PG_RF(float);
     else PG_RF(bf16_t);
+    PG_REQUIRE(!none, "pg_rms_norm_fwd: no kernel for a row of %d lanes x %d chunks", lpr, nch);
   }
 #undef PG_RF
+#undef PG_RF14
 #undef PG_RF1
   PG_LAUNCH_OK("pg_rms_norm_fwd");
   return 0;
@@ -670,7 +679,13 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
   PG_REQUIRE(dx != dy || lddy == C, "pg_rms_norm_bwd: dx in place of dy needs lddy == C");
   RmsBwdK k = {dy, dh, h, rstd, gamma, (long)rows, C, (long)lddy, dx, (float*)workspace, dgamma, accumulate};
   const bool single = rms_bwd_single(rows, lpr, nch);
+  bool none = false;
 #define PG_RBN(T, L, N, EX) PG_KLAUNCH((rms_bwd_kernel<T, L, N, 256, EX>), dim3((unsigned)nb), dim3(256), 0, st, k)
+#define PG_RBN4(T, L, M, EX)                                                                                       \
+  do {                                                                                                             \
+    if (RmsV<T>::N == 4) PG_RBN(T, L, (RmsV<T>::N == 4 ? M : 1), EX);                                              \
+    else none = true;                                                                                              \
+  } while (0)
 #define PG_RB1(T, L, EX)                                                                                           \
   do {                                                                                                             \
     if (single) PG_KLAUNCH((rms_bwd_kernel<T, L, 1, 1024, EX>), dim3(1), dim3(1024), 0, st, k);                    \
@@ -686,28 +701,29 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
       case 64 * 32 + 5: PG_RBN(T, 64, 2, true); break;                                                             \
       case 64 * 32 + 7: PG_RBN(T, 64, 3, true); break;                                                             \
       case 64 * 32 + 9: PG_RBN(T, 64, 4, true); break;                                                             \
-      case 64 * 32 + 11: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 5 : 4), true); break;                                    \
-      case 64 * 32 + 13: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 6 : 4), true); break;                                    \
-      case 64 * 32 + 15: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 7 : 4), true); break;                                    \
-      case 64 * 32 + 17: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 8 : 4), true); break;                                    \
+      case 64 * 32 + 11: PG_RBN4(T, 64, 5, true); break;                                                           \
+      case 64 * 32 + 13: PG_RBN4(T, 64, 6, true); break;                                                           \
+      case 64 * 32 + 15: PG_RBN4(T, 64, 7, true); break;                                                           \
+      case 64 * 32 + 17: PG_RBN4(T, 64, 8, true); break;                                                           \
       case 8 * 32 + 2: PG_RB1(T, 8, false); break;                                                                 \
-      case 8 * 32 + 4: PG_RBN(T, 8, (RmsV<T>::N == 4 ? 2 : 1), false); break;                                      \
-      case 8 * 32 + 6: PG_RBN(T, 8, (RmsV<T>::N == 4 ? 3 : 1), false); break;                                      \
+      case 8 * 32 + 4: PG_RBN4(T, 8, 2, false); break;                                                             \
+      case 8 * 32 + 6: PG_RBN4(T, 8, 3, false); break;                                                             \
       case 16 * 32 + 2: PG_RB1(T, 16, false); break;                                                               \
-      case 16 * 32 + 4: PG_RBN(T, 16, (RmsV<T>::N == 4 ? 2 : 1), false); break;                                    \
-      case 16 * 32 + 6: PG_RBN(T, 16, (RmsV<T>::N == 4 ? 3 : 1), false); break;                                    \
+      case 16 * 32 + 4: PG_RBN4(T, 16, 2, false); break;                                                           \
+      case 16 * 32 + 6: PG_RBN4(T, 16, 3, false); break;                                                           \
       case 32 * 32 + 2: PG_RB1(T, 32, false); break;                                                               \
-      case 32 * 32 + 4: PG_RBN(T, 32, (RmsV<T>::N == 4 ? 2 : 1), false); break;                                    \
-      case 32 * 32 + 6: PG_RBN(T, 32, (RmsV<T>::N == 4 ? 3 : 1), false); break;                                    \
+      case 32 * 32 + 4: PG_RBN4(T, 32, 2, false); break;                                                           \
+      case 32 * 32 + 6: PG_RBN4(T, 32, 3, false); break;                                                           \
       case 64 * 32 + 2: PG_RB1(T, 64, false); break;                                                               \
       case 64 * 32 + 4: PG_RBN(T, 64, 2, false); break;                                                            \
       case 64 * 32 + 6: PG_RBN(T, 64, 3, false); break;                                                            \
       case 64 * 32 + 8: PG_RBN(T, 64, 4, false); break;                                                            \
-      case 64 * 32 + 10: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 5 : 4), false); break;                                   \
-      case 64 * 32 + 12: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 6 : 4), false); break;                                   \
-      case 64 * 32 + 14: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 7 : 4), false); break;                                   \
-      case 64 * 32 + 16: PG_RBN(T, 64, (RmsV<T>::N == 4 ? 8 : 4), false); break;                                   \
+      case 64 * 32 + 10: PG_RBN4(T, 64, 5, false); break;                                                          \
+      case 64 * 32 + 12: PG_RBN4(T, 64, 6, false); break;                                                          \
+      case 64 * 32 + 14: PG_RBN4(T, 64, 7, false); break;                                                          \
+      case 64 * 32 + 16: PG_RBN4(T, 64, 8, false); break;                                                          \
       default:                                                                                                     \
+        if (nch) { none = true; break; }                                                                           \
         for (long r0 = 0; r0 < rows; r0 += MAX_BLOCKS) {                                                           \
           const long n = rows - r0 < MAX_BLOCKS ? rows - r0 : MAX_BLOCKS;                                          \
           const RmsBwdK kr = {rms_at(dy, r0 * lddy, sizeof(T)), rms_at(dh, r0 * C, sizeof(T)), rms_at(h, r0 * C, sizeof(T)), \
@@ -720,8 +736,10 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
   } while (0)
   if (io_flags == 0) PG_RB(float);
   else PG_RB(bf16_t);
+  PG_REQUIRE(!none, "pg_rms_norm_bwd: no kernel for a row of %d lanes x %d chunks", lpr, nch);
 #undef PG_RB
 #undef PG_RB1
+#undef PG_RBN4
 #undef PG_RBN
   if (!(nch && nb == 1)) rms_dgamma((const float*)workspace, (int)nb, C, dgamma, accumulate, st);
   PG_LAUNCH_OK("pg_rms_norm_bwd");
