@@ -320,11 +320,15 @@ int pg_rms_norm_fwd(const void* x, const void* res, const float* gamma, int64_t 
                     int32_t io_flags, void* h, void* y, int64_t ldy, void* q, float* scales, int32_t group, float* rstd, void* stream);
 /* backward: dx (= the residual's gradient) = s (w - h s mean_c(w h s)) + dh with w = dy gamma; dgamma[c] (+)= sum_rows dy h s.  dy has row
  * stride lddy; dh (the gradient that reaches h past the norm; NULL: none), h, dx packed.  dx may be dy (lddy == C), dh or h for C <= 2048.
- * No atomics.  workspace: pg_rms_norm_bwd_workspace bytes.                                                                      */
+ * No atomics.  workspace: pg_rms_norm_bwd_workspace bytes.  _ex: h with a row stride too (a forward pass without residual reads a
+ * channel slice in place and hands it on as h); dx may be h where ldh == C.                                                      */
 int64_t pg_rms_norm_bwd_workspace(int64_t rows, int32_t C, int32_t io_flags);
 int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, const void* h, const float* rstd, const float* gamma, int64_t rows,
                     int32_t C, int32_t io_flags, void* dx, float* dgamma, int32_t accumulate, void* workspace, int64_t workspace_bytes,
                     void* stream);
+int pg_rms_norm_bwd_ex(const void* dy, int64_t lddy, const void* dh, const void* h, int64_t ldh, const float* rstd, const float* gamma,
+                       int64_t rows, int32_t C, int32_t io_flags, void* dx, float* dgamma, int32_t accumulate, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 
 /* ---- losses (models/pose_gan.py)
  * GAN log loss on D logits [rows][K] (sigmoid fused; pose_gan.py:90-98,140-160):

@@ -360,7 +360,7 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(const RmsFwdK p) {
 
 struct RmsBwdK {
   const void* dy; const void* dh; const void* h; const float* rstd; const float* gamma;
-  long rows; int C; long lddy;
+  long rows; int C; long lddy, ldh;
   void* dx; float* part; float* dgamma; int accumulate;
 };
 
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(WG) void rms_bwd_kernel(const RmsBwdK p) {
   }
   for (long row = (long)blockIdx.x * G + grp; row < p.rows; row += (long)gridDim.x * G) {
     const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.lddy;
-    const T* h = reinterpret_cast<const T*>(p.h) + row * p.C;
+    const T* h = reinterpret_cast<const T*>(p.h) + row * p.ldh;
     float a[NCH][V], b[NCH][V], d[NCH][V];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) { rms_load(EX || i < NCH - 1, dy, (i * LPR + ln) * V, p.C, a[i]); rms_load(EX || i < NCH - 1, h, (i * LPR + ln) * V, p.C, b[i]); }
@@ -454,7 +454,7 @@ __global__ __launch_bounds__(256) void rms_bwd_long_kernel(const RmsBwdK p) {
   __shared__ double red[4];
   const long row = blockIdx.x;
   const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.lddy;
-  const T* h = reinterpret_cast<const T*>(p.h) + row * p.C;
+  const T* h = reinterpret_cast<const T*>(p.h) + row * p.ldh;
   const T* dh = p.dh ? reinterpret_cast<const T*>(p.dh) + row * p.C : nullptr;
   const float s = p.rstd[row];
   double dot = 0.0;
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(256) void rms_dgamma_long_kernel(const RmsBwdK p) {
   const T* h = reinterpret_cast<const T*>(p.h) + c;
   double t = 0.0;
   for (long row = blockIdx.y; row < p.rows; row += gridDim.y)
-    t += (double)(rms_ld1(dy + row * p.lddy) * (rms_ld1(h + row * p.C) * p.rstd[row]));
+    t += (double)(rms_ld1(dy + row * p.lddy) * (rms_ld1(h + row * p.ldh) * p.rstd[row]));
   p.part[(long)blockIdx.y * p.C + c] = (float)t;
 }
 
@@ -656,8 +656,14 @@ extern "C" int64_t pg_rms_norm_bwd_workspace(int64_t rows, int32_t C, int32_t io
 extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, const void* h, const float* rstd, const float* gamma,
                                int64_t rows, int32_t C, int32_t io_flags, void* dx, float* dgamma, int32_t accumulate,
                                void* workspace, int64_t workspace_bytes, void* stream) {
-  PG_REQUIRE(dy && h && rstd && gamma && dx && dgamma && rows >= 0 && C > 0 && C <= MAX_C && lddy >= C,
-             "pg_rms_norm_bwd: dy, h, rstd, gamma, dx, dgamma, rows >= 0, 0 < C <= 2^30 and lddy >= C required");
+  return pg_rms_norm_bwd_ex(dy, lddy, dh, h, C, rstd, gamma, rows, C, io_flags, dx, dgamma, accumulate, workspace, workspace_bytes, stream);
+}
+
+extern "C" int pg_rms_norm_bwd_ex(const void* dy, int64_t lddy, const void* dh, const void* h, int64_t ldh, const float* rstd,
+                                  const float* gamma, int64_t rows, int32_t C, int32_t io_flags, void* dx, float* dgamma,
+                                  int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream) {
+  PG_REQUIRE(dy && h && rstd && gamma && dx && dgamma && rows >= 0 && C > 0 && C <= MAX_C && lddy >= C && ldh >= C,
+             "pg_rms_norm_bwd: dy, h, rstd, gamma, dx, dgamma, rows >= 0, 0 < C <= 2^30, lddy >= C and ldh >= C required");
   PG_REQUIRE(io_flags == 0 || io_flags == 3, "pg_rms_norm_bwd: io_flags 0 (fp32) or 3 (bf16)");
   const size_t em = io_flags ? 1 : 3;
   PG_REQUIRE((((size_t)dy | (size_t)dh | (size_t)h | (size_t)dx) & em) == 0 &&
@@ -676,8 +682,8 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
   const long nb = nch ? rms_bwd_blocks(rows, lpr, nch) : rms_long_slices(rows);
   PG_REQUIRE(rows <= (1L << 40), "pg_rms_norm_bwd: too many rows");
   PG_REQUIRE(nch || (dx != dy && dx != dh && dx != h), "pg_rms_norm_bwd: rows of more than 2048 channels are read twice: dx must not be an input");
-  PG_REQUIRE(dx != dy || lddy == C, "pg_rms_norm_bwd: dx in place of dy needs lddy == C");
-  RmsBwdK k = {dy, dh, h, rstd, gamma, (long)rows, C, (long)lddy, dx, (float*)workspace, dgamma, accumulate};
+  PG_REQUIRE((dx != dy || lddy == C) && (dx != h || ldh == C), "pg_rms_norm_bwd: dx in place of dy or h needs rows of C elements there");
+  RmsBwdK k = {dy, dh, h, rstd, gamma, (long)rows, C, (long)lddy, (long)ldh, dx, (float*)workspace, dgamma, accumulate};
   const bool single = rms_bwd_single(rows, lpr, nch);
   bool none = false;
 #define PG_RBN(T, L, N, EX) PG_KLAUNCH((rms_bwd_kernel<T, L, N, 256, EX>), dim3((unsigned)nb), dim3(256), 0, st, k)
@@ -726,8 +732,8 @@ extern "C" int pg_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, con
         if (nch) { none = true; break; }                                                                           \
         for (long r0 = 0; r0 < rows; r0 += MAX_BLOCKS) {                                                           \
           const long n = rows - r0 < MAX_BLOCKS ? rows - r0 : MAX_BLOCKS;                                          \
-          const RmsBwdK kr = {rms_at(dy, r0 * lddy, sizeof(T)), rms_at(dh, r0 * C, sizeof(T)), rms_at(h, r0 * C, sizeof(T)), \
-                              rms_at(rstd, r0, 4), gamma, n, C, (long)lddy, rms_at(dx, r0 * C, sizeof(T)), nullptr, nullptr, 0}; \
+          const RmsBwdK kr = {rms_at(dy, r0 * lddy, sizeof(T)), rms_at(dh, r0 * C, sizeof(T)), rms_at(h, r0 * ldh, sizeof(T)), \
+                              rms_at(rstd, r0, 4), gamma, n, C, (long)lddy, (long)ldh, rms_at(dx, r0 * C, sizeof(T)), nullptr, nullptr, 0}; \
           PG_KLAUNCH((rms_bwd_long_kernel<T>), dim3((unsigned)n), dim3(256), 0, st, kr);                           \
         }                                                                                                          \
         PG_KLAUNCH((rms_dgamma_long_kernel<T>), dim3((C + 255) / 256, (unsigned)nb), dim3(256), 0, st, k);         \

@@ -283,7 +283,6 @@ class _RMSNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps):
         rows = _RMSNormFn._rows
         y, h, rstd = OPS.rms_norm(rows(x), weight, None if residual is None else rows(residual), eps=eps)
-        h = h.contiguous()
         ctx.save_for_backward(h, rstd, weight)
         ctx.has_res = residual is not None
         ctx.set_materialize_grads(False)

@@ -168,6 +168,7 @@ _PROTOS = {
     "pg_rms_norm_fwd": [_vp, _vp, _vp, _i64, _i32, _i64, _i64, _f32, _i32, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _vp],
     "pg_rms_norm_bwd_workspace": [_i64, _i32, _i32],
     "pg_rms_norm_bwd": [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _i32, _vp, _i64, _vp],
+    "pg_rms_norm_bwd_ex": [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _i32, _vp, _i64, _vp],
     "pg_orthogonalise_workspace": [_i64, _i64, _i64],
     "pg_orthogonalise": [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _i64, _i64, _i32, _f32, _vp, _i64, _vp],
     "pg_muon_workspace": [_vp, _i32],

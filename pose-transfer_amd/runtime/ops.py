@@ -112,26 +112,28 @@ def rms_norm_q8(x, gamma, residual=None, eps=1e-6, group=0):
 
 
 def rms_norm_bwd(dy, h, rstd, gamma, dh=None):
-    """(dx, dgamma) of ``rms_norm``: dx is also the residual's gradient; dh: the gradient that reaches h past the norm."""
+    """(dx, dgamma) of ``rms_norm``: dx is also the residual's gradient; dh (packed): the gradient that reaches h past the norm.  h
+    may be a channel slice, as ``rms_norm`` hands it on."""
     if not (torch.is_tensor(h) and h.is_cuda and h.dtype in _IO and h.dim() == 2 and h.shape[1] > 0):
         raise ValueError("rms_norm_bwd: h must be an fp32 or bf16 [rows, channels] tensor on the GPU")
     shape = h.shape
     rows, ch = shape
     _channels(ch)
-    if _rows(h, "h", h, shape) != ch or (dh is not None and _rows(dh, "dh", h, shape) != ch):
-        raise ValueError("rms_norm_bwd: h and dh must be packed")
+    ldh = _rows(h, "h", h, shape)
+    if dh is not None and _rows(dh, "dh", h, shape) != ch:
+        raise ValueError("rms_norm_bwd: dh must be packed")
     lddy = _rows(dy, "dy", h, shape)
     _vector(rstd, "rstd", h, rows)
     _vector(gamma, "gamma", h, ch)
     with _On(h):
-        dx = torch.empty_like(h)
+        dx = h.new_empty((rows, ch))
         dgamma = torch.empty_like(gamma)
         if rows == 0:
             return dx, dgamma.zero_()
         io = _IO[h.dtype]
         need = L.load().pg_rms_norm_bwd_workspace(rows, ch, io)
         ws = torch.empty(need, dtype=torch.uint8, device=h.device) if need else None
-        L.call("pg_rms_norm_bwd", dy.data_ptr(), lddy, L.ptr(dh), h.data_ptr(), rstd.data_ptr(), gamma.data_ptr(), rows, ch, io,
+        L.call("pg_rms_norm_bwd_ex", dy.data_ptr(), lddy, L.ptr(dh), h.data_ptr(), ldh, rstd.data_ptr(), gamma.data_ptr(), rows, ch, io,
                dx.data_ptr(), dgamma.data_ptr(), 0, L.ptr(ws), need, L.stream())
     return dx, dgamma
 

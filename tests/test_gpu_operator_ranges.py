@@ -246,3 +246,34 @@ def test_rms_norm_of_rows_of_2_to_the_27_channels():
     assert float(dgamma.abs().max()) == 0
     del dgamma, gamma, dy
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,C", [(1, 5), (7, 64), (77, 189), (3000, 129), (300, 2048), (5, 2500), (300, 3001)])
+def test_rms_norm_backward_of_a_channel_slice(dtype, rows, C):
+    """x is a slice of a wider tensor and no residual is added: rms_norm hands the slice on as h, and the backward pass reads it there;
+    the same numbers as from a packed copy"""
+    O = ops()
+    x = rnd(30, rows, C + 9, dtype=dtype)[:, 3:C + 3]
+    gamma, dy, dh = rnd(31, C) + 1.0, rnd(32, rows, C, dtype=dtype), rnd(33, rows, C, dtype=dtype)
+    y, h, rstd = O.rms_norm(x, gamma)
+    assert h.data_ptr() == x.data_ptr()
+    yc, hc, rc = O.rms_norm(x.contiguous(), gamma)
+    assert torch.equal(y, yc) and torch.equal(rstd, rc)
+    for d in (None, dh):
+        for a, b in zip(O.rms_norm_bwd(dy, h, rstd, gamma, dh=d), O.rms_norm_bwd(dy, hc, rc, gamma, dh=d)):
+            assert torch.equal(a, b)
+    assert bool((y.double() - x.double() * rstd.double()[:, None] * gamma.double()).abs().max() <= 8 * float(EPS[dtype]) * float(y.abs().max()))
+
+
+def test_rms_norm_module_of_a_channel_slice():
+    from pose_transfer_amd.models.networks import RMSNorm
+    mod = RMSNorm(40)
+    wide = rnd(34, 2, 3, 5, 100)
+    a, b = wide.clone().requires_grad_(), wide[..., 20:60].clone().requires_grad_()
+    wy = rnd(35, 2, 3, 5, 40)
+    ya, yb = mod(a[..., 20:60]), mod(b)
+    assert torch.equal(ya, yb)
+    ga, = torch.autograd.grad((ya * wy).sum(), a)
+    gb, = torch.autograd.grad((yb * wy).sum(), b)
+    assert torch.equal(ga[..., 20:60], gb) and float(ga[..., :20].abs().max()) == 0 and float(ga[..., 60:].abs().max()) == 0

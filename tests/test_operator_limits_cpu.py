@@ -54,3 +54,11 @@ def test_muon_step_refuses_corrections_that_divide_by_zero(bad):
     """1 - beta^0 = 0: the Adam records would become infinite or NaN"""
     assert muon(**bad) != 0
     assert "step >= 1 and betas in [0, 1)" in L.load().pg_last_error().decode()
+
+
+@pytest.mark.parametrize("bad", [dict(ldh=63), dict(ldh=70, dx=P * 3), dict(lddy=63), dict(h=None)])
+def test_rms_norm_bwd_ex_refuses(bad):
+    a = dict(dy=P, lddy=64, h=P * 3, ldh=64, dx=P * 2)
+    a.update(bad)
+    assert L.load().pg_rms_norm_bwd_ex(a["dy"], a["lddy"], None, a["h"], a["ldh"], P, P, 4, 64, 0, a["dx"], P, 0, None, 0, None) != 0
+    assert L.load().pg_last_error().decode().startswith("pg_rms_norm_bwd")
