@@ -277,3 +277,51 @@ def test_rms_norm_module_of_a_channel_slice():
     ga, = torch.autograd.grad((ya * wy).sum(), a)
     gb, = torch.autograd.grad((yb * wy).sum(), b)
     assert torch.equal(ga[..., 20:60], gb) and float(ga[..., :20].abs().max()) == 0 and float(ga[..., 60:].abs().max()) == 0
+
+
+# ------------------------------------------------------------------------------------------------ the trainer's recorded step
+@pytest.mark.parametrize("precision", [0, 3])
+def test_replayed_muon_step_against_the_definition(precision):
+    """a replayed iteration's optimiser launches: each record's displacement against the 64-bit step on the arena's own gradients, at the
+    step number that the device counter gives, twice; a replay that left them out, or took them twice, is off by its whole size"""
+    from types import SimpleNamespace
+
+    from pose_transfer_amd.models.pose_gan import DeformablePose_GAN
+    from pose_transfer_amd.runtime import engine as E
+    from pose_transfer_amd.runtime.tape import TapedIteration
+    from pose_transfer_amd.utils import synth
+    was, E.PRECISION = E.PRECISION, precision
+    try:
+        opt = SimpleNamespace(image_size=(64, 64), use_input_pose=True, pose_dim=18, batch_size=2, num_stacks=4, gen_type="baseline",
+                              dataset="fasion", warp_skip="mask", learning_rate=2e-4, content_loss_layer="none", nn_loss_area_size=1,
+                              gan_penalty_weight=1.0, l1_penalty_weight=100.0, optimizer="muon", muon_momentum=0.9, muon_weight_decay=0.01)
+        model = DeformablePose_GAN(opt, device="cuda:0")
+        b = [torch.from_numpy(np.ascontiguousarray(a)).cuda() for a in synth.batch(1, "muon/T", 2, 18, 64, 64)]
+        b = [b[0], b[1], b[2].float().contiguous(), b[3]]
+        tape = TapedIteration(model, [b, b, b], dict(vars(opt)), warmup=1)               # one eager iteration, one recorded
+        try:
+            arenas = (model.disc.arena, model.gen.arena)
+            for step in (3, 4):
+                before = [(a.params.clone(), a.m.clone(), a.v.clone()) for a in arenas]
+                tape.replay()
+                torch.cuda.synchronize()
+                for arena, (p0, m0, v0) in zip(arenas, before):
+                    assert arena.step == step
+                    table = arena.muon_table()
+                    pr, mr, vr = muon_plain(p0, arena.grads, m0, v0, table, 2e-4, 0.9, True, 0.01, 0.5, 0.999, 1e-8, step)
+                    for e in table:
+                        at = slice(int(e["off"]), int(e["off"]) + int(e["taps"]) * int(e["rows"]) * int(e["cols"]))
+                        a, r = arena.params[at].double() - p0[at].double(), pr[at] - p0[at].double()
+                        # gradients of a real network are far from Gaussian: the products' derived bound for the matrices
+                        tol = (1.5 * NS[0] ** 5 * 2.0 ** -20 if e["kind"] == 0 else 0.0) + 64 * U
+                        assert float(r.norm()) > 0
+                        assert float((a - r).norm()) <= tol * float(r.norm()) + 2 * U * float(pr[at].norm()) + 2 * U * float(p0[at].norm()), tuple(e)
+                    assert bool(((arena.m.double() - mr).abs() <= 4 * U * (m0.double().abs() + arena.grads.double().abs())).all())
+                    if precision == 3:
+                        for k in arena.keys:
+                            at = slice(arena.off[k], arena.off[k] + arena.numel[k])
+                            assert torch.equal(arena.params_bf16[at], arena.params[at].bfloat16())
+        finally:
+            tape.close()
+    finally:
+        E.PRECISION = was
