@@ -367,13 +367,13 @@ int pg_adam_ex(float* p, const float* g, const void* g_bf16, float* m, float* v,
 
 /* ---- matrix optimiser
  * Orthogonalisation by Newton-Schulz products: out = X_steps, X_0 = x / (|x|_F + eps), X_{k+1} = (aI + bA + cA^2) X_k, A = X_k X_k^T
- * on the short side, (a, b, c) = (3.4445, -4.7750, 2.0315): the singular values of x go to within 0.68 .. 1.21.  `batch` matrices of
- * rows x cols, row strides ldx / ldo, matrix strides x_batch / out_batch (elements); x and out fp32 or bf16 each (x may be read
- * by several matrices, out must not overlap itself or x).  Products have the accuracy of fp32 ones whatever the types (about 1e-6 of the
- * result) for rows of the short side whose size is at least 1e-4 of the largest; a smaller one, r of the largest, is off by about
- * 5e-11 / r of itself (6e-6 at r = 1e-5, 5e-5 at 1e-6).  A matrix with an infinity or NaN gives NaN, without effect on the others; a zero
- * matrix gives zeros.  steps 1..32, eps > 0, at most 2^31 - 1
- * elements a matrix, counted with both sides rounded up to 64.
+ * on the short side, (a, b, c) = (3.4445, -4.7750, 2.0315): five steps take the singular values of x from about 2e-3 |x|_F on to within
+ * 0.68 .. 1.21, a smaller one to 485 times its share of |x|_F.  `batch` matrices of rows x cols, row strides ldx / ldo,
+ * matrix strides x_batch / out_batch (elements); x and out fp32 or bf16 each (x may be read by several matrices, out must not overlap
+ * itself or x).  Products have the accuracy of fp32 ones whatever the types (about 1e-6 of the result) for rows and columns whose size is
+ * at least 1e-4 of the largest; a smaller row of the short side, r of the largest, is off by about 5e-11 / r of itself (6e-6 at r = 1e-5,
+ * 5e-5 at 1e-6), a column of the long side by 1e-12 sqrt(long side) / r.  A matrix with an infinity or NaN gives NaN, without effect on the
+ * others; a zero matrix gives zeros.  steps 1..32, eps > 0, at most 2^31 - 1 elements a matrix, counted with both sides rounded up to 64.
  * The workspace (pg_orthogonalise_workspace bytes, 256-byte aligned; -1: sizes out of range) is the call's until its work is done.  */
 int64_t pg_orthogonalise_workspace(int64_t batch, int64_t rows, int64_t cols);
 int pg_orthogonalise(const void* x, int32_t x_is_bf16, int64_t batch, int64_t rows, int64_t cols, int64_t x_batch, int64_t ldx,

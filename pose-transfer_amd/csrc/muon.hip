@@ -19,7 +19,7 @@
 // lies near fp16's end: X0's largest element at 2^14 .. 2^15; |G|, |Q G| <= 1.5, |Q| <= 3.45 and |P| <= 3.45^3 = 41 bound the others.
 // Elements keep 22 bits down to 2^-18 of the largest and 2^-40 of it behind that.  A row that is a fraction r of the others comes out
 // with an error of about max(1e-6, 5e-11 / r) of itself (128 x 1152: 7e-7 at r = 1e-4, 6e-6 at 1e-5, 5e-5 at 1e-6; the limit is
-// 2^-40 in G); fp32 products keep 1e-6.  With the mean square at 1 instead of the largest element at 2^14: 1.7e-4, 1.8e-3, 1.7e-2.
+// 2^-40 in G), a column of the long side (n of them) with about 1e-12 sqrt(n) / r (the planes between stages); fp32 products keep 1e-6.  With the mean square at 1 instead of the largest element at 2^14: 1.7e-4, 1.8e-3, 1.7e-2.
 // A bf16 input (8 bits) is one fp16 value exactly down to 2^-32 of the largest, behind that to 2^-40 of it: one plane.
 //
 // Layout.  A matrix is stored by the caller as [taps][rows][cols] with row and tap strides (a packed convolution weight is one matrix
@@ -155,7 +155,7 @@ __device__ __forceinline__ float ns_grad(const NsStep& s, long i) { return (s.gb
 __device__ __forceinline__ float ns_update(const NsStep& s, float g, float m1) { return s.nesterov ? (1.f - s.mu) * g + s.mu * m1 : m1; }
 
 // one workgroup = k0_elems consecutive elements of a tensor; 28 bytes / element for Adam's, 12 for a matrix's: HBM-bound (77 M elements of
-// 20 matrices: 177 us, 5.2 TB/s; 2.8 M: 12 us)
+// 20 matrices: 177 us, 5.2 TB/s; 2.8 M: 13 us)
 __global__ __launch_bounds__(256) void muon_momentum_kernel(const NsGroup gr, const NsStep s, NsNorm* sq) {
   __shared__ NsNorm red[4];
   __shared__ double bc[2];
@@ -325,8 +325,8 @@ __device__ __forceinline__ int ns_gap(const NsUnit& u, int stage) { return max(0
 __device__ __forceinline__ float ns_value(const NsUnit& u, int stage) { return stage == 0 ? u.c : ns_pow2(-15 - ns_gap(u, stage)); }
 
 // every workgroup joins its matrix's partial sums of squares itself (at most 1024); the first one publishes
-// the matrix's units.  12 bytes / element from fp32 pairs (m', g), HBM-bound: 211 us for 77 M
-// elements (4.4 TB/s); 14 us for 512 x 24576 bf16 (6 bytes)
+// the matrix's units.  12 bytes / element from fp32 pairs (m', g), HBM-bound: 212 - 215 us for 77 M
+// elements (4.3 TB/s); 12 us for 512 x 24576 bf16 (6 bytes)
 template <int SRC>
 __global__ __launch_bounds__(256) void ns_split_kernel(const NsGroup gr, const void* x, const NsStep s, const NsNorm* sq, float eps,
                                                        NsUnit* unit, _Float16* ws) {
@@ -541,8 +541,8 @@ __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
 
 // G = X X^T over one slice of the long side: fp32 partial tiles, in the order of the accumulators (one float4 = four rows of a column).
 // 128 x 128 tiles of the lower triangle, two workgroups per CU; the long side in as many slices as run at once.  The generator's 20 matrices (up to
-// 512 x 24576) take 201 - 212 us, 512 x 24576 alone 29 us (two planes) and 16 us (bf16: one): MFMA-bound with operands from L2.  Where few slices run (16 x
-// 770 x 189: 144 workgroups, 11 - 13 us) it is launch, first transfer and the partial tiles' way out; more stages or slices gave nothing.
+// 512 x 24576) take 202 - 214 us, 512 x 24576 alone 29 us (two planes) and 16 us (bf16: one).  Bound by power: the counters show the MFMAs busy for 47 % of
+// the cycles, and where the chip rests between launches the generator's take 153 us, at 2.0 GHz.  Where few slices run (16 x 770 x 189: 144 workgroups, 11 - 13 us) it is launch, first transfer and the partial tiles' way out; more stages or slices gave nothing.
 template <int PL>
 __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int total, int grp, const _Float16* ws, float* part) {
   typedef NtCore<GT, PL, 2> Core;
@@ -571,8 +571,8 @@ __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int t
             make_float4(c.acc[i][j][4 * q], c.acc[i][j][4 * q + 1], c.acc[i][j][4 * q + 2], c.acc[i][j][4 * q + 3]);
 }
 
-// join of the slices, in order; both triangles of G from the lower one.  One workgroup = one 32 x 32 block, a float4 per thread: 4 - 6 us, mostly
-// launch (12 us for the generator's 20 matrices)
+// join of the slices, in order; both triangles of G from the lower one.  One workgroup = one 32 x 32 block, a float4 per thread: 4 - 7 us, mostly
+// launch (11 - 13 us for the generator's 20 matrices)
 __global__ __launch_bounds__(256) void ns_gram_join_kernel(const NsGroup gr, const float* part, const NsUnit* unit, int stage, _Float16* ws) {
   const NsRef r = ns_find<F_JOIN>(gr, blockIdx.x);
   const NsMat& m = r.m;
@@ -817,8 +817,9 @@ __device__ __forceinline__ void fetch_apply(unsigned pa, unsigned pb0, unsigned 
 }
 
 // A tile is 128 rows x 128 columns, 8 waves (2 x 4) of 64 x 32; K steps of 16 through three stages: 48 KB, three workgroups per CU, so that reads,
-// products and epilogues of different waves run under each other.  MFMA- and power-bound: 312 and 320 us for the generator's two
-// products (128 x 256 tiles, 4 waves of 128 x 64: 302 and 331 us), 512 x 24576 36 us (bf16 X) and 44 us (37 and 47 us), the discriminator's 17 and 18 us (29 and 35 us: 88 tiles).
+// products and epilogues of different waves run under each other.  Bound by power (MFMAs busy for 44 - 47 % of the cycles; after a rest 257 and
+// 273 us at 1.9 GHz): 310 - 320 us for each of the generator's two products (128 x 256 tiles, 4 waves of 128 x 64: 302 and 331 us), 512 x 24576 35 us (bf16 X)
+// and 44 us (37 and 47 us), the discriminator's 18 and 19 us (29 and 35 us: 88 tiles).
 __device__ __forceinline__ void muon_update(const NsStep& s, long at, float keep, float step, float o) {
   const float p = s.p[at] * keep - step * o;
   s.p[at] = p;

@@ -140,8 +140,8 @@ def rms_norm_bwd(dy, h, rstd, gamma, dh=None):
 
 def orthogonalise(x, steps=5, eps=1e-7, out_dtype=None):
     """The orthogonal factor of each matrix of x ([rows, cols] or [batch, rows, cols], fp32 or bf16) by `steps` Newton-Schulz
-    products; out_dtype fp32 or bf16 (default: x's).  Accurate as fp32 products are, but for rows of the short side below 1e-4 of the
-    largest: one of r is off by about 5e-11 / r of itself."""
+    products; out_dtype fp32 or bf16 (default: x's).  Accurate as fp32 products are, but for rows and columns below 1e-4 of the
+    largest: a row of the short side of r is off by about 5e-11 / r of itself, a column of the long one by 1e-12 sqrt(long side) / r."""
     _need(torch.is_tensor(x) and x.is_cuda and x.dtype in _IO, "orthogonalise: x must be an fp32 or bf16 tensor on the GPU")
     _need(x.dim() in (2, 3), "orthogonalise: [rows, cols] or [batch, rows, cols] expected")
     out_dtype = x.dtype if out_dtype is None else out_dtype

@@ -8,7 +8,9 @@ Tolerances.  U = 2^-24, EPS the half step of the stored type.
       ten times outside.)
   rows much smaller than the others: the m x m factor P of a stage is off by an absolute 2^-30 at most (G by 2^-40, Q by 4.8 times that
       and 2^-39 of its own, three of them multiplied: 36 times, then P's own 2^-35 twice), so a row by 2^-30 sqrt(m) |X|_2, |X|_2 <= 1; the
-      row itself, r of the others, grows from r / sqrt(m) to 41 times that: relative 2^-30 m / (41 r)."""
+      row itself, r of the others, grows from r / sqrt(m) to 41 times that: relative 2^-30 m / (41 r).
+  columns of the long side (n of them) much smaller than the others: the planes between stages hold 2^15 X to an absolute 2^-25, so a
+      column is off by 2^-40 sqrt(m); its own size is at least 0.3 r sqrt(m / n) (0.3: a singular value after the first stage)."""
 import math
 
 import numpy as np
@@ -66,6 +68,24 @@ def test_orthogonalise_keeps_small_rows(shape, dtype):
     dim = 1 if tall else 2
     err = (got - ref).norm(dim=dim) / ref.norm(dim=dim)
     tol = BASE + 2.0 ** -30 * short / (41 * size.double())
+    assert bool((err <= tol).all()), (err[:, at].max(0).values.tolist(), tol[at].tolist(), float(err.max()))
+
+
+@pytest.mark.parametrize("shape", ORTHO)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_orthogonalise_keeps_small_columns(shape, dtype):
+    """columns (of the long side) 1e-3 to 1e-7 of the others"""
+    x = rnd(4, *shape)
+    tall = shape[1] > shape[2]
+    size = torch.ones(max(shape[1:]), device="cuda")
+    at = [0, 7, 17, 23, 38]
+    for i, r in zip(at, (1e-3, 1e-4, 1e-5, 1e-6, 1e-7)):
+        size[i] = r
+    x = (x * (size[:, None] if tall else size)).to(dtype)
+    got, ref = ops().orthogonalise(x, out_dtype=torch.float32).double(), ortho_ref(x)
+    dim = 2 if tall else 1
+    err = (got - ref).norm(dim=dim) / ref.norm(dim=dim)
+    tol = BASE + 2.0 ** -40 * math.sqrt(size.numel()) / (0.3 * size.double())
     assert bool((err <= tol).all()), (err[:, at].max(0).values.tolist(), tol[at].tolist(), float(err.max()))
 
 
@@ -281,13 +301,15 @@ def test_rms_norm_module_of_a_channel_slice():
 
 # ------------------------------------------------------------------------------------------------ the trainer's recorded step
 @pytest.mark.parametrize("precision", [0, 3])
-def test_replayed_muon_step_against_the_definition(precision):
+@pytest.mark.parametrize("how", ["tape", "graph"])
+def test_replayed_muon_step_against_the_definition(precision, how):
     """a replayed iteration's optimiser launches: each record's displacement against the 64-bit step on the arena's own gradients, at the
     step number that the device counter gives, twice; a replay that left them out, or took them twice, is off by its whole size"""
     from types import SimpleNamespace
 
     from pose_transfer_amd.models.pose_gan import DeformablePose_GAN
     from pose_transfer_amd.runtime import engine as E
+    from pose_transfer_amd.runtime.graph import GraphedIteration
     from pose_transfer_amd.runtime.tape import TapedIteration
     from pose_transfer_amd.utils import synth
     was, E.PRECISION = E.PRECISION, precision
@@ -298,12 +320,16 @@ def test_replayed_muon_step_against_the_definition(precision):
         model = DeformablePose_GAN(opt, device="cuda:0")
         b = [torch.from_numpy(np.ascontiguousarray(a)).cuda() for a in synth.batch(1, "muon/T", 2, 18, 64, 64)]
         b = [b[0], b[1], b[2].float().contiguous(), b[3]]
-        tape = TapedIteration(model, [b, b, b], dict(vars(opt)), warmup=1)               # one eager iteration, one recorded
+        # one eager iteration and one that is recorded and runs (tape), or two eager ones before the capture (graph)
+        if how == "tape":
+            replay = TapedIteration(model, [b, b, b], dict(vars(opt)), warmup=1)
+        else:
+            replay = GraphedIteration(model, [b, b, b], dict(vars(opt)), warmup=2)
         try:
             arenas = (model.disc.arena, model.gen.arena)
             for step in (3, 4):
                 before = [(a.params.clone(), a.m.clone(), a.v.clone()) for a in arenas]
-                tape.replay()
+                replay.replay()
                 torch.cuda.synchronize()
                 for arena, (p0, m0, v0) in zip(arenas, before):
                     assert arena.step == step
@@ -322,6 +348,6 @@ def test_replayed_muon_step_against_the_definition(precision):
                             at = slice(arena.off[k], arena.off[k] + arena.numel[k])
                             assert torch.equal(arena.params_bf16[at], arena.params[at].bfloat16())
         finally:
-            tape.close()
+            replay.close()
     finally:
         E.PRECISION = was
