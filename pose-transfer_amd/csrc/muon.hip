@@ -19,7 +19,8 @@
 // lies near fp16's end: X0's largest element at 2^14 .. 2^15; |G|, |Q G| <= 1.5, |Q| <= 3.45 and |P| <= 3.45^3 = 41 bound the others.
 // Elements keep 22 bits down to 2^-18 of the largest and 2^-40 of it behind that.  A row that is a fraction r of the others comes out
 // with an error of about max(1e-6, 5e-11 / r) of itself (128 x 1152: 7e-7 at r = 1e-4, 6e-6 at 1e-5, 5e-5 at 1e-6; the limit is
-// 2^-40 in G), a column of the long side (n of them) with about 1e-12 sqrt(n) / r (the planes between stages); fp32 products keep 1e-6.  With the mean square at 1 instead of the largest element at 2^14: 1.7e-4, 1.8e-3, 1.7e-2.
+// 2^-40 in G), a column of the long side (n of them) with about 1e-12 sqrt(n) / r (the planes between stages); fp32 products keep 1e-6.
+// With the mean square at 1 instead of the largest element at 2^14, rows came out at 1.7e-4, 1.8e-3 and 1.7e-2.
 // A bf16 input (8 bits) is one fp16 value exactly down to 2^-32 of the largest, behind that to 2^-40 of it: one plane.
 //
 // Layout.  A matrix is stored by the caller as [taps][rows][cols] with row and tap strides (a packed convolution weight is one matrix
@@ -542,7 +543,8 @@ __device__ __forceinline__ void tri(int t, int& bi, int& bj) {
 // G = X X^T over one slice of the long side: fp32 partial tiles, in the order of the accumulators (one float4 = four rows of a column).
 // 128 x 128 tiles of the lower triangle, two workgroups per CU; the long side in as many slices as run at once.  The generator's 20 matrices (up to
 // 512 x 24576) take 202 - 214 us, 512 x 24576 alone 29 us (two planes) and 16 us (bf16: one).  Bound by power: the counters show the MFMAs busy for 47 % of
-// the cycles, and where the chip rests between launches the generator's take 153 us, at 2.0 GHz.  Where few slices run (16 x 770 x 189: 144 workgroups, 11 - 13 us) it is launch, first transfer and the partial tiles' way out; more stages or slices gave nothing.
+// the cycles, and where the chip rests between launches the generator's take 153 us, at 2.0 GHz.  Where few slices
+// run (16 x 770 x 189: 144 workgroups, 11 - 13 us) it is launch, first transfer and the partial tiles' way out; more stages or slices gave nothing.
 template <int PL>
 __global__ __launch_bounds__(256, 2) void ns_gram_kernel(const NsGroup gr, int total, int grp, const _Float16* ws, float* part) {
   typedef NtCore<GT, PL, 2> Core;
